@@ -97,6 +97,15 @@ class TpShare(C.Structure):
                                                                       "attn_col0", "attn_cols")]
 
 
+class PagedCache(C.Structure):
+    _fields_ = [("struct_size", C.c_size_t), ("keys", C.c_void_p), ("values", C.c_void_p), ("page_table", C.c_void_p)] + [
+        (n, C.c_int32) for n in ("n_pages", "page_size", "n_sequences", "max_pages", "n_head_kv", "head_dim")]
+
+
+class Rope(C.Structure):
+    _fields_ = [("struct_size", C.c_size_t), ("base", C.c_double), ("neox", C.c_int32), ("n_axes", C.c_int32), ("sections", C.c_int32 * 4)]
+
+
 TOKEN_CALLBACK = C.CFUNCTYPE(C.c_int32, C.c_int32, C.c_void_p)
 
 # name -> (restype, argtypes); every symbol include/dooms_cuda.h declares
@@ -179,6 +188,15 @@ SIGNATURES = {
     "dooms_cuda_argmax_noalloc": (C.c_int32, [C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p]),
     "dooms_cuda_attention_scratch_bytes": (C.c_int64, [C.c_int32, C.c_int32, C.c_int32]),
     "dooms_cuda_attention_decode": (C.c_int32, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_void_p]),
+    "dooms_cuda_rope_store_paged": (C.c_int32, [C.POINTER(PagedCache), C.POINTER(Rope), C.c_void_p, C.c_int64, C.c_int32, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32,
+                                                C.c_void_p, C.c_void_p]),
+    "dooms_cuda_attention_paged_scratch_bytes": (C.c_int64, [C.c_int32, C.c_int32, C.c_int32]),
+    "dooms_cuda_attention_paged": (C.c_int32, [C.POINTER(PagedCache), C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p, C.c_int32, C.c_int32, C.c_float,
+                                               C.c_void_p, C.c_int64, C.c_void_p]),
+    "dooms_cuda_attention_prompt_paged": (C.c_int32, [C.POINTER(PagedCache), C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32, C.c_int32, C.c_int32, C.c_float,
+                                                      C.c_void_p, C.c_int64, C.c_void_p]),
+    "dooms_cuda_sample_rows": (C.c_int32, [C.c_void_p, C.c_int64, C.c_int32, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
+                                           C.c_void_p]),
     "dooms_cuda_tp_share": (C.c_int32, [C.POINTER(LlamaConfig), C.c_int32, C.c_int32, C.POINTER(TpShare)]),
     "dooms_cuda_tp_share_blocks": (C.c_int32, [C.POINTER(LlamaConfig), C.c_int32, C.c_int32, C.c_int64, C.c_int64, C.POINTER(TpShare)]),
     "dooms_cuda_nccl_unique_id": (C.c_int32, [C.c_char_p, C.c_void_p]),

@@ -3,8 +3,11 @@
 
 #include <cuda_runtime.h>
 
+#include <algorithm>
+#include <cmath>
 #include <cstddef>
 #include <cstring>
+#include <initializer_list>
 #include <memory>
 #include <mutex>
 #include <string>
@@ -152,6 +155,42 @@ void * g_argmax_noalloc_ptr[64];      // the array's device address, per device,
 std::mutex g_argmax_noalloc_mutex;
 
 bool matrix_dtype(int32_t dt) { return dt == DOOMS_F16 || dt == DOOMS_Q4_0 || dt == DOOMS_Q5_0 || dt == DOOMS_Q8_0 || dt == DOOMS_Q4_K || dt == DOOMS_Q6_K; }
+
+// Every pointer has to be memory that kernels of the current device can use: a pointer of another device, or plain host memory, would fault in the kernel.
+int32_t check_device(const char * what, std::initializer_list<const void *> pointers) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) { (void)cudaGetLastError(); return fail(DOOMS_UNSUPPORTED, std::string(what) + ": no CUDA device"); }
+    for (const void * p : pointers) {
+        if (!p) continue;
+        cudaPointerAttributes at{};
+        const cudaError_t e = cudaPointerGetAttributes(&at, p);
+        if (e != cudaSuccess) { (void)cudaGetLastError(); return fail(DOOMS_UNSUPPORTED, std::string(what) + ": " + cudaGetErrorString(e)); }
+        const bool here = at.type == cudaMemoryTypeManaged || (at.type == cudaMemoryTypeDevice && at.device == dev) || (at.type == cudaMemoryTypeHost && at.devicePointer == p);
+        if (!here) return fail(DOOMS_INVALID_ARGUMENT, std::string(what) + ": a pointer is not memory of the current device");
+    }
+    return DOOMS_OK;
+}
+
+bool aligned16(const void * p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+constexpr int kMostGroup = 64;      // query heads per key / value head
+int32_t check_paged(const char * what, const dooms_cuda_paged_cache * c, int32_t n_head, cuda::PagedCache * out) {
+    int32_t code = DOOMS_OK;
+    if (!struct_ok(c, "cache", &code)) return code;
+    if (c->struct_size < sizeof *c || !c->keys || !c->values || !c->page_table || !aligned16(c->keys) || !aligned16(c->values) || c->n_pages < 1 || c->n_sequences < 1 ||
+        c->max_pages < 1 || c->n_head_kv < 1 || c->page_size < 16 || c->page_size > 65536 || (c->page_size & (c->page_size - 1)) != 0) {
+        return fail(DOOMS_INVALID_ARGUMENT, std::string(what) + ": cache: a NULL or unaligned pointer, a count below 1, or a page_size that is not a power of two in [16, 65536]");
+    }
+    if (c->head_dim != 64 && c->head_dim != 128) return fail(DOOMS_UNSUPPORTED, std::string(what) + ": head_dim has to be 64 or 128");
+    if (n_head < 1 || n_head % c->n_head_kv != 0 || n_head / c->n_head_kv > kMostGroup) {
+        return fail(DOOMS_INVALID_ARGUMENT, std::string(what) + ": n_head has to be a multiple of n_head_kv, at most " + std::to_string(kMostGroup) + " times");
+    }
+    if (int64_t(c->n_pages) * c->page_size > INT32_MAX || int64_t(n_head) * c->head_dim > (1 << 20)) {
+        return fail(DOOMS_INVALID_ARGUMENT, std::string(what) + ": more than 2^31 - 1 positions in the pool, or rows of more than 2^20 values");
+    }
+    *out = {c->keys, c->values, c->page_table, c->n_pages, c->page_size, c->n_sequences, c->max_pages, c->n_head_kv, c->head_dim};
+    return DOOMS_OK;
+}
 
 }  // namespace
 
@@ -777,6 +816,7 @@ DOOMS_CUDA_API int32_t dooms_cuda_kernel_status(void * stream, int32_t * flag) {
     if (err) *err = 0;
     if (flag) *flag = seen;
     if (seen == 0) return DOOMS_OK;
+    if (seen == cuda::kErrorPaged) return fail(DOOMS_INTERNAL, "a page id, sequence, position or length of a paged cache call was out of range (flag 8); the output of its row is not valid");
     return fail(DOOMS_INTERNAL, "a kernel gave up a bounded wait (flag " + std::to_string(seen) + (seen == 2 ? ": matmul" : seen == 4 ? ": matvec / gate_up tensor copy" : "") +
                                     "); its output is not valid");
 }
@@ -845,6 +885,92 @@ DOOMS_CUDA_API int32_t dooms_cuda_attention_decode(const float * d_q, const void
     const int splits = cuda::attention_splits(n_head, n_keys);
     return launch_result(cuda::launch_attention_decode(d_q, d_kc, d_vc, d_out, static_cast<float *>(d_scratch), nullptr, nullptr, n_keys, splits, s,
                                                        static_cast<cudaStream_t>(stream)), "attention_decode");
+}
+
+DOOMS_CUDA_API int32_t dooms_cuda_rope_store_paged(const dooms_cuda_paged_cache * cache, const dooms_cuda_rope * rope, const float * d_qkv, int64_t qkv_stride, int32_t n_head,
+                                                   int32_t n_rows, const int32_t * d_sequence, const int32_t * d_at, const int32_t * d_positions, int32_t q_dtype, void * d_q,
+                                                   void * stream) {
+    cuda::PagedCache c{};
+    int32_t code = check_paged("rope_store_paged", cache, n_head, &c);
+    if (code != DOOMS_OK || !struct_ok(rope, "rope", &code)) return code;
+    if (rope->struct_size < sizeof *rope || !(rope->base > 1.0) || !(rope->base < 1e300) || rope->n_axes < 1 || rope->n_axes > 4) {
+        return fail(DOOMS_INVALID_ARGUMENT, "rope_store_paged: rope: base > 1 and 1 to 4 axes are required");
+    }
+    cuda::RopeSections r{rope->base, rope->neox != 0, rope->n_axes, {0, 0, 0, 0}};
+    int64_t pairs = 0;
+    for (int x = 0; x < rope->n_axes; x++) {
+        if (rope->sections[x] < 0) return fail(DOOMS_INVALID_ARGUMENT, "rope_store_paged: rope: a negative section");
+        pairs += r.sections[x] = rope->sections[x];
+    }
+    if (pairs != c.head_dim / 2) return fail(DOOMS_INVALID_ARGUMENT, "rope_store_paged: rope: the sections have to add up to head_dim / 2");
+    if (q_dtype != DOOMS_F32 && q_dtype != DOOMS_F16) return fail(DOOMS_UNSUPPORTED, "rope_store_paged: q_dtype has to be f32 or f16");
+    const int64_t row = (int64_t(n_head) + 2 * int64_t(c.n_head_kv)) * c.head_dim;
+    if (n_rows == 0) return DOOMS_OK;
+    if (!d_qkv || !d_sequence || !d_at || !d_positions || !d_q || n_rows < 0 || qkv_stride < row || qkv_stride % 4 != 0 || !aligned16(d_qkv) || !aligned16(d_q)) {
+        return fail(DOOMS_INVALID_ARGUMENT, "rope_store_paged: a NULL or unaligned pointer, a negative n_rows, or a qkv_stride that is no multiple of 4 or shorter than a row");
+    }
+    code = check_device("rope_store_paged", {c.keys, c.values, c.page_table, d_qkv, d_sequence, d_at, d_positions, d_q});
+    if (code != DOOMS_OK) return code;
+    return launch_result(cuda::launch_rope_store_paged(c, r, d_qkv, qkv_stride, n_head, n_rows, d_sequence, d_at, d_positions, d_q, q_dtype == DOOMS_F16, kernel_error_word(),
+                                                       static_cast<cudaStream_t>(stream)), "rope_store_paged");
+}
+
+DOOMS_CUDA_API int64_t dooms_cuda_attention_paged_scratch_bytes(int32_t n_head, int32_t n_head_kv, int32_t head_dim) {
+    if (n_head_kv < 1 || n_head < 1 || n_head % n_head_kv != 0 || n_head / n_head_kv > kMostGroup || (head_dim != 64 && head_dim != 128)) return 0;
+    return int64_t(std::max(cuda::attention_paged_scratch_bytes(n_head, n_head_kv, head_dim), cuda::attention_prompt_scratch_bytes(n_head, n_head_kv, head_dim)));
+}
+
+DOOMS_CUDA_API int32_t dooms_cuda_attention_paged(const dooms_cuda_paged_cache * cache, int32_t dtype, const void * d_q, const int32_t * d_sequence, const int32_t * d_lengths,
+                                                  int32_t max_length, void * d_out, int32_t n_head, int32_t n_rows, float scale, void * d_scratch, int64_t scratch_bytes,
+                                                  void * stream) {
+    cuda::PagedCache c{};
+    int32_t code = check_paged("attention_paged", cache, n_head, &c);
+    if (code != DOOMS_OK) return code;
+    if (dtype != DOOMS_F32 && dtype != DOOMS_F16) return fail(DOOMS_UNSUPPORTED, "attention_paged: dtype has to be f32 or f16");
+    if (n_rows == 0) return DOOMS_OK;
+    if (!d_q || !d_sequence || !d_lengths || !d_out || !d_scratch || n_rows < 0 || max_length < 0 || !aligned16(d_q) || !aligned16(d_out) || !aligned16(d_scratch) ||
+        !(scale >= 0.f) || !(scale < 1e30f)) {
+        return fail(DOOMS_INVALID_ARGUMENT, "attention_paged: a NULL or unaligned pointer, a negative size, or a scale that is negative or not finite");
+    }
+    if (scratch_bytes < dooms_cuda_attention_paged_scratch_bytes(n_head, c.n_head_kv, c.head_dim)) return fail(DOOMS_RESOURCE_EXHAUSTED, "attention_paged: the scratch is too small");
+    code = check_device("attention_paged", {c.keys, c.values, c.page_table, d_q, d_sequence, d_lengths, d_out, d_scratch});
+    if (code != DOOMS_OK) return code;
+    return launch_result(cuda::launch_attention_paged(c, d_q, d_out, dtype == DOOMS_F16, n_head, n_rows, d_sequence, d_lengths, max_length,
+                                                      scale > 0.f ? scale : 1.f / std::sqrt(float(c.head_dim)), d_scratch, kernel_error_word(), static_cast<cudaStream_t>(stream)),
+                         "attention_paged");
+}
+
+DOOMS_CUDA_API int32_t dooms_cuda_attention_prompt_paged(const dooms_cuda_paged_cache * cache, const void * d_q, const int32_t * d_sequence, const int32_t * d_start,
+                                                         const int32_t * d_lengths, void * d_out, int32_t n_head, int32_t n_prompts, int32_t n_rows, float scale,
+                                                         void * d_scratch, int64_t scratch_bytes, void * stream) {
+    cuda::PagedCache c{};
+    int32_t code = check_paged("attention_prompt_paged", cache, n_head, &c);
+    if (code != DOOMS_OK) return code;
+    if (n_rows == 0 || n_prompts == 0) return DOOMS_OK;
+    if (!d_q || !d_sequence || !d_start || !d_lengths || !d_out || !d_scratch || d_q == d_out || n_rows < 0 || n_prompts < 0 || !aligned16(d_q) || !aligned16(d_out) ||
+        !aligned16(d_scratch) || !(scale >= 0.f) || !(scale < 1e30f)) {
+        return fail(DOOMS_INVALID_ARGUMENT, "attention_prompt_paged: a NULL or unaligned pointer, one buffer as input and output, a negative size, or a scale that is negative or not finite");
+    }
+    if (scratch_bytes < dooms_cuda_attention_paged_scratch_bytes(n_head, c.n_head_kv, c.head_dim)) return fail(DOOMS_RESOURCE_EXHAUSTED, "attention_prompt_paged: the scratch is too small");
+    code = check_device("attention_prompt_paged", {c.keys, c.values, c.page_table, d_q, d_sequence, d_start, d_lengths, d_out, d_scratch});
+    if (code != DOOMS_OK) return code;
+    return launch_result(cuda::launch_attention_prompt_paged(c, d_q, d_out, n_head, n_rows, n_prompts, d_sequence, d_start, d_lengths,
+                                                             scale > 0.f ? scale : 1.f / std::sqrt(float(c.head_dim)), d_scratch, kernel_error_word(),
+                                                             static_cast<cudaStream_t>(stream)), "attention_prompt_paged");
+}
+
+DOOMS_CUDA_API int32_t dooms_cuda_sample_rows(const float * d_logits, int64_t stride, int32_t rows, int32_t n, const float * d_temperature, const int32_t * d_top_k,
+                                              const float * d_top_p, const float * d_min_p, const float * d_uniform, int32_t * d_tokens, float * d_probability, void * stream) {
+    if (rows == 0) return DOOMS_OK;
+    if (!d_logits || !d_uniform || !d_tokens || rows < 0 || n < 1 || stride < n) {
+        return fail(DOOMS_INVALID_ARGUMENT, "sample_rows: a NULL pointer, a negative count of rows, no logits, or a stride shorter than a row");
+    }
+    if (n > cuda::sample_rows_most()) return fail(DOOMS_UNSUPPORTED, "sample_rows: rows of at most " + std::to_string(cuda::sample_rows_most()) + " logits");
+    if (rows > (1 << 24)) return fail(DOOMS_INVALID_ARGUMENT, "sample_rows: at most 2^24 rows");
+    const int32_t code = check_device("sample_rows", {d_logits, d_temperature, d_top_k, d_top_p, d_min_p, d_uniform, d_tokens, d_probability});
+    if (code != DOOMS_OK) return code;
+    return launch_result(cuda::launch_sample_rows(d_logits, stride, rows, n, d_temperature, d_top_k, d_top_p, d_min_p, d_uniform, d_tokens, d_probability,
+                                                  static_cast<cudaStream_t>(stream)), "sample_rows");
 }
 
 DOOMS_CUDA_API int32_t dooms_cuda_tp_share_blocks(const dooms_llama_config * config, int32_t tp_rank, int32_t tp_size, int64_t attn_block, int64_t ffn_block,

@@ -273,5 +273,31 @@ cudaError_t launch_gemm_tc_rows16(const void * W16, const void * W2_16, const Te
                                   int64_t y_stride, int64_t y16_stride, uint32_t flags, int32_t * error, cudaStream_t stream, int k_splits = 1, int64_t split_stride = 0);
 cudaError_t launch_add_shares(float * x, const float * shares, int k_splits, int64_t n, int64_t split_stride, cudaStream_t stream);
 
+// ---- a serving step over a key / value cache in pages ----
+// Pools of f16 [n_pages][page_size][n_head_kv][head_dim] (page_size a power of two from 16, head_dim 64 or 128) and the page ids of every sequence. Ids, sequences,
+// positions and lengths are read on the device; one that is out of range is not followed: its row is skipped and *error becomes 8.
+constexpr int kErrorPaged = 8;
+struct PagedCache {
+    void * keys, * values;
+    const int32_t * page_table;       // [n_sequences][max_pages]
+    int n_pages, page_size, n_sequences, max_pages, n_head_kv, head_dim;
+};
+struct RopeSections { double base; int neox, n_axes, sections[4]; };      // rotary pairs per axis, in order; together head_dim / 2
+// rope_store_paged.cu. qkv: n_rows rows (stride floats apart, a multiple of 4) of n_head query heads, then the key and the value heads; sequence[r] < 0: an idle row.
+cudaError_t launch_rope_store_paged(const PagedCache & cache, const RopeSections & rope, const float * qkv, int64_t stride, int n_head, int n_rows, const int32_t * sequence,
+                                    const int32_t * at, const int32_t * positions, void * q_out, bool half_q, int * error, cudaStream_t stream);
+// attention_paged.cu, one new token per row. q and out: [n_rows][n_head][head_dim], f16 or f32.
+size_t attention_paged_scratch_bytes(int n_head, int n_head_kv, int head_dim);
+cudaError_t launch_attention_paged(const PagedCache & cache, const void * q, void * out, bool half_io, int n_head, int n_rows, const int32_t * sequence, const int32_t * lengths,
+                                   int max_length, float scale, void * scratch, int * error, cudaStream_t stream);
+// attention_prompt_paged.cu. q and out f16 [n_rows][n_head][head_dim]; prompt i has the rows start[i] .. start[i + 1] - 1, the last positions of its sequence's lengths[i].
+size_t attention_prompt_scratch_bytes(int n_head, int n_head_kv, int head_dim);
+cudaError_t launch_attention_prompt_paged(const PagedCache & cache, const void * q, void * out, int n_head, int n_rows, int n_prompts, const int32_t * sequence,
+                                          const int32_t * start, const int32_t * lengths, float scale, void * scratch, int * error, cudaStream_t stream);
+// sample_rows.cu. n at most sample_rows_most().
+int sample_rows_most();
+cudaError_t launch_sample_rows(const float * logits, int64_t stride, int rows, int n, const float * temperature, const int32_t * top_k, const float * top_p, const float * min_p,
+                               const float * uniform, int32_t * tokens, float * probability, cudaStream_t stream);
+
 }  // namespace cuda
 }  // namespace dooms

@@ -222,7 +222,8 @@ DOOMS_CUDA_API int32_t dooms_cuda_matmul(int32_t dtype, const void * d_w, const 
                                          int32_t tokens, int64_t rows, int64_t cols, uint32_t flags, void * stream);
 /* No counterpart in the reference (Metal command buffers report their own errors). The matvec / gate_up / matmul kernels above wait for their tensor copies
  * and tensor-core stages with a limit; a wait that runs out sets a process-wide error word instead of hanging the GPU, and the kernel's output is then
- * not valid. This call waits for `stream`, reads the word into *flag (may be NULL; 0: none, 2: matmul, 4: matvec / gate_up) and clears it; it returns
+ * not valid. This call waits for `stream`, reads the word into *flag (may be NULL; 0: none, 2: matmul, 4: matvec / gate_up, 8: an entry of a paged cache call out of range,
+ * 16: a wait of attention_paged / attention_prompt_paged) and clears it; it returns
  * DOOMS_OK when the word was 0 and DOOMS_INTERNAL otherwise. */
 DOOMS_CUDA_API int32_t dooms_cuda_kernel_status(void * stream, int32_t * flag);
 /* norm_vec (llama_kernels.h:1272-1286): xn = x * rsqrt(mean(x^2) + eps) * gamma for `rows` rows of `cols`. */
@@ -242,6 +243,64 @@ DOOMS_CUDA_API int32_t dooms_cuda_argmax_noalloc(const float * d_logits, int64_t
 DOOMS_CUDA_API int64_t dooms_cuda_attention_scratch_bytes(int32_t n_head, int32_t head_dim, int32_t n_keys);
 DOOMS_CUDA_API int32_t dooms_cuda_attention_decode(const float * d_q, const void * d_kc, const void * d_vc, float * d_out, void * d_scratch, int32_t n_head,
                                                    int32_t n_head_kv, int32_t head_dim, int32_t n_keys, void * stream);
+
+/* ---- The parts of a serving step over a key / value cache in pages, on DEVICE pointers like the single kernels above. No counterpart in the reference, which
+ * keeps one contiguous cache (metal_llama_decoder.mm:560-590) and samples on the host (src/models/vlm/text_decoder.cpp:231-246).
+ * Every pointer is memory of the current device (or managed, or mapped host memory); anything else is refused with DOOMS_INVALID_ARGUMENT before a launch, as
+ * are NULL pointers and bad sizes. What only the device can read (page ids, sequences, positions, lengths) is checked there: an entry that is out of range is
+ * not followed, its row's output is not valid, and dooms_cuda_kernel_status then reports flag 8. Calls allocate nothing and may be captured. Calls that
+ * overlap on the GPU need scratch memory of their own; a scratch needs no initialization. ---- */
+/* keys / values: f16 [n_pages][page_size][n_head_kv][head_dim], 16-byte aligned. page_table: int32 [n_sequences][max_pages], the pages of each sequence in the
+ * order of its positions; entries past a sequence's last position are not read. page_size: a power of two, 16 to 65536; head_dim: 64 or 128 (others:
+ * DOOMS_UNSUPPORTED). A page may belong to several sequences as long as no call writes to it. The struct is host memory and read during the call. */
+typedef struct dooms_cuda_paged_cache {
+    size_t struct_size;
+    void * keys;
+    void * values;
+    const int32_t * page_table;
+    int32_t n_pages, page_size, n_sequences, max_pages, n_head_kv, head_dim;
+} dooms_cuda_paged_cache;
+/* Rotary positions: base > 1, pairs (i, i + head_dim / 2) with neox, (2i, 2i + 1) without (rotate_pair, llama_kernels.h:513-518), turned by position * base^(-2i / head_dim).
+ * n_axes 1 to 4: the first sections[0] pairs turn by the first axis' position, the next sections[1] by the second's (time, height, width of image and video
+ * rows); the sections add up to head_dim / 2. n_axes = 1 is the decoder's own rotation. */
+typedef struct dooms_cuda_rope {
+    size_t struct_size;
+    double base;
+    int32_t neox, n_axes;
+    int32_t sections[4];
+} dooms_cuda_rope;
+/* rope_store (llama_kernels.h:521-545) for rows of many sequences: of row r of d_qkv (n_head query heads, n_head_kv key heads, n_head_kv value heads of f32, rows
+ * qkv_stride floats apart, a multiple of 4; 16-byte aligned) the queries are turned into d_q [n_rows][n_head][head_dim] (q_dtype DOOMS_F32 or DOOMS_F16; 16-byte
+ * aligned, apart from d_qkv), keys (turned) and values are rounded to f16 and written to position d_at[r] of sequence d_sequence[r] (negative: an idle row, nothing
+ * of which is read or written). d_positions: int32 [n_axes][n_rows]. No position twice in one call. n_head: a multiple of n_head_kv, at most 64 times. */
+DOOMS_CUDA_API int32_t dooms_cuda_rope_store_paged(const dooms_cuda_paged_cache * cache, const dooms_cuda_rope * rope, const float * d_qkv, int64_t qkv_stride, int32_t n_head,
+                                                   int32_t n_rows, const int32_t * d_sequence, const int32_t * d_at, const int32_t * d_positions, int32_t q_dtype, void * d_q,
+                                                   void * stream);
+/* Bytes of scratch memory (16-byte aligned) that attention_paged and attention_prompt_paged work in, for any number of rows; 0: bad arguments. */
+DOOMS_CUDA_API int64_t dooms_cuda_attention_paged_scratch_bytes(int32_t n_head, int32_t n_head_kv, int32_t head_dim);
+/* attention_split + attention_combine (llama_kernels.h:860-929) for one new token of each of many sequences: row r of d_q [n_rows][n_head][head_dim] (turned) attends to
+ * the first d_lengths[r] positions of sequence d_sequence[r] (negative: an idle row, whose output is left as it is; length 0: zeros). d_q and d_out: dtype DOOMS_F32 or
+ * DOOMS_F16, 16-byte aligned; with f32 the products are as exact as f32 arithmetic. max_length: at least every length (a longer one is out of range); it may be generous.
+ * scale: of the scores; 0: 1 / sqrt(head_dim). */
+DOOMS_CUDA_API int32_t dooms_cuda_attention_paged(const dooms_cuda_paged_cache * cache, int32_t dtype, const void * d_q, const int32_t * d_sequence, const int32_t * d_lengths,
+                                                  int32_t max_length, void * d_out, int32_t n_head, int32_t n_rows, float scale, void * d_scratch, int64_t scratch_bytes,
+                                                  void * stream);
+/* attention_prefill<64 / 128> (llama_kernels.h:640-769) for the packed prompts of many sequences: d_q [n_rows][n_head][head_dim] f16; prompt i has rows d_start[i] to
+ * d_start[i + 1] - 1 (d_start: int32 [n_prompts + 1], not descending, d_start[0] >= 0, d_start[n_prompts] <= n_rows), which are the last positions of the d_lengths[i]
+ * that sequence d_sequence[i] (negative: an idle prompt) has: a prompt may go on behind what is cached, and its own keys and values are in the cache already. A row
+ * sees the positions up to its own; one that sees none (a prompt longer than its length) gives zeros. d_out [n_rows][n_head][head_dim] f16, apart from d_q; rows of no
+ * prompt are left as they are. Queries and probabilities enter the products as f16, as in the reference's tiles (:660, 708-713). */
+DOOMS_CUDA_API int32_t dooms_cuda_attention_prompt_paged(const dooms_cuda_paged_cache * cache, const void * d_q, const int32_t * d_sequence, const int32_t * d_start,
+                                                         const int32_t * d_lengths, void * d_out, int32_t n_head, int32_t n_prompts, int32_t n_rows, float scale,
+                                                         void * d_scratch, int64_t scratch_bytes, void * stream);
+/* One token per row of n logits (rows `stride` floats apart), as dooms_cuda_sample's chain picks it, from given random numbers d_uniform[r] in [0, 1): in the order (logit
+ * descending, index ascending) the first d_top_k[r] (0 or less: all), then the shortest run whose probability reaches d_top_p[r] (1 or more: all), then those of at
+ * least d_min_p[r] times the largest probability (0 or less: all), probabilities being those at temperature 1; then the first whose cumulative probability at temperature
+ * d_temperature[r] exceeds d_uniform[r]. At least one token is kept. temperature <= 0: the largest logit. A NaN is never picked, nor a logit of -inf; a row that has
+ * nothing else gives its first number (0: none) with probability 0. NULL: temperature 1, top-k, top-p and min-p off. d_probability (may be NULL): the token's
+ * probability among those kept. n at most 262144. */
+DOOMS_CUDA_API int32_t dooms_cuda_sample_rows(const float * d_logits, int64_t stride, int32_t rows, int32_t n, const float * d_temperature, const int32_t * d_top_k,
+                                              const float * d_top_p, const float * d_min_p, const float * d_uniform, int32_t * d_tokens, float * d_probability, void * stream);
 
 /* ---- A text language model on the decoder: the `Llm` surface of the reference (src/pipeline/llm_pipeline.h:16-82) and its C face dooms_llm_*
  * (include/dooms/dooms_c.h:73-138, src/api/c_api.cpp:322-504) for the decoder's own engine. Vocabulary, byte-level BPE tokenizer and sampler are this
