@@ -1,94 +1,520 @@
-// Attention of one new token per row over its sequence's pages: o = sum_j softmax_j(scale q . k_j) v_j over the row's positions j < length. One warp per (row,
-// query head): a lane holds D / 32 of the head's values.
+// Attention of one new token per row over its sequence's pages: o = sum_j softmax_j(scale q . k_j) v_j over the row's positions j < length, the query heads of a
+// key / value head reading it once.
+//
+// Bound by device memory: 4 D bytes per (key, key / value head), each read once, against 4 G D flops. So the work is dealt by bytes, not by rows: all (row, head
+// group) items, cut into tiles of 64 keys, are laid end to end and every block (two per SM) takes the same number of consecutive tiles, whatever the lengths: one
+// row of 131071 keys and 256 ragged ones run alike. A block walks its span with one warp that fills a ring of shared-memory stages by tensor copies (the pages' rows
+// land in the 128-byte swizzle) and four warps that take 16 keys of each stage; an item that lies whole in a span is written out, of an item that is cut each
+// block leaves (max, sum, output) and k_attention_paged_join adds them up. A block has at most two cut items, so the scratch memory depends on the
+// grid alone and its contents at the start do not matter.
+//
+// The G query heads are rows of m16n8k16 MMAs (f16 operands, f32 accumulators; more than 16 are several items). With f32 queries, query and probabilities enter as f16
+// value + f16 rounding error (2^-22 together), the query after its row was scaled by a power of two, and each tile's products are added to the outputs in f32
+// (round to nearest; the tensor core's own accumulation truncates): as exact as f32 arithmetic. Probabilities are kept times 2^10, so that their second part
+// stays in f16's normal range.
+#include <cuda.h>
 #include <math_constants.h>
+
+#include <algorithm>
+#include <chrono>
 
 #include "launch.cuh"
 #include "paged.cuh"
+#include "ptx.cuh"
 
 namespace dooms {
 namespace cuda {
 
+using namespace dooms::dev;
+
 namespace {
 
-// (also the first form of a prompt's attention: a query sees the positions up to its own)
-template <int D, class T>
-__device__ void one_query(const PagedView & c, int seq, int n, const T * q, T * out, int kvh, float scale, int lane) {
-    constexpr int kPer = D / 32;
-    float qv[kPer], o[kPer] = {}, top = -CUDART_INF_F, sum = 0.f;
-    for (int i = 0; i < kPer; i++) qv[i] = float(q[lane + 32 * i]) * scale;
-    for (int j = 0; j < n; j++) {
-        const int64_t row = c.row(seq, j);
-        if (row < 0) { c.fail(); continue; }
-        const __half * k = c.k + (row * c.n_kv + kvh) * D, * v = c.v + (row * c.n_kv + kvh) * D;
-        float s = 0.f;
-        for (int i = 0; i < kPer; i++) s += qv[i] * __half2float(k[lane + 32 * i]);
-        for (int m = 16; m; m >>= 1) s += __shfl_xor_sync(0xffffffffu, s, m);
-        const float t = fmaxf(top, s), keep = expf(top - t), e = expf(s - t);
-        sum = sum * keep + e;
-        for (int i = 0; i < kPer; i++) o[i] = o[i] * keep + e * __half2float(v[lane + 32 * i]);
-        top = t;
+constexpr int kTile = 64, kWarps = 4, kThreads = (kWarps + 1) * 32;
+constexpr int kBlocksPerSm = 2, kMostBlocks = kBlocksPerSm * 160;
+constexpr int kHeads = 16;                 // query heads of an item
+constexpr float kLift = 10.f;              // probabilities are kept times 2^kLift
+
+struct Args {
+    PagedView c;
+    const void * q;
+    void * out;
+    int n_head, group, parts;              // group: query heads per key / value head; parts: items they make
+    int n_rows, max_length;
+    const int32_t * sequence, * lengths;
+    float scale_log2;
+    unsigned long long call;               // the call's number, not zero
+    unsigned long long * arrived;          // [block]: of the item cut behind that block, the call's number << 16 | blocks that have left their part
+    float * part;                          // [block][2]: outputs [kHeads][D], then (max, sum) [kHeads]
+};
+
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap * map, int x, int y, int z, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+                 ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+// (a, b) as f16 pairs; `rest`: what the rounding left, rounded to f16 too
+__device__ __forceinline__ uint32_t split2(float a, float b, uint32_t * rest) {
+    const __half2 h = __floats2half2_rn(a, b);
+    if (rest) {
+        const float2 f = __half22float2(h);
+        const __half2 r = __floats2half2_rn(a - f.x, b - f.y);
+        *rest = *reinterpret_cast<const uint32_t *>(&r);
     }
-    for (int i = 0; i < kPer; i++) out[lane + 32 * i] = T(sum > 0.f ? o[i] / sum : 0.f);
+    return *reinterpret_cast<const uint32_t *>(&h);
 }
 
-template <int D, class T>
-__global__ void __launch_bounds__(128) k_attention_paged(const PagedView c, const T * q, T * out, int n_head, int n_rows, const int32_t * sequence, const int32_t * lengths,
-                                                         int max_length, float scale) {
-    const int w = int(blockIdx.x) * 4 + threadIdx.x / 32, lane = threadIdx.x % 32;
-    if (w >= n_rows * n_head) return;
-    const int r = w / n_head, h = w % n_head, seq = sequence[r];
-    if (seq < 0) return;
-    int n = lengths[r];
-    if (seq >= c.n_sequences || n < 0 || n > min(max_length, c.capacity())) { c.fail(); return; }
-    one_query<D, T>(c, seq, n, q + int64_t(w) * D, out + int64_t(w) * D, h / (n_head / c.n_kv), scale, lane);
+// Probabilities the same way, cut instead of rounded so that the rest has the first part's sign, and never zero beside a first part that is not (at least 2^-24, which
+// is 2^-34 of a probability): a value of infinity among those seen gives infinity, not infinity times zero.
+__device__ __forceinline__ uint32_t split_p(float a, float b, uint32_t * rest) {
+    uint32_t hi;
+    asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(hi) : "f"(b), "f"(a));
+    const __half2 h = *reinterpret_cast<const __half2 *>(&hi);
+    const float2 f = __half22float2(h);
+    const __half2 r = __hmax2(__floats2half2_rn(a - f.x, b - f.y), __hmin2(h, __half2half2(__ushort_as_half(1))));
+    *rest = *reinterpret_cast<const uint32_t *>(&r);
+    return hi;
 }
 
-template <int D>
-__global__ void __launch_bounds__(128) k_attention_prompt(const PagedView c, const __half * q, __half * out, int n_head, int n_rows, const int32_t * sequence, const int32_t * start,
-                                                          const int32_t * lengths, int n_sequences, float scale) {
-    const int64_t w = int64_t(blockIdx.x) * 4 + threadIdx.x / 32;
-    const int lane = threadIdx.x % 32;
-    if (w >= int64_t(n_rows) * n_head) return;
-    const int r = int(w / n_head), h = int(w % n_head);
-    int i = 0;
-    for (int j = 0; j < n_sequences; j++) if (start[j] < 0 || start[j + 1] < start[j] || start[j + 1] > n_rows) c.fail();
-    while (i < n_sequences && !(r >= start[i] && r < start[i + 1] && start[i] >= 0 && start[i + 1] <= n_rows)) i++;
-    if (i == n_sequences) return;
-    const int seq = sequence[i], n = lengths[i] - (start[i + 1] - 1 - r);
-    if (seq < 0) return;
-    if (seq >= c.n_sequences || lengths[i] < 0 || lengths[i] > c.capacity()) { c.fail(); return; }
-    one_query<D, __half>(c, seq, n, q + w * D, out + w * D, h / (n_head / c.n_kv), scale, lane);
+// Whether row r is one to attend with, and its length; an idle row and one whose entries are out of range have none (-1).
+__device__ __forceinline__ int row_length(const Args & a, int r) {
+    const int s = __ldg(a.sequence + r), n = __ldg(a.lengths + r);
+    return s >= 0 && s < a.c.n_sequences && n >= 0 && n <= min(a.max_length, a.c.capacity()) ? n : -1;
+}
+__device__ __forceinline__ int64_t row_tiles(const Args & a, int r) { const int n = row_length(a, r); return n > 0 ? (n + kTile - 1) / kTile : 0; }
+
+// A place in the line of all tiles: tile `tile` of item (row, part), of which there are `tiles`.
+struct Place { int row, part, tile, tiles; };
+
+// The number of tiles of all rows together; block-wide. kFind: also the row in which tile `at` (of one item per row) lies and the tiles in front of that row.
+// Each thread adds up a run of rows, the block scans the runs, the thread whose run holds `at` walks it.
+__device__ int64_t count_tiles(const Args & a, int64_t * sums) {
+    const int per = (a.n_rows + kThreads - 1) / kThreads, r0 = min(a.n_rows, int(threadIdx.x) * per), r1 = min(a.n_rows, r0 + per);
+    int64_t mine = 0;
+    for (int r = r0; r < r1; r++) mine += row_tiles(a, r);
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+    int64_t run = mine;
+    for (int d = 1; d < 32; d <<= 1) { const int64_t o = __shfl_up_sync(0xffffffffu, run, d); if (lane >= d) run += o; }
+    if (lane == 31) sums[kThreads + warp] = run;
+    __syncthreads();
+    int64_t total = 0;
+    for (int w = 0; w <= kWarps; w++) { if (w < warp) run += sums[kThreads + w]; total += sums[kThreads + w]; }
+    sums[threadIdx.x] = run - mine;      // tiles in front of this thread's rows
+    __syncthreads();
+    return total;
+}
+
+template <int D> constexpr int kSlot = kHeads * (D + 2);      // floats of a part
+
+// Adds up the parts of a cut item, with the block's 128 threads of the four warps, four values a thread: the first block's second slot, the others' first, sixteen
+// parts at a time (their loads in flight together), in the order of the blocks.
+template <int D, bool HALF>
+__device__ __forceinline__ void join(const Args & a, int first, int count, int row, int head0, int heads) {
+    constexpr int kAtOnce = 16;
+    for (int u = threadIdx.x; u < heads * (D / 4); u += kWarps * 32) {
+        const int h = u / (D / 4), d = u % (D / 4) * 4;
+        float m = -CUDART_INF_F, l = 0.f;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int i0 = 0; i0 < count; i0 += kAtOnce) {
+            float2 st[kAtOnce];
+            float4 x[kAtOnce];
+            float top = m;
+            #pragma unroll
+            for (int i = 0; i < kAtOnce; i++) {
+                const bool there = i0 + i < count;
+                const float * p = a.part + (int64_t(first + i0 + i) * 2 + (i0 + i == 0 ? 1 : 0)) * kSlot<D>;
+                st[i] = there ? __ldcg(reinterpret_cast<const float2 *>(p + kHeads * D + 2 * h)) : make_float2(-CUDART_INF_F, 0.f);
+                x[i] = there ? __ldcg(reinterpret_cast<const float4 *>(p + h * D + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+            #pragma unroll
+            for (int i = 0; i < kAtOnce; i++) top = fmaxf(top, st[i].x);
+            const float minus = top == -CUDART_INF_F ? 0.f : top, keep = ex2(m - minus);
+            l *= keep;
+            v.x *= keep; v.y *= keep; v.z *= keep; v.w *= keep;
+            #pragma unroll
+            for (int i = 0; i < kAtOnce; i++) {
+                const float share = ex2(st[i].x - minus);
+                l = fmaf(st[i].y, share, l);
+                v.x = fmaf(x[i].x, share, v.x); v.y = fmaf(x[i].y, share, v.y); v.z = fmaf(x[i].z, share, v.z); v.w = fmaf(x[i].w, share, v.w);
+            }
+            m = top;
+        }
+        const float by = l > 0.f || l != l ? 1.f / l : 0.f;
+        const int64_t at = (int64_t(row) * a.n_head + head0 + h) * D + d;
+        if (HALF) {
+            *reinterpret_cast<__half2 *>(static_cast<__half *>(a.out) + at) = __floats2half2_rn(v.x * by, v.y * by);
+            *reinterpret_cast<__half2 *>(static_cast<__half *>(a.out) + at + 2) = __floats2half2_rn(v.z * by, v.w * by);
+        } else {
+            *reinterpret_cast<float4 *>(static_cast<float *>(a.out) + at) = make_float4(v.x * by, v.y * by, v.z * by, v.w * by);
+        }
+    }
+}
+
+template <int D, bool HALF, bool WIDE>      // WIDE: items of more than 8 query heads
+struct Kernel {
+    static constexpr int kStages = D == 128 ? 3 : 6;
+    static constexpr int kStageBytes = kTile * D * 2 * 2;
+    static constexpr int kPairs = WIDE ? 2 : 1;
+    static constexpr int kMergeBytes = 3 * (D / 8) * 32 * 8;       // three warps' halves of 8 rows
+    static constexpr int kSmem = 1024 + kStages * kStageBytes + kMergeBytes + 3 * kHeads * 8 + (kThreads + 8) * 8 + 16 * kStages + 32;
+    static constexpr int KK = D / 16, NN = D / 8;
+};
+
+template <int D, bool HALF, bool WIDE>
+__global__ void __launch_bounds__(kThreads, kBlocksPerSm) k_attention_paged(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const Args a) {
+    using K = Kernel<D, HALF, WIDE>;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    const uint32_t ring = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    uint8_t * const base = smem_raw + (ring - smem_u32(smem_raw));
+    float2 * const merge = reinterpret_cast<float2 *>(base + K::kStages * K::kStageBytes);                       // [3][NN][32]
+    float2 * const stats = reinterpret_cast<float2 *>(reinterpret_cast<uint8_t *>(merge) + K::kMergeBytes);     // [3][kHeads] (max, sum)
+    int64_t * const sums = reinterpret_cast<int64_t *>(stats + 3 * kHeads);
+    const uint32_t full = smem_u32(sums + kThreads + 8), empty = full + 8 * K::kStages;
+    int * const last = reinterpret_cast<int *>(sums + kThreads + 7);
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < K::kStages; s++) { mbar_init(full + 8 * s, 1); mbar_init(empty + 8 * s, kWarps); }
+        mbar_init_fence();
+    }
+    pdl_wait();
+    // rows without positions are zero; entries out of range are reported
+    for (int r = blockIdx.x; r < a.n_rows; r += gridDim.x) {
+        const int n = row_length(a, r);
+        if (n < 0 && a.sequence[r] >= 0 && threadIdx.x == 0) a.c.fail();
+        if (n == 0) {
+            for (int i = threadIdx.x; i < a.n_head * D; i += kThreads) {
+                if (HALF) static_cast<__half *>(a.out)[int64_t(r) * a.n_head * D + i] = __half(0.f);
+                else static_cast<float *>(a.out)[int64_t(r) * a.n_head * D + i] = 0.f;
+            }
+        }
+    }
+    const int items = a.c.n_kv * a.parts;
+    const int64_t total = count_tiles(a, sums) * items;
+    const int64_t blocks = min(int64_t(gridDim.x), total);
+    if (int64_t(blockIdx.x) >= blocks) return;
+    if (threadIdx.x == 0) {      // the arrival counter of the item that this block's span may end in, unless it is set up (a replay's stays where its item was not cut)
+        const unsigned long long was = *reinterpret_cast<volatile unsigned long long *>(a.arrived + blockIdx.x);
+        if ((was >> 16) != a.call) atomicExch(a.arrived + blockIdx.x, a.call << 16);
+    }
+    const int64_t from = total * blockIdx.x / blocks, to = total * (blockIdx.x + 1) / blocks;
+    Place p;
+    int64_t item_at;      // the first tile of the item at hand
+    {
+        const int per = (a.n_rows + kThreads - 1) / kThreads;
+        int th = 0;
+        for (int step = 128; step; step >>= 1) if (th + step < kThreads && sums[th + step] * items <= from) th += step;
+        int64_t at = sums[th] * items;
+        int r = th * per;
+        int64_t t = row_tiles(a, r);
+        while (at + t * items <= from) { at += t * items; t = row_tiles(a, ++r); }
+        p.row = r; p.tiles = int(t); p.part = int((from - at) / t); p.tile = int((from - at) % t);
+        item_at = at + int64_t(p.part) * t;
+    }
+    auto next_item = [&] {
+        item_at += p.tiles;
+        p.tile = 0;
+        if (++p.part == items) { p.part = 0; do { p.tiles = int(row_tiles(a, ++p.row)); } while (p.tiles == 0); }
+    };
+    bool ok = true;
+    int stage = 0;
+    uint32_t phase = 0;
+    auto advance = [&] { if (++stage == K::kStages) { stage = 0; phase ^= 1u; } };
+    int64_t left = to - from;
+
+    if (warp == kWarps) {
+        // ---- the copies: lane i brings piece i of a tile (the rows of one page, or 64 of them; half a head of 128), keys and values ----
+        const int box = min(kTile, 1 << a.c.page_shift), pieces = kTile / box;
+        while (left > 0) {
+            const int n = row_length(a, p.row), kvh = p.part / a.parts;
+            const int32_t * table = a.c.table + int64_t(a.sequence[p.row]) * a.c.max_pages;
+            for (; p.tile < p.tiles && left > 0; p.tile++, left--) {
+                const int valid = min(kTile, n - p.tile * kTile), used = (valid + box - 1) / box;
+                const int piece = lane / (D / 64), half = lane % (D / 64);
+                int page = 0;
+                const int key = p.tile * kTile + piece * box;
+                if (piece < used) {
+                    page = __ldg(table + (key >> a.c.page_shift));
+                    if (uint32_t(page) >= uint32_t(a.c.n_pages)) { a.c.fail(); page = 0; }
+                }
+                ok = ok && mbar_wait(empty + 8 * stage, phase ^ 1u);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                if (lane == 0) mbar_arrive_expect_tx(full + 8 * stage, uint32_t(used * box) * D * 4u);
+                __syncwarp();
+                if (piece < used) {
+                    const uint32_t dst = ring + stage * K::kStageBytes + half * (kTile * 128) + piece * box * 128;
+                    const int z = (page << a.c.page_shift) + (key & ((1 << a.c.page_shift) - 1));
+                    tma_load_3d(dst, &kmap, half * 64, kvh, z, full + 8 * stage);
+                    tma_load_3d(dst + kTile * D * 2, &vmap, half * 64, kvh, z, full + 8 * stage);
+                }
+                advance();
+            }
+            if (!ok) break;
+            if (left > 0) next_item();
+        }
+        (void)pieces;
+    } else {
+        const int g = lane >> 2, t = lane & 3;
+        // where this lane's ldmatrix rows lie in a stage: keys 16 warp + ..
+        const int krow = warp * 16 + (lane & 7) + ((lane >> 4) & 1) * 8, kchunk = (lane >> 3) & 1;
+        const int vrow = warp * 16 + (lane & 7) + ((lane >> 3) & 1) * 8, vchunk = lane >> 4;
+        const uint32_t kat = uint32_t(krow) * 128u, vat = uint32_t(vrow) * 128u + kTile * D * 2, sw = uint32_t(lane & 7);
+        while (left > 0) {
+            const int n = row_length(a, p.row), kvh = p.part / a.parts, head0 = kvh * a.group + (p.part % a.parts) * kHeads;
+            const int heads = min(kHeads, a.group - (p.part % a.parts) * kHeads);
+            // the item's queries as A operands: rows g and (WIDE) g + 8
+            uint32_t qh[K::KK][4], ql[HALF ? 1 : K::KK][4];
+            float f[K::kPairs];
+            #pragma unroll
+            for (int e = 0; e < 2; e++) {
+                const bool there = e < K::kPairs && g + 8 * e < heads;
+                const int64_t at = (int64_t(p.row) * a.n_head + head0 + g + 8 * e) * D + 2 * t;
+                if (HALF) {
+                    #pragma unroll
+                    for (int kk = 0; kk < K::KK; kk++) {
+                        const uint32_t * q = reinterpret_cast<const uint32_t *>(static_cast<const __half *>(a.q) + at + 16 * kk);
+                        qh[kk][e] = there ? __ldg(q) : 0u;
+                        qh[kk][2 + e] = there ? __ldg(q + 4) : 0u;
+                    }
+                    if (e < K::kPairs) f[e] = a.scale_log2;
+                } else {
+                    float2 v[K::KK][2];
+                    float most = 0.f;
+                    #pragma unroll
+                    for (int kk = 0; kk < K::KK; kk++) {
+                        const float2 * q = reinterpret_cast<const float2 *>(static_cast<const float *>(a.q) + at + 16 * kk);
+                        v[kk][0] = there ? __ldg(q) : make_float2(0.f, 0.f);
+                        v[kk][1] = there ? __ldg(q + 4) : make_float2(0.f, 0.f);
+                        most = fmaxf(fmaxf(most, fmaxf(fabsf(v[kk][0].x), fabsf(v[kk][0].y))), fmaxf(fabsf(v[kk][1].x), fabsf(v[kk][1].y)));
+                    }
+                    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+                    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+                    // a power of two that brings the row's largest value into [1, 2); rows of zeros, of subnormals and with infinities go as they are
+                    const uint32_t ex = __float_as_uint(most) >> 23;
+                    const bool fit = ex > 1 && ex < 253;
+                    const float down = fit ? __uint_as_float((254u - ex) << 23) : 1.f;
+                    if (e < K::kPairs) f[e] = a.scale_log2 * (fit ? __uint_as_float(ex << 23) : 1.f);
+                    #pragma unroll
+                    for (int kk = 0; kk < K::KK; kk++) {
+                        qh[kk][e] = split2(v[kk][0].x * down, v[kk][0].y * down, &ql[HALF ? 0 : kk][e]);
+                        qh[kk][2 + e] = split2(v[kk][1].x * down, v[kk][1].y * down, &ql[HALF ? 0 : kk][2 + e]);
+                    }
+                }
+            }
+            float o[K::NN][2 * K::kPairs], top[K::kPairs], sum[K::kPairs];
+            #pragma unroll
+            for (int j = 0; j < K::NN; j++) { o[j][0] = o[j][1] = 0.f; if (WIDE) o[j][2 * K::kPairs - 2] = o[j][2 * K::kPairs - 1] = 0.f; }
+            #pragma unroll
+            for (int e = 0; e < K::kPairs; e++) { top[e] = -CUDART_INF_F; sum[e] = 0.f; }
+            const bool starts = p.tile == 0;
+            for (; p.tile < p.tiles && left > 0; p.tile++, left--) {
+                const int valid = min(kTile, n - p.tile * kTile) - warp * 16;      // of this warp's 16 keys
+                ok = ok && mbar_wait(full + 8 * stage, phase);
+                ok = __all_sync(0xffffffffu, ok);
+                if (valid > 0) {
+                    const uint32_t st = ring + stage * K::kStageBytes;
+                    float s[2][4] = {};
+                    [[maybe_unused]] float rest[2][4] = {};
+                    #pragma unroll
+                    for (int kk = 0; kk < K::KK; kk++) {
+                        uint32_t b[4];
+                        ldsm4(st + kat + (kk / 4) * (kTile * 128) + (((uint32_t(kk % 4) * 2 + kchunk) ^ sw) << 4), b);
+                        if (HALF) {
+                            mma_f16(s[0], qh[kk], b[0], b[1]);
+                            mma_f16(s[1], qh[kk], b[2], b[3]);
+                        } else {      // sixteen products at a time, added up in f32: a chain through the accumulator loses 1e-6 of a probability on heads of 128
+                            #pragma unroll
+                            for (int j = 0; j < 2; j++) {
+                                float c[4] = {0.f, 0.f, 0.f, 0.f};
+                                mma_f16(c, qh[kk], b[2 * j], b[2 * j + 1]);
+                                mma_f16(rest[j], ql[HALF ? 0 : kk], b[2 * j], b[2 * j + 1]);
+                                #pragma unroll
+                                for (int i = 0; i < 2 * K::kPairs; i++) s[j][i] += c[i];
+                            }
+                        }
+                    }
+                    if (!HALF) {
+                        #pragma unroll
+                        for (int j = 0; j < 2; j++) {
+                            #pragma unroll
+                            for (int i = 0; i < 2 * K::kPairs; i++) s[j][i] += rest[j][i];
+                        }
+                    }
+                    if (valid < 16) {      // the last page's rest: no score, and no value (a page may hold anything there)
+                        #pragma unroll
+                        for (int j = 0; j < 2; j++) {
+                            #pragma unroll
+                            for (int i = 0; i < 4; i++) if (8 * j + 2 * t + (i & 1) >= valid) s[j][i] = -CUDART_INF_F;
+                        }
+                        for (int i = lane; i < (16 - valid) * (D / 8); i += 32) {
+                            const uint32_t row = uint32_t(warp * 16 + valid + i / (D / 8)), c = uint32_t(i % (D / 8));
+                            asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(st + kTile * D * 2 + (c / 8) * (kTile * 128) + row * 128u + (c % 8) * 16u), "r"(0u) : "memory");
+                        }
+                        __syncwarp();
+                    }
+                    uint32_t ph[4] = {0u, 0u, 0u, 0u}, pl[4] = {0u, 0u, 0u, 0u};
+                    float keep[K::kPairs];
+                    #pragma unroll
+                    for (int e = 0; e < K::kPairs; e++) {
+                        const float f_e = f[e];
+                        float m = fmaxf(fmaxf(s[0][2 * e], s[0][2 * e + 1]), fmaxf(s[1][2 * e], s[1][2 * e + 1])) * f_e;
+                        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+                        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+                        m = fmaxf(m, top[e]);
+                        const float minus = m == -CUDART_INF_F ? 0.f : kLift - m;
+                        keep[e] = ex2(top[e] + (m == -CUDART_INF_F ? 0.f : -m));
+                        top[e] = m;
+                        float x[2][2];
+                        #pragma unroll
+                        for (int j = 0; j < 2; j++) { x[j][0] = ex2(fmaf(s[j][2 * e], f_e, minus)); x[j][1] = ex2(fmaf(s[j][2 * e + 1], f_e, minus)); }
+                        sum[e] = sum[e] * keep[e] + ((x[0][0] + x[0][1]) + (x[1][0] + x[1][1]));
+                        ph[e] = HALF ? split2(x[0][0], x[0][1], nullptr) : split_p(x[0][0], x[0][1], &pl[e]);
+                        ph[2 + e] = HALF ? split2(x[1][0], x[1][1], nullptr) : split_p(x[1][0], x[1][1], &pl[2 + e]);
+                    }
+                    #pragma unroll
+                    for (int j = 0; j < K::NN; j += 2) {
+                        uint32_t b[4];
+                        ldsm4_t(st + vat + (j / 8) * (kTile * 128) + (((uint32_t(j % 8) + vchunk) ^ sw) << 4), b);
+                        #pragma unroll
+                        for (int i = 0; i < 2; i++) {
+                            float c[4] = {0.f, 0.f, 0.f, 0.f};
+                            mma_f16(c, ph, b[2 * i], b[2 * i + 1]);
+                            if (!HALF) mma_f16(c, pl, b[2 * i], b[2 * i + 1]);
+                            #pragma unroll
+                            for (int e = 0; e < 2 * K::kPairs; e++) o[j + i][e] = fmaf(o[j + i][e], keep[e / 2], c[e]);
+                        }
+                    }
+                    if (valid < 16) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");      // (the zeros, before a copy may land on them)
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(empty + 8 * stage);
+                advance();
+            }
+            const bool ends = p.tile == p.tiles;
+            // ---- the four warps' results: warps 1 to 3 hand theirs to warp 0, eight rows at a time ----
+            #pragma unroll
+            for (int e = 0; e < K::kPairs; e++) {
+                sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], 1);
+                sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], 2);
+                asm volatile("bar.sync 1, 128;" ::: "memory");      // warp 0 is done with the last hand-over
+                if (warp > 0) {
+                    if (t == 0) stats[(warp - 1) * kHeads + g] = make_float2(top[e], sum[e]);
+                    #pragma unroll
+                    for (int j = 0; j < K::NN; j++) merge[((warp - 1) * K::NN + j) * 32 + lane] = make_float2(o[j][2 * e], o[j][2 * e + 1]);
+                }
+                asm volatile("bar.sync 1, 128;" ::: "memory");
+                if (warp == 0) {
+                    float m = top[e], share[4], l;
+                    #pragma unroll
+                    for (int w = 0; w < 3; w++) m = fmaxf(m, stats[w * kHeads + g].x);
+                    const float minus = m == -CUDART_INF_F ? 0.f : m;
+                    share[0] = ex2(top[e] - minus);
+                    l = sum[e] * share[0];
+                    #pragma unroll
+                    for (int w = 0; w < 3; w++) { const float2 x = stats[w * kHeads + g]; share[w + 1] = ex2(x.x - minus); l += x.y * share[w + 1]; }
+                    const bool whole = starts && ends;
+                    const float by = whole ? (l > 0.f || l != l ? 1.f / l : 0.f) : 1.f;
+                    const int h = g + 8 * e;
+                    float * const part = a.part + (int64_t(blockIdx.x) * 2 + (starts ? 1 : 0)) * kSlot<D>;
+                    const int64_t at = (int64_t(p.row) * a.n_head + head0 + h) * D + 2 * t;
+                    if (h < heads) {
+                        if (!whole && t == 0) *reinterpret_cast<float2 *>(part + kHeads * D + 2 * h) = make_float2(m, l);
+                        #pragma unroll
+                        for (int j = 0; j < K::NN; j++) {
+                            float2 v = make_float2(o[j][2 * e] * share[0], o[j][2 * e + 1] * share[0]);
+                            #pragma unroll
+                            for (int w = 0; w < 3; w++) {
+                                const float2 x = merge[(w * K::NN + j) * 32 + lane];
+                                v.x = fmaf(x.x, share[w + 1], v.x);
+                                v.y = fmaf(x.y, share[w + 1], v.y);
+                            }
+                            v.x *= by;
+                            v.y *= by;
+                            if (!whole) *reinterpret_cast<float2 *>(part + h * D + 8 * j + 2 * t) = v;
+                            else if (HALF) *reinterpret_cast<__half2 *>(static_cast<__half *>(a.out) + at + 8 * j) = __floats2half2_rn(v.x, v.y);
+                            else *reinterpret_cast<float2 *>(static_cast<float *>(a.out) + at + 8 * j) = v;
+                        }
+                    }
+                }
+            }
+            if (!(starts && ends)) {
+                const int first = int(((item_at + 1) * blocks - 1) / total), count = int(((item_at + p.tiles) * blocks - 1) / total) - first + 1;
+                if (warp == 0) {
+                    __threadfence();
+                    __syncwarp();
+                    if (lane == 0) {
+                        // (the block in front of whose last item the counter stands has set it up when it began)
+                        unsigned long long * const cell = a.arrived + first;
+                        uint32_t polls = 0;
+                        while ((*reinterpret_cast<volatile unsigned long long *>(cell) >> 16) != a.call && ++polls < kMaxPolls) {}
+                        ok = ok && polls < kMaxPolls;
+                        const int now = ok ? int(atomicAdd(cell, 1ull) & 0xffffu) + 1 : 0;
+                        if (now == count) *reinterpret_cast<volatile unsigned long long *>(cell) = 0;
+                        *last = now == count;
+                    }
+                }
+                asm volatile("bar.sync 1, 128;" ::: "memory");
+                if (*last) {
+                    __threadfence();
+                    join<D, HALF>(a, first, count, p.row, head0, heads);
+                }
+            }
+            if (left > 0) next_item();
+        }
+    }
+    if (!ok && lane == 0 && a.c.error) *reinterpret_cast<volatile int *>(a.c.error) = kErrorPagedWait;
+}
+
+template <int D, bool HALF, bool WIDE>
+cudaError_t launch(const Args & a, const TensorMap & kmap, const TensorMap & vmap, int blocks, cudaStream_t stream) {
+    constexpr int bytes = Kernel<D, HALF, WIDE>::kSmem;
+    static std::atomic<uint64_t> done{0};
+    cudaError_t e = allow_dynamic_smem(k_attention_paged<D, HALF, WIDE>, bytes, done);
+    if (e != cudaSuccess) return e;
+    return launch_pdl(k_attention_paged<D, HALF, WIDE>, dim3(unsigned(blocks)), dim3(kThreads), bytes, stream, reinterpret_cast<const CUtensorMap &>(kmap),
+                      reinterpret_cast<const CUtensorMap &>(vmap), a);
 }
 
 }  // namespace
 
-size_t attention_paged_scratch_bytes(int, int, int) { return 256; }
-size_t attention_prompt_scratch_bytes(int, int, int) { return 256; }
+size_t attention_paged_scratch_bytes(int, int, int head_dim) { return size_t(kMostBlocks) * (2 * kHeads * (head_dim + 2) * 4 + 8); }
 
 cudaError_t launch_attention_paged(const PagedCache & cache, const void * q, void * out, bool half_io, int n_head, int n_rows, const int32_t * sequence, const int32_t * lengths,
-                                   int max_length, float scale, void *, int * error, cudaStream_t stream) {
-    const PagedView c = paged_view(cache, error);
-    const unsigned blocks = unsigned((int64_t(n_rows) * n_head + 3) / 4);
-    auto go = [&]<class T>(auto kernel, T) {
-        kernel<<<blocks, 128, 0, stream>>>(c, static_cast<const T *>(q), static_cast<T *>(out), n_head, n_rows, sequence, lengths, max_length, scale);
-    };
-    if (cache.head_dim == 128) half_io ? go(k_attention_paged<128, __half>, __half()) : go(k_attention_paged<128, float>, 0.f);
-    else if (cache.head_dim == 64) half_io ? go(k_attention_paged<64, __half>, __half()) : go(k_attention_paged<64, float>, 0.f);
-    else return cudaErrorInvalidValue;
-    return cudaGetLastError();
-}
-
-cudaError_t launch_attention_prompt_paged(const PagedCache & cache, const void * q, void * out, int n_head, int n_rows, int n_sequences, const int32_t * sequence,
-                                          const int32_t * start, const int32_t * lengths, float scale, void *, int * error, cudaStream_t stream) {
-    const PagedView c = paged_view(cache, error);
-    const unsigned blocks = unsigned((int64_t(n_rows) * n_head + 3) / 4);
-    auto go = [&](auto kernel) {
-        kernel<<<blocks, 128, 0, stream>>>(c, static_cast<const __half *>(q), static_cast<__half *>(out), n_head, n_rows, sequence, start, lengths, n_sequences, scale);
-    };
-    if (cache.head_dim == 128) go(k_attention_prompt<128>);
-    else if (cache.head_dim == 64) go(k_attention_prompt<64>);
-    else return cudaErrorInvalidValue;
-    return cudaGetLastError();
+                                   int max_length, float scale, void * scratch, int * error, cudaStream_t stream) {
+    Args a{};
+    a.c = paged_view(cache, error);
+    a.q = q; a.out = out;
+    a.n_head = n_head; a.group = n_head / cache.n_head_kv; a.parts = (a.group + kHeads - 1) / kHeads;
+    a.n_rows = n_rows; a.max_length = max_length;
+    a.sequence = sequence; a.lengths = lengths;
+    a.scale_log2 = scale * 1.44269504f;
+    static std::atomic<unsigned long long> calls{(unsigned long long)(std::chrono::steady_clock::now().time_since_epoch().count()) * 0x9E3779B97F4A7C15ull >> 20};
+    do a.call = calls.fetch_add(1, std::memory_order_relaxed) & 0xffffffffffffull; while (a.call == 0 || a.call == 0xffffffffffffull);
+    a.arrived = static_cast<unsigned long long *>(scratch);
+    a.part = reinterpret_cast<float *>(a.arrived + kMostBlocks);
+    const int blocks = std::min(kMostBlocks, kBlocksPerSm * sm_count());
+    TensorMap kmap, vmap;
+    cudaError_t e = make_pages_map(&kmap, cache.keys, cache, std::min(kTile, cache.page_size));
+    if (e == cudaSuccess) e = make_pages_map(&vmap, cache.values, cache, std::min(kTile, cache.page_size));
+    if (e != cudaSuccess) return e;
+    const bool wide = a.group > 8;
+    if (cache.head_dim == 128) {
+        if (half_io) return wide ? launch<128, true, true>(a, kmap, vmap, blocks, stream) : launch<128, true, false>(a, kmap, vmap, blocks, stream);
+        return wide ? launch<128, false, true>(a, kmap, vmap, blocks, stream) : launch<128, false, false>(a, kmap, vmap, blocks, stream);
+    }
+    if (cache.head_dim != 64) return cudaErrorInvalidValue;
+    if (half_io) return wide ? launch<64, true, true>(a, kmap, vmap, blocks, stream) : launch<64, true, false>(a, kmap, vmap, blocks, stream);
+    return wide ? launch<64, false, true>(a, kmap, vmap, blocks, stream) : launch<64, false, false>(a, kmap, vmap, blocks, stream);
 }
 
 }  // namespace cuda

@@ -700,6 +700,18 @@ cudaError_t make_rows_map(TensorMap * out, const void * base, int64_t rows, int6
     return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
+cudaError_t make_pages_map(TensorMap * out, const void * pool, const PagedCache & c, int box_rows) {
+    EncodeTiledFn fn = encode_tiled();
+    if (!fn) return cudaErrorNotSupported;
+    const cuuint64_t dims[3] = {cuuint64_t(c.head_dim), cuuint64_t(c.n_head_kv), cuuint64_t(c.n_pages) * cuuint64_t(c.page_size)};
+    const cuuint64_t strides[2] = {cuuint64_t(c.head_dim) * 2, cuuint64_t(c.head_dim) * 2 * cuuint64_t(c.n_head_kv)};
+    const cuuint32_t box[3] = {64u, 1u, cuuint32_t(box_rows)};
+    const cuuint32_t estr[3] = {1u, 1u, 1u};
+    const CUresult r = fn(reinterpret_cast<CUtensorMap *>(out), CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void *>(pool), dims, strides, box, estr,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
 // The token count from which quantized projections run on f16 rows, when the environment sets one; -1: by on_rows16's own rules.
 static int rows16_from() {
     static const int v = [] { const char * e = getenv("DOOMS_GEMM_PRE_FROM"); return e ? std::max(0, atoi(e)) : -1; }();
