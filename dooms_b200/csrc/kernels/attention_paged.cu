@@ -5,8 +5,8 @@
 // group) items, cut into tiles of 64 keys, are laid end to end and every block (two per SM) takes the same number of consecutive tiles, whatever the lengths: one
 // row of 131071 keys and 256 ragged ones run alike. A block walks its span with one warp that fills a ring of shared-memory stages by tensor copies (the pages' rows
 // land in the 128-byte swizzle) and four warps that take 16 keys of each stage; an item that lies whole in a span is written out, of an item that is cut each
-// block leaves (max, sum, output) and k_attention_paged_join adds them up. A block has at most two cut items, so the scratch memory depends on the
-// grid alone and its contents at the start do not matter.
+// block leaves (max, sum, output), and the last of them to arrive adds them up in the order of the blocks. A block has at most two cut items, so the scratch memory
+// depends on the grid alone, and its contents at the start do not matter.
 //
 // The G query heads are rows of m16n8k16 MMAs (f16 operands, f32 accumulators; more than 16 are several items). With f32 queries, query and probabilities enter as f16
 // value + f16 rounding error (2^-22 together), the query after its row was scaled by a power of two, and each tile's products are added to the outputs in f32
@@ -16,7 +16,6 @@
 #include <math_constants.h>
 
 #include <algorithm>
-#include <chrono>
 
 #include "launch.cuh"
 #include "paged.cuh"
@@ -96,8 +95,7 @@ __device__ __forceinline__ int64_t row_tiles(const Args & a, int r) { const int 
 // A place in the line of all tiles: tile `tile` of item (row, part), of which there are `tiles`.
 struct Place { int row, part, tile, tiles; };
 
-// The number of tiles of all rows together; block-wide. kFind: also the row in which tile `at` (of one item per row) lies and the tiles in front of that row.
-// Each thread adds up a run of rows, the block scans the runs, the thread whose run holds `at` walks it.
+// The number of tiles of all rows together; block-wide. Each thread adds up a run of rows; sums[th] becomes the tiles in front of thread th's run.
 __device__ int64_t count_tiles(const Args & a, int64_t * sums) {
     const int per = (a.n_rows + kThreads - 1) / kThreads, r0 = min(a.n_rows, int(threadIdx.x) * per), r1 = min(a.n_rows, r0 + per);
     int64_t mine = 0;
@@ -202,10 +200,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) k_attention_paged(cons
     const int64_t total = count_tiles(a, sums) * items;
     const int64_t blocks = min(int64_t(gridDim.x), total);
     if (int64_t(blockIdx.x) >= blocks) return;
-    if (threadIdx.x == 0) {      // the arrival counter of the item that this block's span may end in, unless it is set up (a replay's stays where its item was not cut)
-        const unsigned long long was = *reinterpret_cast<volatile unsigned long long *>(a.arrived + blockIdx.x);
-        if ((was >> 16) != a.call) atomicExch(a.arrived + blockIdx.x, a.call << 16);
-    }
+    paged_counter_begin(a.arrived + blockIdx.x, a.call);      // of the item that this block's span may end in
     const int64_t from = total * blockIdx.x / blocks, to = total * (blockIdx.x + 1) / blocks;
     Place p;
     int64_t item_at;      // the first tile of the item at hand
@@ -453,14 +448,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) k_attention_paged(cons
                     __threadfence();
                     __syncwarp();
                     if (lane == 0) {
-                        // (the block in front of whose last item the counter stands has set it up when it began)
-                        unsigned long long * const cell = a.arrived + first;
-                        uint32_t polls = 0;
-                        while ((*reinterpret_cast<volatile unsigned long long *>(cell) >> 16) != a.call && ++polls < kMaxPolls) {}
-                        ok = ok && polls < kMaxPolls;
-                        const int now = ok ? int(atomicAdd(cell, 1ull) & 0xffffu) + 1 : 0;
-                        if (now == count) *reinterpret_cast<volatile unsigned long long *>(cell) = 0;
-                        *last = now == count;
+                        *last = paged_counter_arrive(a.arrived + first, a.call, count, &ok);
                     }
                 }
                 asm volatile("bar.sync 1, 128;" ::: "memory");
@@ -498,14 +486,14 @@ cudaError_t launch_attention_paged(const PagedCache & cache, const void * q, voi
     a.n_rows = n_rows; a.max_length = max_length;
     a.sequence = sequence; a.lengths = lengths;
     a.scale_log2 = scale * 1.44269504f;
-    static std::atomic<unsigned long long> calls{(unsigned long long)(std::chrono::steady_clock::now().time_since_epoch().count()) * 0x9E3779B97F4A7C15ull >> 20};
-    do a.call = calls.fetch_add(1, std::memory_order_relaxed) & 0xffffffffffffull; while (a.call == 0 || a.call == 0xffffffffffffull);
+    a.call = paged_call();
     a.arrived = static_cast<unsigned long long *>(scratch);
     a.part = reinterpret_cast<float *>(a.arrived + kMostBlocks);
     const int blocks = std::min(kMostBlocks, kBlocksPerSm * sm_count());
+    const int64_t rows = int64_t(cache.n_pages) * cache.page_size;
     TensorMap kmap, vmap;
-    cudaError_t e = make_pages_map(&kmap, cache.keys, cache, std::min(kTile, cache.page_size));
-    if (e == cudaSuccess) e = make_pages_map(&vmap, cache.values, cache, std::min(kTile, cache.page_size));
+    cudaError_t e = make_heads_map(&kmap, cache.keys, cache.head_dim, cache.n_head_kv, rows, 1, std::min(kTile, cache.page_size));
+    if (e == cudaSuccess) e = make_heads_map(&vmap, cache.values, cache.head_dim, cache.n_head_kv, rows, 1, std::min(kTile, cache.page_size));
     if (e != cudaSuccess) return e;
     const bool wide = a.group > 8;
     if (cache.head_dim == 128) {

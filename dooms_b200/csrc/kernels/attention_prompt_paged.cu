@@ -1,68 +1,567 @@
-// Attention of one new token per row over its sequence's pages: o = sum_j softmax_j(scale q . k_j) v_j over the row's positions j < length. One warp per (row,
-// query head): a lane holds D / 32 of the head's values.
+// Causal attention of packed prompts over a paged cache with grouped heads: query j of a prompt, at position length - queries + j of its sequence, sees the positions
+// up to its own: o = sum_p softmax_p(scale q . k_p) v_p.
+//
+// Bound by the tensor cores and the exponentials: 4 D flops and one exponential per (query head, key), which on heads of 128 take the same time (128 x 128 scores: 512
+// cycles of tcgen05.mma for S, 512 for O, 1024 of the special function units). Both run on tcgen05:
+//   * A unit is one key / value head and 2 x floor(128 / G) queries: the G query heads that share the head are rows of the same tile (row = query * G + head), so that a
+//     unit reads K and V once for all of them and short prompts fill the tile's rows. Its two tiles of 128 rows, A and B, take turns: while one's scores are in the
+//     softmax the tensor core works on the other.
+//   * One thread issues the MMAs: S = Q K^T (operands by tensor copies in the 128-byte swizzle, accumulator in tensor memory), then O += P V with P (f16) read from
+//     tensor memory, where the softmax left it over the scores it came from, and V as it lies in its pages (its 128-byte rows are the N-major form of the
+//     operand). One warp brings Q, K and V: a tile of 128 keys is one copy per page and 64 values.
+//   * Four warps per tile do the softmax, a thread per row: the row's scores come from tensor memory once, maximum and sum need no other thread. Outputs are scaled
+//     back only when a row's maximum has grown by more than 2^8 since they were last (probabilities may stand up to 2^8 higher meanwhile).
+// Blocks are persistent, one per SM. The units of all prompts lie end to end, each as long as its last query's keys and a constant for what a unit costs besides; every
+// block takes the same length of this line, cutting units between key tiles. The parts of a cut unit (f32 outputs, maxima, sums) are joined by the last of its
+// blocks to arrive, in the order of the blocks: one prompt of 8192 queries, four pieces of 500 behind 6000 keys and a single query behind 40000 keep all SMs alike.
+// Queries and probabilities are f16 (the type queries come in; a probability's rounding is 2^-12 of it on average, the outputs' own rounding the same again),
+// scores, sums and outputs f32.
+#include <cuda.h>
 #include <math_constants.h>
+
+#include <algorithm>
 
 #include "launch.cuh"
 #include "paged.cuh"
+#include "ptx.cuh"
 
 namespace dooms {
 namespace cuda {
 
+using namespace dooms::dev;
+
 namespace {
 
-// (also the first form of a prompt's attention: a query sees the positions up to its own)
-template <int D, class T>
-__device__ void one_query(const PagedView & c, int seq, int n, const T * q, T * out, int kvh, float scale, int lane) {
-    constexpr int kPer = D / 32;
-    float qv[kPer], o[kPer] = {}, top = -CUDART_INF_F, sum = 0.f;
-    for (int i = 0; i < kPer; i++) qv[i] = float(q[lane + 32 * i]) * scale;
-    for (int j = 0; j < n; j++) {
-        const int64_t row = c.row(seq, j);
-        if (row < 0) { c.fail(); continue; }
-        const __half * k = c.k + (row * c.n_kv + kvh) * D, * v = c.v + (row * c.n_kv + kvh) * D;
-        float s = 0.f;
-        for (int i = 0; i < kPer; i++) s += qv[i] * __half2float(k[lane + 32 * i]);
-        for (int m = 16; m; m >>= 1) s += __shfl_xor_sync(0xffffffffu, s, m);
-        const float t = fmaxf(top, s), keep = expf(top - t), e = expf(s - t);
-        sum = sum * keep + e;
-        for (int i = 0; i < kPer; i++) o[i] = o[i] * keep + e * __half2float(v[lane + 32 * i]);
-        top = t;
-    }
-    for (int i = 0; i < kPer; i++) out[lane + 32 * i] = T(sum > 0.f ? o[i] / sum : 0.f);
+constexpr int kRows = 128, kHalf = 64;      // rows of a tile, and keys of a tile
+constexpr int kThreads = 320;               // two softmax groups of four warps, the copies' warp, the MMAs' warp
+constexpr int kMostBlocks = 160;
+constexpr int kUnitCost = 256;              // what a unit costs besides its keys, in keys
+constexpr int kShortestSpan = kUnitCost + kRows;      // of the line, per block: a block inside a cut unit has at least two whole tiles
+constexpr float kRescale = 8.f;             // log2 of the growth of a maximum that is let be
+constexpr float kLift = 6.f;                // probabilities are kept times 2^kLift: those of 2^-20 are still normal f16 values, and 2^(kLift + kRescale) is one
+
+struct Args {
+    PagedView c;
+    __half * out;
+    int n_head, group, tile_queries, n_prompts, n_rows;      // tile_queries: queries per tile
+    const int32_t * sequence, * start, * lengths;
+    float scale_log2;
+    unsigned long long call, * arrived;
+    float * part;                           // [block][2][tile]: outputs [D / 4][kRows] float4, then (max, sum) [kRows]
+};
+
+template <int D> constexpr int kTilePart = kRows * (D + 2);
+template <int D> constexpr int kTileBytes = kRows * D * 2;
+template <int D> constexpr int kRing = D == 128 ? 2 : 4;          // stages of K, and of V
+template <int D> constexpr int kSmem = 1024 + 2 * kTileBytes<D> + 2 * kRing<D> * kTileBytes<D> + (kThreads + 16) * 8 + 256;
+
+// ---- tcgen05 and copies ----
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap * map, int x, int y, int z, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+                 ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_commit(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+// D (+)= A B with A and B in shared memory
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+// the same with A in tensor memory
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+                 ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+#define R8(r, i) "=r"(r[i]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3]), "=r"(r[i + 4]), "=r"(r[i + 5]), "=r"(r[i + 6]), "=r"(r[i + 7])
+#define W8(r, i) "r"(r[i]), "r"(r[i + 1]), "r"(r[i + 2]), "r"(r[i + 3]), "r"(r[i + 4]), "r"(r[i + 5]), "r"(r[i + 6]), "r"(r[i + 7])
+// 32 columns of this lane's row; the values are there after tc_wait_ld
+__device__ __forceinline__ void tc_ld32(uint32_t at, uint32_t * r) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+                 : R8(r, 0), R8(r, 8), R8(r, 16), R8(r, 24) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void tc_st32(uint32_t at, const uint32_t * r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};"
+                 ::W8(r, 0), W8(r, 8), W8(r, 16), W8(r, 24), "r"(at) : "memory");
+}
+#undef R8
+#undef W8
+__device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// Operand tiles of 128-byte rows in the 128-byte swizzle, groups of 8 rows 1024 bytes apart. K-major (Q, K): a row is 64 values of the reduction, a slice of 16 of
+// them is addressed by its byte offset. N-major (V): a row is one key and 64 of the outputs' columns, the next 64 columns lie a whole tile half further.
+__device__ __forceinline__ uint64_t desc_k(uint32_t at) { return uint64_t((at & 0x3FFFFu) >> 4) | (uint64_t(1) << 16) | (uint64_t(1024 >> 4) << 32) | (uint64_t(1) << 46) | (uint64_t(2) << 61); }
+__device__ __forceinline__ uint64_t desc_n(uint32_t at) {
+    return uint64_t((at & 0x3FFFFu) >> 4) | (uint64_t((kRows * 128) >> 4) << 16) | (uint64_t(1024 >> 4) << 32) | (uint64_t(1) << 46) | (uint64_t(2) << 61);
+}
+// f16 operands, f32 accumulator, M = 128, N = n; n_major: B is N-major
+constexpr uint32_t idesc(int n, bool n_major) { return (1u << 4) | (n_major ? 1u << 16 : 0u) | (uint32_t(n >> 3) << 17) | (uint32_t(kRows >> 4) << 24); }
+
+__device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+
+// ---- the line of units ----
+// The part of prompt i that has something to see: its first row, its queries, the keys in front of its first query; no queries for one that is idle or out of range.
+struct Prompt { int row, queries, ahead, seq; };
+__device__ __forceinline__ Prompt prompt_at(const Args & a, int i, bool * bad = nullptr) {
+    const int s = __ldg(a.sequence + i), b = __ldg(a.start + i), e = __ldg(a.start + i + 1), n = __ldg(a.lengths + i);
+    const bool fine = s < a.c.n_sequences && n >= 0 && n <= a.c.capacity() && b >= 0 && e >= b && e <= a.n_rows;
+    if (bad) *bad = s >= 0 && !fine;
+    if (s < 0 || !fine) return {0, 0, 0, s};
+    const int unseen = max(0, e - b - n);
+    return {b + unseen, e - b - unseen, n - (e - b - unseen), s};
+}
+struct Unit { int prompt, kvh, tile; };        // tile: of 2 tile_queries queries
+// The length of the line up to unit `tile` of a prompt and head.
+__device__ __forceinline__ int64_t units_length(const Prompt & p, int wide, int tile) {
+    const int last = (p.queries + wide - 1) / wide;      // (the last unit ends with the prompt)
+    const int64_t t = tile;
+    return t * (p.ahead + kUnitCost) + wide * (t * (t + 1) / 2) - (tile == last ? int64_t(last) * wide - p.queries : 0);
+}
+__device__ __forceinline__ int64_t prompt_length(const Args & a, const Prompt & p) {
+    const int wide = 2 * a.tile_queries;
+    return p.queries ? a.c.n_kv * units_length(p, wide, (p.queries + wide - 1) / wide) : 0;
 }
 
 template <int D>
-__global__ void __launch_bounds__(128) k_attention_prompt(const PagedView c, const __half * q, __half * out, int n_head, int n_rows, const int32_t * sequence, const int32_t * start,
-                                                          const int32_t * lengths, int n_sequences, float scale) {
-    const int64_t w = int64_t(blockIdx.x) * 4 + threadIdx.x / 32;
-    const int lane = threadIdx.x % 32;
-    if (w >= int64_t(n_rows) * n_head) return;
-    const int r = int(w / n_head), h = int(w % n_head);
-    int i = 0;
-    for (int j = 0; j < n_sequences; j++) if (start[j] < 0 || start[j + 1] < start[j] || start[j + 1] > n_rows) c.fail();
-    while (i < n_sequences && !(r >= start[i] && r < start[i + 1] && start[i] >= 0 && start[i + 1] <= n_rows)) i++;
-    if (i == n_sequences) return;
-    const int seq = sequence[i], n = lengths[i] - (start[i + 1] - 1 - r);
-    if (seq < 0) return;
-    if (seq >= c.n_sequences || lengths[i] < 0 || lengths[i] > c.capacity()) { c.fail(); return; }
-    one_query<D, __half>(c, seq, n, q + w * D, out + w * D, h / (n_head / c.n_kv), scale, lane);
+__global__ void __launch_bounds__(kThreads, 1) k_attention_prompt(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
+                                                                  const __grid_constant__ CUtensorMap vmap, const Args a) {
+    constexpr int S = kRing<D>;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    const uint32_t q_at = (smem_u32(smem_raw) + 1023u) & ~1023u, k_at = q_at + 2 * kTileBytes<D>, v_at = k_at + S * kTileBytes<D>;
+    int64_t * const sums = reinterpret_cast<int64_t *>(smem_raw + (v_at + S * kTileBytes<D> - smem_u32(smem_raw)));
+    int * const flag = reinterpret_cast<int *>(sums + kThreads + 15);
+    const uint32_t bars = smem_u32(sums + kThreads + 16);
+    const uint32_t q_full = bars, q_empty = bars + 8, s_full = bars + 16, p_full = bars + 32, o_done = bars + 48, k_full = bars + 64, k_empty = k_full + 8 * S, v_full = k_empty + 8 * S,
+                   v_empty = v_full + 8 * S, v_fixed = v_empty + 8 * S, tmem_slot = v_fixed + 8 * S;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    if (threadIdx.x == 0) {
+        mbar_init(q_full, 1); mbar_init(q_empty, 1);
+        for (int x = 0; x < 2; x++) { mbar_init(s_full + 8 * x, 1); mbar_init(p_full + 8 * x, 4); mbar_init(o_done + 8 * x, 1); }
+        for (int s = 0; s < S; s++) { mbar_init(k_full + 8 * s, 1); mbar_init(k_empty + 8 * s, 1); mbar_init(v_full + 8 * s, 1); mbar_init(v_empty + 8 * s, 1); mbar_init(v_fixed + 8 * s, 1); }
+        mbar_init_fence();
+    }
+    pdl_wait();
+
+    // ---- what is out of range is reported, queries that see nothing are zero; then the line ----
+    const int wide = 2 * a.tile_queries;
+    for (int i = blockIdx.x; i < a.n_prompts; i += gridDim.x) {
+        bool bad = false;
+        const Prompt p = prompt_at(a, i, &bad);
+        if (bad && threadIdx.x == 0) a.c.fail();
+        if (bad || p.seq < 0) continue;
+        const int b = a.start[i], unseen = (a.start[i + 1] - b) - p.queries;
+        for (int64_t u = threadIdx.x; u < int64_t(unseen) * a.n_head * D; u += kThreads) a.out[int64_t(b) * a.n_head * D + u] = __half(0.f);
+    }
+    const int per = (a.n_prompts + kThreads - 1) / kThreads;
+    {
+        const int i0 = min(a.n_prompts, int(threadIdx.x) * per), i1 = min(a.n_prompts, i0 + per);
+        int64_t mine = 0;
+        for (int i = i0; i < i1; i++) mine += prompt_length(a, prompt_at(a, i));
+        int64_t run = mine;
+        for (int d = 1; d < 32; d <<= 1) { const int64_t o = __shfl_up_sync(0xffffffffu, run, d); if (lane >= d) run += o; }
+        if (lane == 31) sums[kThreads + warp] = run;
+        __syncthreads();
+        for (int w = 0; w < warp; w++) run += sums[kThreads + w];
+        sums[threadIdx.x] = run - mine;
+        if (threadIdx.x == kThreads - 1) sums[kThreads + 14] = run;
+        __syncthreads();
+    }
+    const int64_t total = sums[kThreads + 14];
+    const int64_t blocks = max(int64_t(1), min(int64_t(gridDim.x), total / kShortestSpan));
+    if (total == 0 || int64_t(blockIdx.x) >= blocks) return;
+    paged_counter_begin(a.arrived + blockIdx.x, a.call);
+    if (warp == 9) {      // the MMAs' warp owns the tensor memory
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(tmem_slot) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    uint32_t tmem;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(tmem_slot));
+
+    const int64_t from = total * blockIdx.x / blocks, to = total * (blockIdx.x + 1) / blocks;
+    Unit u;
+    Prompt p;
+    int64_t unit_at;      // where unit u begins
+    {
+        int th = 0;
+        for (int step = 256; step; step >>= 1) if (th + step < kThreads && sums[th + step] <= from) th += step;
+        int64_t at = sums[th];
+        int i = th * per;
+        int64_t n;
+        for (;; i++) { p = prompt_at(a, i); n = prompt_length(a, p); if (at + n > from) break; at += n; }
+        const int tiles = (p.queries + wide - 1) / wide;
+        const int64_t head = n / a.c.n_kv;
+        const int kvh = int((from - at) / head);
+        at += kvh * head;
+        int t = 0;
+        for (int step = 1 << 30; step; step >>= 1) if (t + step < tiles && at + units_length(p, wide, t + step) <= from) t += step;
+        u = {i, kvh, t};
+        unit_at = at + units_length(p, wide, t);
+    }
+    // The segment of unit u that is this block's: key tiles [t0, t1) of its `tiles`.
+    struct Segment { int row, queries, first, keys, tiles, t0, t1; int64_t next; };
+    auto tile_of = [&](int64_t x, int tiles) { return int(max(int64_t(0), min(int64_t(tiles), (x - kUnitCost + kRows / 2) / kRows))); };      // (x - kUnitCost < 0 rounds to 0)
+    auto segment = [&]() -> Segment {
+        const int q0 = u.tile * wide, n = min(wide, p.queries - q0), keys = p.ahead + q0 + n, tiles = (keys + kRows - 1) / kRows;
+        const int64_t end = unit_at + keys + kUnitCost;
+        return {p.row + q0, n, p.ahead + q0, keys, tiles, from > unit_at ? tile_of(from - unit_at, tiles) : 0, to < end ? tile_of(to - unit_at, tiles) : tiles, end};
+    };
+    auto next_unit = [&](const Segment & s) {
+        unit_at = s.next;
+        if (++u.tile * wide < p.queries) return;
+        u.tile = 0;
+        if (++u.kvh < a.c.n_kv) return;
+        u.kvh = 0;
+        do { u.prompt++; } while (u.prompt < a.n_prompts && (p = prompt_at(a, u.prompt)).queries == 0);
+    };
+    // key tiles of the segment that tile x of the unit (its queries [x tile_queries, ..)) takes part in
+    auto steps_of = [&](const Segment & s, int x) {
+        const int q = min(s.queries, (x + 1) * a.tile_queries);
+        if (q <= x * a.tile_queries) return 0;
+        return max(0, min(s.t1, (s.first + q + kRows - 1) / kRows) - s.t0);
+    };
+    bool ok = true;
+
+    if (warp == 8) {
+        // ---- the copies ----
+        const int box = min(kRows, 1 << a.c.page_shift), piece = lane / (D / 64), half = lane % (D / 64);
+        int stage = 0, units = 0;
+        uint32_t phase = 0;
+        while (unit_at < to && ok) {
+            const Segment s = segment();
+            if (s.t0 < s.t1) {
+                ok = mbar_wait(q_empty, uint32_t(units & 1) ^ 1u);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                units++;
+                if (lane == 0) {
+                    const int boxes = s.queries > a.tile_queries ? 2 : 1;
+                    mbar_arrive_expect_tx(q_full, uint32_t(boxes * a.tile_queries * a.group) * D * 2u);
+                    for (int x = 0; x < boxes; x++) {
+                        for (int h = 0; h < D / 64; h++) tma_load_3d(q_at + x * kTileBytes<D> + h * (kRows * 128), &qmap, h * 64, u.kvh * a.group, s.row + x * a.tile_queries, q_full);
+                    }
+                }
+                __syncwarp();
+                const int32_t * table = a.c.table + int64_t(p.seq) * a.c.max_pages;
+                for (int t = s.t0; t < s.t1 && ok; t++) {
+                    const int valid = min(kRows, s.keys - t * kRows), used = (valid + box - 1) / box, key = t * kRows + piece * box;
+                    int page = 0;
+                    if (piece < used) {
+                        page = __ldg(table + (key >> a.c.page_shift));
+                        if (uint32_t(page) >= uint32_t(a.c.n_pages)) { a.c.fail(); page = 0; }
+                    }
+                    const int z = (page << a.c.page_shift) + (key & ((1 << a.c.page_shift) - 1));
+                    const uint32_t at = stage * kTileBytes<D> + half * (kRows * 128) + piece * box * 128;
+                    #pragma unroll
+                    for (int kv = 0; kv < 2; kv++) {
+                        const uint32_t full = (kv ? v_full : k_full) + 8 * stage;
+                        ok = ok && mbar_wait((kv ? v_empty : k_empty) + 8 * stage, phase ^ 1u);
+                        ok = __all_sync(0xffffffffu, ok);
+                        if (!ok) break;
+                        if (lane == 0) mbar_arrive_expect_tx(full, uint32_t(used * box) * D * 2u);
+                        __syncwarp();
+                        if (piece < used) tma_load_3d((kv ? v_at : k_at) + at, kv ? &vmap : &kmap, half * 64, u.kvh, z, full);
+                    }
+                    if (!ok) break;
+                    if (valid < kRows) {      // values behind the last key seen are zeros: a probability of zero times what a page may hold there has to stay zero
+                        ok = mbar_wait(v_full + 8 * stage, phase);
+                        ok = __all_sync(0xffffffffu, ok);
+                        for (int i = lane; i < (kRows - valid) * (D / 8); i += 32) {
+                            const uint32_t row = uint32_t(valid + i / (D / 8)), c = uint32_t(i % (D / 8));
+                            asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(v_at + stage * kTileBytes<D> + (c / 8) * (kRows * 128) + row * 128u + (c % 8) * 16u), "r"(0u) : "memory");
+                        }
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(v_fixed + 8 * stage);
+                    }
+                    if (++stage == S) { stage = 0; phase ^= 1u; }
+                }
+            }
+            next_unit(s);
+        }
+    } else if (warp == 9) {
+        // ---- the MMAs ----
+        if (lane == 0) {
+            constexpr uint32_t id_s = idesc(kRows, false), id_o = idesc(D, true);
+            int kstage = 0, vstage = 0, units = 0;
+            uint32_t kphase = 0, vphase = 0, fixed = 0, done[2] = {0, 0};      // fixed: the phases of v_fixed, a bit per stage; done: probabilities taken
+            auto scores = [&](int x) {
+                #pragma unroll
+                for (int kk = 0; kk < D / 16; kk++) {
+                    const uint32_t at = (kk / 4) * (kRows * 128) + (kk % 4) * 32;
+                    mma_ss(tmem + x * kRows, desc_k(q_at + x * kTileBytes<D> + at), desc_k(k_at + kstage * kTileBytes<D> + at), id_s, kk != 0);
+                }
+                tc_commit(s_full + 8 * x);
+            };
+            while (unit_at < to && ok) {
+                const Segment s = segment();
+                const int n = s.t1 - s.t0;
+                if (n > 0) {
+                    const int steps[2] = {steps_of(s, 0), steps_of(s, 1)};
+                    ok = mbar_wait(q_full, uint32_t(units & 1)) && mbar_wait(k_full + 8 * kstage, kphase);
+                    if (!ok) break;
+                    units++;
+                    tc_fence_after();
+                    for (int x = 0; x < 2; x++) if (steps[x] > 0) scores(x);
+                    tc_commit(k_empty + 8 * kstage);
+                    if (n == 1) tc_commit(q_empty);
+                    if (++kstage == S) { kstage = 0; kphase ^= 1u; }
+                    for (int j = 0; j < n && ok; j++) {
+                        bool have_v = false, have_k = false;
+                        for (int x = 0; x < 2 && ok; x++) {
+                            if (j < steps[x]) {
+                                ok = mbar_wait(p_full + 8 * x, done[x] & 1u);
+                                if (ok && !have_v) {
+                                    ok = mbar_wait(v_full + 8 * vstage, vphase);
+                                    if (ok && s.keys - (s.t0 + j) * kRows < kRows) { ok = mbar_wait(v_fixed + 8 * vstage, fixed >> vstage & 1u); fixed ^= 1u << vstage; }
+                                    have_v = true;
+                                }
+                                if (!ok) break;
+                                done[x]++;
+                                tc_fence_after();
+                                #pragma unroll
+                                for (int kk = 0; kk < kRows / 16; kk++) {
+                                    mma_ts(tmem + 256 + x * kRows, tmem + x * kRows + kHalf + kk * 8, desc_n(v_at + vstage * kTileBytes<D> + kk * (16 * 128)), id_o, (j | kk) != 0);
+                                }
+                                tc_commit(o_done + 8 * x);
+                            }
+                            if (j + 1 < steps[x]) {
+                                if (!have_k) { ok = mbar_wait(k_full + 8 * kstage, kphase); have_k = true; }
+                                if (!ok) break;
+                                tc_fence_after();
+                                scores(x);
+                            }
+                        }
+                        if (!ok) break;
+                        tc_commit(v_empty + 8 * vstage);
+                        if (++vstage == S) { vstage = 0; vphase ^= 1u; }
+                        if (j + 1 < n) {
+                            tc_commit(k_empty + 8 * kstage);
+                            if (j + 2 == n) tc_commit(q_empty);
+                            if (++kstage == S) { kstage = 0; kphase ^= 1u; }
+                        }
+                    }
+                }
+                next_unit(s);
+            }
+        }
+        __syncwarp();
+    } else {
+        // ---- softmax: group x (four warps) has tile x, a thread has row r of it ----
+        const int x = warp / 4, r = threadIdx.x % kRows;
+        const uint32_t lanes = uint32_t((warp % 4) * 32) << 16, s_at = tmem + lanes + x * kRows, o_at = tmem + lanes + 256 + x * kRows;
+        const int query = x * a.tile_queries + r / a.group, head = r % a.group;      // of the unit
+        const bool row_there = r < a.tile_queries * a.group;
+        uint32_t step = 0;      // scores taken
+        while (unit_at < to) {
+            const Segment s = segment();
+            if (s.t0 < s.t1) {
+                const int n = steps_of(s, x);
+                float ref = 0.f, sum = 0.f;      // the row's reference (what its probabilities are relative to) and sum
+                bool seen = false;
+                const int position = s.first + min(query, s.queries - 1), lowest = s.first + x * a.tile_queries;      // the row's, and the tile's first
+                for (int j = 0; j < n; j++) {
+                    ok = ok && mbar_wait(s_full + 8 * x, step & 1u);
+                    ok = __all_sync(0xffffffffu, ok);
+                    tc_fence_after();
+                    // The scores come in halves of 64, the second of which stays in registers; the first is read again when its turn comes (all 128 held at once
+                    // spill). Probabilities go over the second half's place.
+                    const int first = (s.t0 + j) * kRows;
+                    const bool masked = first + kRows - 1 > lowest;
+                    const int limit = position - first;
+                    uint32_t v[kHalf];
+                    auto load = [&](int half) {
+                        #pragma unroll
+                        for (int c = 0; c < kHalf; c += 32) tc_ld32(s_at + half * kHalf + c, v + c);
+                        tc_wait_ld();
+                        if (masked) {
+                            #pragma unroll
+                            for (int c = 0; c < kHalf; c++) v[c] = half * kHalf + c <= limit ? v[c] : 0xff800000u;
+                        }
+                    };
+                    float m4[4];
+                    #pragma unroll
+                    for (int half = 0; half < 2; half++) {
+                        load(half);
+                        #pragma unroll
+                        for (int c = 0; c < kHalf; c++) m4[c % 4] = half == 0 && c < 4 ? __uint_as_float(v[c]) : fmaxf(m4[c % 4], __uint_as_float(v[c]));
+                    }
+                    const float m = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * a.scale_log2;
+                    const bool grows = row_there && m > -CUDART_INF_F && (!seen || m > ref + kRescale);
+                    if (__any_sync(0xffffffffu, grows && seen)) {
+                        // outputs so far, relative to the new reference
+                        const float by = grows && seen ? ex2(ref - m) : 1.f;
+                        ok = ok && mbar_wait(o_done + 8 * x, (step - 1) & 1u);
+                        ok = __all_sync(0xffffffffu, ok);
+                        tc_fence_after();
+                        #pragma unroll
+                        for (int c = 0; c < D; c += 32) {
+                            uint32_t o[32];
+                            tc_ld32(o_at + c, o);
+                            tc_wait_ld();
+                            #pragma unroll
+                            for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * by);
+                            tc_st32(o_at + c, o);
+                        }
+                        sum *= by;
+                    }
+                    if (grows) { ref = m; seen = true; }
+                    const float minus = kLift - ref;
+                    float s4[4] = {0.f, 0.f, 0.f, 0.f};
+                    #pragma unroll
+                    for (int half = 1; half >= 0; half--) {
+                        if (half == 0) load(0);
+                        #pragma unroll
+                        for (int c = 0; c < kHalf; c += 2) {
+                            const float e0 = ex2(fmaf(__uint_as_float(v[c]), a.scale_log2, minus)), e1 = ex2(fmaf(__uint_as_float(v[c + 1]), a.scale_log2, minus));
+                            s4[c / 2 % 2 * 2] += e0;
+                            s4[c / 2 % 2 * 2 + 1] += e1;
+                            const __half2 h = __floats2half2_rn(e0, e1);
+                            v[c / 2] = *reinterpret_cast<const uint32_t *>(&h);
+                        }
+                        tc_st32(s_at + kHalf + half * 32, v);
+                    }
+                    sum += (s4[0] + s4[1]) + (s4[2] + s4[3]);
+                    tc_wait_st();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(p_full + 8 * x);
+                    step++;
+                }
+                // ---- the unit's outputs, or the segment's part of them ----
+                if (n > 0) {
+                    ok = ok && mbar_wait(o_done + 8 * x, (step - 1) & 1u);
+                    ok = __all_sync(0xffffffffu, ok);
+                    tc_fence_after();
+                }
+                const bool whole = s.t0 == 0 && s.t1 == s.tiles;
+                if (whole) {
+                    const bool mine = row_there && query < s.queries;
+                    const float by = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+                    __half * const out = a.out + ((int64_t(s.row) + query) * a.n_head + u.kvh * a.group + head) * D;
+                    if (n > 0) {
+                        #pragma unroll
+                        for (int c = 0; c < D; c += 32) {
+                            uint32_t o[32];
+                            tc_ld32(o_at + c, o);
+                            tc_wait_ld();
+                            #pragma unroll
+                            for (int i = 0; i < 32; i += 2) {
+                                const __half2 h = __floats2half2_rn(__uint_as_float(o[i]) * by, __uint_as_float(o[i + 1]) * by);
+                                o[i / 2] = *reinterpret_cast<const uint32_t *>(&h);
+                            }
+                            #pragma unroll
+                            for (int i = 0; i < 4; i++) if (mine) reinterpret_cast<uint4 *>(out + c)[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                        }
+                    }
+                } else {
+                    float * const part = a.part + ((int64_t(blockIdx.x) * 2 + (s.t0 == 0 ? 1 : 0)) * 2 + x) * kTilePart<D>;
+                    if (n > 0) {
+                        #pragma unroll
+                        for (int c = 0; c < D; c += 32) {
+                            uint32_t o[32];
+                            tc_ld32(o_at + c, o);
+                            tc_wait_ld();
+                            #pragma unroll
+                            for (int i = 0; i < 8; i++) {
+                                reinterpret_cast<uint4 *>(part)[(c / 4 + i) * kRows + r] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                            }
+                        }
+                    }
+                    // (a tile without a step in this segment leaves no outputs, and a maximum that says so)
+                    reinterpret_cast<float2 *>(part + kRows * D)[r] = make_float2(n > 0 && seen ? ref : -CUDART_INF_F, n > 0 ? sum : 0.f);
+                    tc_fence_before();
+                    __threadfence();
+                    asm volatile("bar.sync 1, 256;" ::: "memory");
+                    // the blocks that share the unit: those whose tiles are not none
+                    int b0 = int(((unit_at + 1) * blocks - 1) / total), b1 = int((s.next * blocks - 1) / total);
+                    if (tile_of(total * (b0 + 1) / blocks - unit_at, s.tiles) == 0) b0++;
+                    if (tile_of(total * b1 / blocks - unit_at, s.tiles) == s.tiles) b1--;
+                    if (threadIdx.x == 0) *flag = paged_counter_arrive(a.arrived + b0, a.call, b1 - b0 + 1, &ok);
+                    asm volatile("bar.sync 1, 256;" ::: "memory");
+                    if (*flag) {
+                        __threadfence();
+                        auto part_of = [&](int b) { return a.part + ((int64_t(b) * 2 + (b == b0 ? 1 : 0)) * 2 + x) * kTilePart<D>; };
+                        float top = -CUDART_INF_F, l = 0.f;
+                        for (int b = b0; b <= b1; b++) top = fmaxf(top, __ldcg(reinterpret_cast<const float2 *>(part_of(b) + kRows * D) + r).x);
+                        const float minus = top == -CUDART_INF_F ? 0.f : top;
+                        const bool mine = row_there && query < s.queries;
+                        for (int b = b0; b <= b1; b++) { const float2 st = __ldcg(reinterpret_cast<const float2 *>(part_of(b) + kRows * D) + r); l = fmaf(st.y, ex2(st.x - minus), l); }
+                        const float by = l > 0.f || l != l ? 1.f / l : 0.f;
+                        __half * const out = a.out + ((int64_t(s.row) + query) * a.n_head + u.kvh * a.group + head) * D;
+                        for (int c = 0; c < D / 4; c += 8) {
+                            float4 o[8] = {};
+                            for (int b = b0; b <= b1; b++) {
+                                const float * pt = part_of(b);
+                                const float st = __ldcg(reinterpret_cast<const float2 *>(pt + kRows * D) + r).x, share = ex2(st - minus);
+                                float4 w[8];
+                                #pragma unroll
+                                for (int i = 0; i < 8; i++) w[i] = st > -CUDART_INF_F ? __ldcg(reinterpret_cast<const float4 *>(pt) + (c + i) * kRows + r) : make_float4(0.f, 0.f, 0.f, 0.f);
+                                #pragma unroll
+                                for (int i = 0; i < 8; i++) {
+                                    o[i].x = fmaf(w[i].x, share, o[i].x); o[i].y = fmaf(w[i].y, share, o[i].y);
+                                    o[i].z = fmaf(w[i].z, share, o[i].z); o[i].w = fmaf(w[i].w, share, o[i].w);
+                                }
+                            }
+                            #pragma unroll
+                            for (int i = 0; i < 8; i += 2) {
+                                const __half2 h[4] = {__floats2half2_rn(o[i].x * by, o[i].y * by), __floats2half2_rn(o[i].z * by, o[i].w * by),
+                                                      __floats2half2_rn(o[i + 1].x * by, o[i + 1].y * by), __floats2half2_rn(o[i + 1].z * by, o[i + 1].w * by)};
+                                if (mine) *reinterpret_cast<uint4 *>(out + (c + i) * 4) = *reinterpret_cast<const uint4 *>(h);
+                            }
+                        }
+                    }
+                }
+                tc_fence_before();
+            }
+            next_unit(s);
+        }
+    }
+    if (!ok && lane == 0 && a.c.error) *reinterpret_cast<volatile int *>(a.c.error) = kErrorPagedWait;
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+}
+
+template <int D>
+cudaError_t launch(const Args & a, const TensorMap & qmap, const TensorMap & kmap, const TensorMap & vmap, int blocks, cudaStream_t stream) {
+    static std::atomic<uint64_t> done{0};
+    const cudaError_t e = allow_dynamic_smem(k_attention_prompt<D>, kSmem<D>, done);
+    if (e != cudaSuccess) return e;
+    return launch_pdl(k_attention_prompt<D>, dim3(unsigned(blocks)), dim3(kThreads), kSmem<D>, stream, reinterpret_cast<const CUtensorMap &>(qmap),
+                      reinterpret_cast<const CUtensorMap &>(kmap), reinterpret_cast<const CUtensorMap &>(vmap), a);
 }
 
 }  // namespace
 
-size_t attention_prompt_scratch_bytes(int, int, int) { return 256; }
+size_t attention_prompt_scratch_bytes(int, int, int head_dim) { return size_t(kMostBlocks) * (2 * 2 * kRows * (head_dim + 2) * 4 + 8); }
 
-cudaError_t launch_attention_prompt_paged(const PagedCache & cache, const void * q, void * out, int n_head, int n_rows, int n_sequences, const int32_t * sequence,
-                                          const int32_t * start, const int32_t * lengths, float scale, void *, int * error, cudaStream_t stream) {
-    const PagedView c = paged_view(cache, error);
-    const unsigned blocks = unsigned((int64_t(n_rows) * n_head + 3) / 4);
-    auto go = [&](auto kernel) {
-        kernel<<<blocks, 128, 0, stream>>>(c, static_cast<const __half *>(q), static_cast<__half *>(out), n_head, n_rows, sequence, start, lengths, n_sequences, scale);
-    };
-    if (cache.head_dim == 128) go(k_attention_prompt<128>);
-    else if (cache.head_dim == 64) go(k_attention_prompt<64>);
-    else return cudaErrorInvalidValue;
-    return cudaGetLastError();
+cudaError_t launch_attention_prompt_paged(const PagedCache & cache, const void * q, void * out, int n_head, int n_rows, int n_prompts, const int32_t * sequence,
+                                          const int32_t * start, const int32_t * lengths, float scale, void * scratch, int * error, cudaStream_t stream) {
+    Args a{};
+    a.c = paged_view(cache, error);
+    a.out = static_cast<__half *>(out);
+    a.n_head = n_head; a.group = n_head / cache.n_head_kv; a.tile_queries = kRows / a.group; a.n_prompts = n_prompts; a.n_rows = n_rows;
+    a.sequence = sequence; a.start = start; a.lengths = lengths;
+    a.scale_log2 = scale * 1.44269504f;
+    a.call = paged_call();
+    a.arrived = static_cast<unsigned long long *>(scratch);
+    a.part = reinterpret_cast<float *>(a.arrived + kMostBlocks);
+    TensorMap qmap, kmap, vmap;
+    const int box = std::min(kRows, cache.page_size);
+    cudaError_t e = make_heads_map(&qmap, q, cache.head_dim, n_head, n_rows, a.group, a.tile_queries);
+    if (e == cudaSuccess) e = make_heads_map(&kmap, cache.keys, cache.head_dim, cache.n_head_kv, int64_t(cache.n_pages) * cache.page_size, 1, box);
+    if (e == cudaSuccess) e = make_heads_map(&vmap, cache.values, cache.head_dim, cache.n_head_kv, int64_t(cache.n_pages) * cache.page_size, 1, box);
+    if (e != cudaSuccess) return e;
+    const int blocks = std::min(kMostBlocks, sm_count());
+    if (cache.head_dim == 128) return launch<128>(a, qmap, kmap, vmap, blocks, stream);
+    if (cache.head_dim == 64) return launch<64>(a, qmap, kmap, vmap, blocks, stream);
+    return cudaErrorInvalidValue;
 }
 
 }  // namespace cuda

@@ -700,14 +700,14 @@ cudaError_t make_rows_map(TensorMap * out, const void * base, int64_t rows, int6
     return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
-cudaError_t make_pages_map(TensorMap * out, const void * pool, const PagedCache & c, int box_rows) {
+cudaError_t make_heads_map(TensorMap * out, const void * base, int head_dim, int heads, int64_t rows, int box_heads, int box_rows) {
     EncodeTiledFn fn = encode_tiled();
     if (!fn) return cudaErrorNotSupported;
-    const cuuint64_t dims[3] = {cuuint64_t(c.head_dim), cuuint64_t(c.n_head_kv), cuuint64_t(c.n_pages) * cuuint64_t(c.page_size)};
-    const cuuint64_t strides[2] = {cuuint64_t(c.head_dim) * 2, cuuint64_t(c.head_dim) * 2 * cuuint64_t(c.n_head_kv)};
-    const cuuint32_t box[3] = {64u, 1u, cuuint32_t(box_rows)};
+    const cuuint64_t dims[3] = {cuuint64_t(head_dim), cuuint64_t(heads), cuuint64_t(rows)};
+    const cuuint64_t strides[2] = {cuuint64_t(head_dim) * 2, cuuint64_t(head_dim) * 2 * cuuint64_t(heads)};
+    const cuuint32_t box[3] = {64u, cuuint32_t(box_heads), cuuint32_t(box_rows)};
     const cuuint32_t estr[3] = {1u, 1u, 1u};
-    const CUresult r = fn(reinterpret_cast<CUtensorMap *>(out), CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void *>(pool), dims, strides, box, estr,
+    const CUresult r = fn(reinterpret_cast<CUtensorMap *>(out), CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void *>(base), dims, strides, box, estr,
                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }

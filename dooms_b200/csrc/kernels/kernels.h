@@ -252,9 +252,8 @@ cudaError_t make_activation_map(TensorMap * out, const void * base, int64_t rows
 // A matrix of `rows` rows of row_bytes bytes (a multiple of 16, 16-byte aligned base) as a 2-D tensor of 16-bit words, copied in boxes of box_rows rows x
 // box_bytes bytes (a multiple of 16, at most 512), no swizzle, rows past the end read as zeros.
 cudaError_t make_rows_map(TensorMap * out, const void * base, int64_t rows, int64_t row_bytes, int box_bytes, int box_rows);
-// A pool of a paged cache as a tensor (head_dim, n_head_kv, positions), copied in boxes of 64 values x one head x box_rows positions, 128-byte swizzle.
-struct PagedCache;
-cudaError_t make_pages_map(TensorMap * out, const void * pool, const PagedCache & cache, int box_rows);
+// f16 [rows][heads][head_dim] as a tensor, copied in boxes of 64 values x box_heads x box_rows, 128-byte swizzle: a row of 128 bytes for each head of each row.
+cudaError_t make_heads_map(TensorMap * out, const void * base, int head_dim, int heads, int64_t rows, int box_heads, int box_rows);
 bool gemm_tc_supported(int dt, const void * W, int64_t N, int64_t K);
 // Y[m][n] (+)= X[m] . W[n] (+ bias[n]) for M tokens; X is the f16 buffer behind xmap. With W2: silu(X . W[n]) * (X . W2[n]). Y (f32) and / or Y16 (f16)
 // receive the result. *error is set to 2 if a pipeline wait ran out.

@@ -3,6 +3,9 @@
 // position that a kernel takes from device memory is checked before an address is made of it; what fails is skipped and reported through the error word.
 #include <cuda_fp16.h>
 
+#include <atomic>
+#include <chrono>
+
 #include "kernels.h"
 
 namespace dooms {
@@ -24,6 +27,28 @@ struct PagedView {
         return (int64_t(page) << page_shift) + (at & ((1 << page_shift) - 1));
     }
 };
+
+// Arrival counters in scratch memory whose contents at the start do not matter: a counter is (a call's own number, 48 bits, not zero) << 16 | blocks that have
+// arrived. The block that owns the counter sets it up when it begins; others (behind it in the grid) wait until it carries the call's number. The last
+// one to arrive leaves zero, so that a replayed call, whose number is the same, finds no count of its own; one that nobody arrived at stays set up for the replay.
+inline unsigned long long paged_call() {
+    static std::atomic<unsigned long long> calls{(unsigned long long)(std::chrono::steady_clock::now().time_since_epoch().count()) * 0x9E3779B97F4A7C15ull >> 20};
+    unsigned long long c;
+    do c = calls.fetch_add(1, std::memory_order_relaxed) & 0xffffffffffffull; while (c == 0 || c == 0xffffffffffffull);
+    return c;
+}
+__device__ __forceinline__ void paged_counter_begin(unsigned long long * counter, unsigned long long call) {
+    if (threadIdx.x == 0 && (*reinterpret_cast<volatile unsigned long long *>(counter) >> 16) != call) atomicExch(counter, call << 16);
+}
+// One thread, behind a barrier of those whose stores it stands for and a __threadfence of each: whether it is the last of `count` to arrive.
+__device__ __forceinline__ bool paged_counter_arrive(unsigned long long * counter, unsigned long long call, int count, bool * ok) {
+    uint32_t polls = 0;
+    while ((*reinterpret_cast<volatile unsigned long long *>(counter) >> 16) != call && ++polls < (1u << 22)) {}
+    *ok = *ok && polls < (1u << 22);
+    if (!*ok || int(atomicAdd(counter, 1ull) & 0xffffu) + 1 != count) return false;
+    *reinterpret_cast<volatile unsigned long long *>(counter) = 0;
+    return true;
+}
 
 inline PagedView paged_view(const PagedCache & c, int * error) {
     int shift = 0;
