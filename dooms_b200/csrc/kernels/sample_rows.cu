@@ -4,7 +4,7 @@
 //   the token: the first whose cumulative weight e^(-g / T) exceeds u times the kept tokens' total.
 //
 // A row belongs to a cluster of up to eight blocks; each holds its share of the logits in shared memory, so that they are read once. No sort of the row: a cut
-// ("the first element at which a cumulative weight reaches a goal") is found by a histogram of 1/32 nat per bin over all blocks of the cluster, then by sorting
+// ("the first element at which a cumulative weight reaches a goal") is found by a histogram of 1/8 nat per bin over all blocks of the cluster, then by sorting
 // the few elements of the bin where the goal falls (or of all bins up to there, where they are few: then everything else is decided in that list too). A bin of
 // more than kList elements (flat logits, or many equal ones) is divided again by the bits of the logits, down to a single value, whose elements are then
 // counted out in the order of their indices.
@@ -14,6 +14,7 @@
 #include <math_constants.h>
 
 #include <algorithm>
+#include <cmath>
 
 #include "kernels.h"
 #include "launch.cuh"
@@ -26,11 +27,12 @@ using namespace dooms::dev;
 
 namespace {
 
-constexpr int kThreads = 512, kBins = 1024, kList = 1024, kMostBlocks = 8;
+constexpr int kThreads = 512, kBins = 256, kList = 512, kMostBlocks = 8;
 constexpr int kMostSlice = 32768;      // logits per block
-constexpr float kBinsPerNat = 32.f;
+constexpr float kBinsPerNat = 8.f;
+constexpr int kNearBins = 48;          // a short top-k is looked for among the logits less than 6 below the largest first
 constexpr double kNoLimit = 1e300;     // (gaps are below 2^129, or infinite)
-static_assert(kBins == 2 * kThreads && kList == 2 * kThreads, "two bins and two list elements per thread");
+static_assert(kList == kThreads && kBins <= kThreads, "one list element and at most one bin per thread");
 
 struct SampleArgs {
     const float * logits;
@@ -43,17 +45,17 @@ struct SampleArgs {
 };
 
 struct Shared {
-    unsigned long long mass[kBins];        // this block's histogram
-    uint32_t count[kBins];
-    unsigned long long local[kList];       // this block's elements of the list
+    uint32_t count[kBins], low[kBins], high[kBins];      // this block's histogram: elements, and their weights in two words
+    double power[64];                                    // 2^(-i / 64)
+    unsigned long long local[kList];                     // this block's elements of the list
     unsigned long long all[kList], sorted[kList];
-    unsigned long long warp_sum[2][kThreads / 32];
+    unsigned long long warp_sum[kThreads / 32];
     uint32_t n_local, lo_key, hi_key, index, ties;
     float top;
     // what a step leaves for all threads
-    int bin, list_to;
-    uint32_t in_bin;
-    unsigned long long before, total, total_count;
+    int bin;
+    uint32_t in_bin, up_to;
+    unsigned long long before, total;
 };
 
 __device__ __forceinline__ uint32_t key_of(float x) { const uint32_t b = __float_as_uint(x); return b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u); }
@@ -80,144 +82,154 @@ struct Row {
     uint32_t rank, blocks;
     Shared & s;
     float top;
-    // what is kept so far: elements in front of or at (key, index), and with a gap of at most `limit`
-    uint32_t cut_key = 0, cut_index = 0xffffffffu;
-    double limit = kNoLimit;
+    double top64;
+    // what is kept so far: logits of at least `least`, and in front of or at (cut, cut_index)
+    float least = -INFINITY, cut = -INFINITY;
+    uint32_t cut_index = 0;
+    bool histogram_used = false, list_used = false;      // whether other blocks may be reading this block's
 
-    __device__ bool kept(float v, int i) const {
-        if (!(v > -CUDART_INF_F)) return false;
-        const uint32_t k = key_of(v);
-        return (k > cut_key || (k == cut_key && uint32_t(first + i) <= cut_index)) && gap(v) <= limit && gap(v) < kNoLimit;
+    __device__ __forceinline__ bool kept(float v, int i) const { return v >= least && (v > cut || (v == cut && uint32_t(first + i) <= cut_index && v > -CUDART_INF_F)); }
+    __device__ __forceinline__ double gap(float v) const { return v == top ? 0.0 : top64 - double(v); }
+    __device__ __forceinline__ int bin(float v) const { return v == top ? 0 : int(fminf((top - v) * kBinsPerNat, float(kBins - 1))); }
+    // per: log2(e) / T; the weight 2^(45 - gap * per), rounded. 2^-y = 2^-n 2^(-i / 64) 2^-r with y = n + i / 64 + r: a table and the exponential's series to the
+    // fourth power (|r| <= 1/128: what is left out is 4e-14 of it)
+    __device__ __forceinline__ unsigned long long weight(float v, double per) const {
+        const double y = gap(v) * per;
+        if (!(y < 46.0)) return 0ull;
+        constexpr double kMagic = 6755399441055744.0, kLn2 = 0.69314718055994530942;      // 1.5 2^52: what is added to it is rounded to a whole number in its low bits
+        const double at = fma(y, 64.0, kMagic);
+        const uint32_t k = uint32_t(__double2loint(at));
+        const double r = fma(at - kMagic, -1.0 / 64.0, y) * -kLn2;
+        const double e = fma(fma(fma(fma(r, 1.0 / 24.0, 1.0 / 6.0), r, 0.5), r, 1.0), r, 1.0) * s.power[k & 63u];
+        const double scaled = fma(e, __hiloint2double(int((1023u + 45u - (k >> 6)) << 20), 0), 4503599627370496.0);      // + 2^52
+        return (unsigned long long)(__double_as_longlong(scaled)) & 0xfffffffffffffull;
     }
-    __device__ double gap(float v) const { return v == top ? 0.0 : double(top) - double(v); }
-    __device__ int bin(float v) const { return v == top ? 0 : int(fminf((top - v) * kBinsPerNat, float(kBins - 1))); }
-    // kind < 0: one per element; otherwise e^(-gap * kind)
-    __device__ unsigned long long weight(float v, double kind) const { return kind < 0 ? 1ull : (unsigned long long)(rint(exp(-gap(v) * kind) * 35184372088832.0)); }
 };
 
-// Inclusive sums over the block of two values per thread (its elements 2 tid and 2 tid + 1 of kBins or kList).
-__device__ void scan_pairs(unsigned long long (&v)[2], unsigned long long * warp_sum) {
+// Inclusive sums over the block of a value per thread; *total: of all.
+__device__ __forceinline__ unsigned long long scan(unsigned long long v, unsigned long long * warp_sum, unsigned long long * total) {
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    unsigned long long t = v[0] + v[1];
-    for (int d = 1; d < 32; d <<= 1) { const unsigned long long o = __shfl_up_sync(0xffffffffu, t, d); if (lane >= d) t += o; }
+    #pragma unroll
+    for (int d = 1; d < 32; d <<= 1) { const unsigned long long o = __shfl_up_sync(0xffffffffu, v, d); if (lane >= d) v += o; }
     __syncthreads();
-    if (lane == 31) warp_sum[warp] = t;
+    if (lane == 31) warp_sum[warp] = v;
     __syncthreads();
-    if (warp == 0) {
-        unsigned long long w = lane < kThreads / 32 ? warp_sum[lane] : 0;
-        for (int d = 1; d < 32; d <<= 1) { const unsigned long long o = __shfl_up_sync(0xffffffffu, w, d); if (lane >= d) w += o; }
-        if (lane < kThreads / 32) warp_sum[lane] = w;
-    }
-    __syncthreads();
-    if (warp > 0) t += warp_sum[warp - 1];
-    v[0] = t - v[1];
-    v[1] = t;
+    unsigned long long w = lane < kThreads / 32 ? warp_sum[lane] : 0;
+    #pragma unroll
+    for (int d = 1; d < kThreads / 32; d <<= 1) { const unsigned long long o = __shfl_up_sync(0xffffffffu, w, d); if (lane >= d) w += o; }
+    *total = __shfl_sync(0xffffffffu, w, kThreads / 32 - 1);
+    const unsigned long long ahead = __shfl_sync(0xffffffffu, w, max(0, warp - 1));
+    return warp ? v + ahead : v;
 }
 
 // All blocks' elements for which take(value, i) holds (at most kList of them over the cluster), sorted, into s.sorted; returns their number.
 template <class Take>
 __device__ int gather(Row & r, Take take) {
     Shared & s = r.s;
+    if (r.list_used) cluster_barrier();      // (others may still read the last one)
+    r.list_used = true;
     if (threadIdx.x == 0) s.n_local = 0;
     __syncthreads();
     for (int i = threadIdx.x; i < r.here; i += kThreads) {
-        if (take(r.x[i], i)) s.local[atomicAdd(&s.n_local, 1u)] = (unsigned long long)key_of(r.x[i]) << 32 | (0xffffffffu - uint32_t(r.first + i));
+        const float v = r.x[i];
+        if (take(v, i)) s.local[atomicAdd(&s.n_local, 1u)] = (unsigned long long)key_of(v) << 32 | (0xffffffffu - uint32_t(r.first + i));
     }
     cluster_barrier();
-    uint32_t n = 0;
+    // one element per thread: where it is, from the blocks' counts
+    uint32_t n = 0, from = 0, at = 0;
     for (uint32_t b = 0; b < r.blocks; b++) {
         const uint32_t m = ld_remote(&s.n_local, b);
-        for (uint32_t i = threadIdx.x; i < m; i += kThreads) s.all[n + i] = ld_remote(&s.local[i], b);
+        if (threadIdx.x >= n && threadIdx.x < n + m) { from = b; at = threadIdx.x - n; }
         n += m;
     }
-    cluster_barrier();
-    for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
-        const unsigned long long e = s.all[i];
+    unsigned long long mine = 0;
+    if (threadIdx.x < n) s.all[threadIdx.x] = mine = ld_remote(&s.local[at], from);
+    __syncthreads();
+    if (threadIdx.x < n) {
         uint32_t ahead = 0;
-        for (uint32_t j = 0; j < n; j++) ahead += s.all[j] > e;
-        s.sorted[ahead] = e;
+        #pragma unroll 8
+        for (uint32_t j = 0; j < n; j++) ahead += s.all[j] > mine;
+        s.sorted[ahead] = mine;
     }
     __syncthreads();
     return int(n);
 }
 
-// Where the cumulative weight (of `kind`) over the sorted list's first n elements, on top of `before`, reaches goal(total): the element's place (n: nowhere).
+// Where the cumulative weight over the sorted list's first n elements, on top of `before`, reaches goal(total): the element's place (n: nowhere). by_count: one each.
 template <class Goal>
-__device__ int place_in_list(Row & r, int n, double kind, unsigned long long before, Goal goal, unsigned long long * total) {
+__device__ int place_in_list(Row & r, int n, bool by_count, double per, unsigned long long before, Goal goal, unsigned long long * total) {
     Shared & s = r.s;
-    unsigned long long v[2];
-    #pragma unroll
-    for (int e = 0; e < 2; e++) { const int i = 2 * threadIdx.x + e; v[e] = i < n ? r.weight(value_of(uint32_t(s.sorted[i] >> 32)), kind) : 0ull; }
-    const unsigned long long own[2] = {v[0], v[1]};
-    scan_pairs(v, s.warp_sum[0]);
-    if (threadIdx.x == 0) s.bin = n;
-    if (threadIdx.x == kThreads - 1) s.total = before + v[1];
+    const int i = threadIdx.x;
+    const unsigned long long own = i < n ? (by_count ? 1ull : r.weight(value_of(uint32_t(s.sorted[i] >> 32)), per)) : 0ull;
+    unsigned long long all;
+    const unsigned long long upto = before + scan(own, s.warp_sum, &all);
+    if (i == 0) s.bin = n;
     __syncthreads();
-    *total = s.total;
-    const unsigned long long g = goal(s.total);
-    #pragma unroll
-    for (int e = 0; e < 2; e++) {
-        const int i = 2 * threadIdx.x + e;
-        if (i < n && before + v[e] >= g && before + v[e] - own[e] < g) s.bin = i;
-    }
+    *total = before + all;
+    const unsigned long long g = goal(before + all);
+    if (i < n && upto >= g && upto - own < g) s.bin = i;
     __syncthreads();
-    const int at = s.bin;
-    __syncthreads();
-    return at;
+    return s.bin;      // (written again only behind a barrier)
 }
 
-// A histogram over the kept elements that in(v, i) takes, by bin_of(v); leaves in s the first bin where the cumulative weight on top of `before` reaches
-// goal(total), what is in front of it, and how many elements it and the bins in front hold. s.bin = kBins: the goal is not reached.
+// A histogram over the kept elements that in(v) takes, by bin_of(v); leaves in s the first bin where the cumulative weight on top of `before` reaches
+// goal(total), what is in front of it, and how many elements it holds, and it and the bins in front. s.bin = kBins: the goal is not reached.
 template <class In, class BinOf, class Goal>
-__device__ void histogram(Row & r, double kind, unsigned long long before, In in, BinOf bin_of, Goal goal) {
+__device__ void histogram(Row & r, bool by_count, double per, unsigned long long before, In in, BinOf bin_of, Goal goal) {
     Shared & s = r.s;
-    for (int b = threadIdx.x; b < kBins; b += kThreads) { s.mass[b] = 0; s.count[b] = 0; }
+    if (r.histogram_used) cluster_barrier();      // (others may still read the last one)
+    r.histogram_used = true;
+    if (threadIdx.x < kBins) s.count[threadIdx.x] = s.low[threadIdx.x] = s.high[threadIdx.x] = 0;
     __syncthreads();
+    #pragma unroll 2
     for (int i = threadIdx.x; i < r.here; i += kThreads) {
         const float v = r.x[i];
         if (!r.kept(v, i) || !in(v)) continue;
         const int b = bin_of(v);
         atomicAdd(&s.count[b], 1u);
-        if (kind >= 0) atomicAdd(&s.mass[b], r.weight(v, kind));
+        if (!by_count) {      // two words: the low one's overflow is carried into the high one
+            const unsigned long long w = r.weight(v, per);
+            const uint32_t low = uint32_t(w), was = atomicAdd(&s.low[b], low), high = uint32_t(w >> 32) + (was + low < was ? 1u : 0u);
+            if (high) atomicAdd(&s.high[b], high);
+        }
     }
     cluster_barrier();
-    unsigned long long m[2] = {0, 0}, c[2] = {0, 0};
-    for (uint32_t blk = 0; blk < r.blocks; blk++) {
-        #pragma unroll
-        for (int e = 0; e < 2; e++) {
-            const int b = 2 * threadIdx.x + e;
-            c[e] += ld_remote(&s.count[b], blk);
-            if (kind >= 0) m[e] += ld_remote(&s.mass[b], blk);
+    unsigned long long m = 0;
+    uint32_t c = 0;
+    if (threadIdx.x < kBins) {
+        const int b = threadIdx.x;
+        #pragma unroll 8
+        for (uint32_t blk = 0; blk < r.blocks; blk++) {
+            c += ld_remote(&s.count[b], blk);
+            if (!by_count) m += ((unsigned long long)ld_remote(&s.high[b], blk) << 32) + ld_remote(&s.low[b], blk);
         }
+        if (by_count) m = c;
     }
-    if (kind < 0) { m[0] = c[0]; m[1] = c[1]; }
-    const unsigned long long own_m[2] = {m[0], m[1]}, own_c[2] = {c[0], c[1]};
-    scan_pairs(m, s.warp_sum[0]);
-    scan_pairs(c, s.warp_sum[1]);
-    if (threadIdx.x == kThreads - 1) { s.total = before + m[1]; s.total_count = c[1]; s.bin = kBins; }
+    unsigned long long total, elements = 0;
+    const unsigned long long upto = before + scan(m, s.warp_sum, &total);
+    total += before;
+    if (threadIdx.x == 0) { s.total = total; s.bin = kBins; }
+    const unsigned long long up_to = by_count ? upto - before : scan(c, s.warp_sum, &elements);
     __syncthreads();
-    const unsigned long long g = goal(s.total);
-    #pragma unroll
-    for (int e = 0; e < 2; e++) {
-        if (before + m[e] >= g && before + m[e] - own_m[e] < g) {
-            s.bin = 2 * threadIdx.x + e;
-            s.before = before + m[e] - own_m[e];
-            s.in_bin = uint32_t(own_c[e]);
-            s.list_to = int(min(c[e], (unsigned long long)(kList + 1)));
-        }
+    const unsigned long long g = goal(total);
+    if (upto >= g && upto - m < g) {
+        s.bin = threadIdx.x;
+        s.before = upto - m;
+        s.in_bin = c;
+        s.up_to = uint32_t(up_to);
     }
-    cluster_barrier();      // the next step may change the histogram that other blocks have read
+    __syncthreads();
 }
 
-// The element at which the cumulative weight over what is kept, past the histogram that is in s, reaches the goal: as its (key, index). The goal is reached.
-__device__ void resolve(Row & r, double kind, unsigned long long goal, uint32_t * key, uint32_t * index) {
+// The element at which the cumulative weight over what is kept, past the histogram that is in s, reaches the goal: as its (value, index). The goal is reached.
+__device__ void resolve(Row & r, bool by_count, double per, unsigned long long goal, float * value, uint32_t * index) {
     Shared & s = r.s;
     const int bin = s.bin;
     unsigned long long before = s.before;
     uint32_t count = s.in_bin, lo = 0, hi = 0xffffffffu;
     auto in = [&](float v) { const uint32_t k = key_of(v); return r.bin(v) == bin && k >= lo && k <= hi; };
     while (count > kList) {
-        __syncthreads();
+        cluster_barrier();
         if (threadIdx.x == 0) { s.lo_key = 0xffffffffu; s.hi_key = 0; }
         __syncthreads();
         uint32_t l = 0xffffffffu, h = 0;
@@ -232,9 +244,8 @@ __device__ void resolve(Row & r, double kind, unsigned long long goal, uint32_t 
         lo = 0xffffffffu;
         hi = 0;
         for (uint32_t b = 0; b < r.blocks; b++) { lo = min(lo, ld_remote(&s.lo_key, b)); hi = max(hi, ld_remote(&s.hi_key, b)); }
-        cluster_barrier();
         if (lo == hi) {      // one value: the goal falls on its m-th element in the order of the indices
-            const unsigned long long w = r.weight(value_of(lo), kind), m = (goal - before + w - 1) / w;
+            const unsigned long long w = by_count ? 1ull : r.weight(value_of(lo), per), m = (goal - before + w - 1) / w;
             uint32_t mine = 0;
             for (int i = threadIdx.x; i < r.here; i += kThreads) mine += r.kept(r.x[i], i) && key_of(r.x[i]) == lo;
             if (threadIdx.x == 0) { s.ties = 0; s.index = 0xffffffffu; }
@@ -242,91 +253,88 @@ __device__ void resolve(Row & r, double kind, unsigned long long goal, uint32_t 
             mine = __reduce_add_sync(0xffffffffu, mine);
             if (threadIdx.x % 32 == 0) atomicAdd(&s.ties, mine);
             cluster_barrier();
-            unsigned long long ahead = 0;
-            for (uint32_t b = 0; b < r.rank; b++) ahead += ld_remote(&s.ties, b);
-            if (ahead < m && m <= ahead + s.ties) {
-                unsigned long long seen = ahead;
+            unsigned long long seen = 0;
+            for (uint32_t b = 0; b < r.rank; b++) seen += ld_remote(&s.ties, b);
+            if (seen < m && m <= seen + s.ties) {
                 for (int base = 0; base < r.here; base += kThreads) {
                     const int i = base + threadIdx.x;
                     const bool is = i < r.here && r.kept(r.x[i], i) && key_of(r.x[i]) == lo;
-                    const int total = __syncthreads_count(is);
-                    if (seen + total >= m) {
-                        // the (m - seen)-th lane that holds one
-                        const uint32_t ballot = __ballot_sync(0xffffffffu, is);
-                        if (threadIdx.x % 32 == 0) s.count[threadIdx.x / 32] = __popc(ballot);
-                        __syncthreads();
-                        unsigned long long at = seen + __popc(ballot & ((1u << (threadIdx.x % 32)) - 1u)) + 1;
-                        for (int w2 = 0; w2 < int(threadIdx.x / 32); w2++) at += s.count[w2];
-                        if (is && at == m) s.index = uint32_t(r.first + i);
-                        break;
-                    }
-                    seen += total;
+                    unsigned long long here;
+                    const unsigned long long at = seen + scan(is, s.warp_sum, &here);
+                    if (is && at == m) s.index = uint32_t(r.first + i);
+                    seen += here;
+                    if (seen >= m) break;
                 }
             }
             cluster_barrier();
             uint32_t found = 0xffffffffu;
             for (uint32_t b = 0; b < r.blocks; b++) found = min(found, ld_remote(&s.index, b));
-            cluster_barrier();
-            *key = lo;
+            *value = value_of(lo);
             *index = found;
             return;
         }
-        const int shift = max(0, 32 - __clz(hi - lo) - 10);
+        const int shift = max(0, 32 - __clz(hi - lo) - 8);
         const uint32_t top = hi;
-        histogram(r, kind, before, in, [&](float v) { return int((top - key_of(v)) >> shift); }, [&](unsigned long long) { return goal; });
-        __syncthreads();
+        histogram(r, by_count, per, before, in, [&](float v) { return int((top - key_of(v)) >> shift); }, [&](unsigned long long) { return goal; });
         before = s.before;
         count = s.in_bin;
         hi = top - (uint32_t(s.bin) << shift);
         lo = max(lo, hi - min(hi, (1u << shift) - 1u));
-        __syncthreads();
     }
     const int n = gather(r, [&](float v, int i) { return r.kept(v, i) && in(v); });
     unsigned long long total;
-    const int at = place_in_list(r, n, kind, before, [&](unsigned long long) { return goal; }, &total);
+    const int at = place_in_list(r, n, by_count, per, before, [&](unsigned long long) { return goal; }, &total);
     const unsigned long long e = s.sorted[min(at, max(n - 1, 0))];
-    *key = uint32_t(e >> 32);
+    *value = value_of(uint32_t(e >> 32));
     *index = 0xffffffffu - uint32_t(e);
-    __syncthreads();
 }
 
-__global__ void __launch_bounds__(kThreads) k_sample_rows(const SampleArgs a) {
+__global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const SampleArgs a) {
     extern __shared__ __align__(16) uint8_t smem[];
     Shared & s = *reinterpret_cast<Shared *>(smem);
-    float * const x = reinterpret_cast<float *>(smem + sizeof(Shared));
+    float * const x = reinterpret_cast<float *>(smem + (sizeof(Shared) + 15) / 16 * 16);
     uint32_t rank, blocks;
     asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
     asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(blocks));
     const int row = int(blockIdx.x / blocks);
     const float * logits = a.logits + int64_t(row) * a.stride;
     const int first = int(rank) * a.slice, here = max(0, min(a.slice, a.n - first));
+    const float * from = logits + first;
+    // the share of the row into shared memory, 16 bytes at a time where it begins on such a boundary
+    const bool wide = (reinterpret_cast<uintptr_t>(from) & 15u) == 0;
+    const int quads = wide ? here / 4 : 0;
+    for (int i = threadIdx.x; i < quads; i += kThreads) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(x + 4 * i)), "l"(from + 4 * i) : "memory");
+    for (int i = 4 * quads + threadIdx.x; i < here; i += kThreads) asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(x + i)), "l"(from + i) : "memory");
+    if (threadIdx.x < 64) s.power[threadIdx.x] = exp2(double(threadIdx.x) * (-1.0 / 64.0));
+    const float t = a.temperature ? a.temperature[row] : 1.f, top_p = a.top_p ? a.top_p[row] : 1.f, min_p = a.min_p ? a.min_p[row] : 0.f, uniform = a.uniform[row];
+    const int k = a.top_k ? a.top_k[row] : 0;
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();
     float top = -CUDART_INF_F;
-    #pragma unroll 8
+    #pragma unroll 4
     for (int i = threadIdx.x; i < here; i += kThreads) {
-        float v = __ldg(logits + first + i) + 0.f;      // (one zero)
+        float v = x[i] + 0.f;                           // (one zero)
         v = v == v ? v : -CUDART_INF_F;                 // a NaN never wins
         x[i] = v;
         top = fmaxf(top, v);
     }
+    #pragma unroll
     for (int m = 16; m; m >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, m));
-    float * const tops = reinterpret_cast<float *>(s.warp_sum[0]);
+    float * const tops = reinterpret_cast<float *>(s.warp_sum);
     if (threadIdx.x % 32 == 0) tops[threadIdx.x / 32] = top;
     __syncthreads();
     if (threadIdx.x == 0) { for (int w = 1; w < kThreads / 32; w++) top = fmaxf(top, tops[w]); s.top = top; s.index = 0xffffffffu; }
     cluster_barrier();
     for (uint32_t b = 0; b < blocks; b++) top = fmaxf(top, ld_cluster(smem_u32(&s.top), b));
-    cluster_barrier();      // (s.top and the warps' values have been read)
 
-    Row r{x, first, here, rank, blocks, s, top};
-    const float t = a.temperature ? a.temperature[row] : 1.f, top_p = a.top_p ? a.top_p[row] : 1.f, min_p = a.min_p ? a.min_p[row] : 0.f;
-    const int k = a.top_k ? a.top_k[row] : 0;
+    Row r{x, first, here, rank, blocks, s, top, double(top)};
     uint32_t token = 0;
     double chance = 1.0;
     if (!(top > -CUDART_INF_F) || !(t > 0.f)) {
         // the lowest index of the largest logit; a row with nothing above the lowest: the first that is a number, with nothing to draw
         uint32_t found = 0xffffffffu;
         if (top > -CUDART_INF_F) { for (int i = threadIdx.x; i < here; i += kThreads) if (x[i] == top) { found = uint32_t(first + i); break; } }
-        else { for (int i = threadIdx.x; i < here; i += kThreads) { const float v = logits[first + i]; if (v == v) { found = uint32_t(first + i); break; } } }
+        else { for (int i = threadIdx.x; i < here; i += kThreads) { const float v = from[i]; if (v == v) { found = uint32_t(first + i); break; } } }
         found = __reduce_min_sync(0xffffffffu, found);
         if (threadIdx.x % 32 == 0) atomicMin(&s.index, found);
         cluster_barrier();
@@ -335,59 +343,65 @@ __global__ void __launch_bounds__(kThreads) k_sample_rows(const SampleArgs a) {
         if (token == 0xffffffffu) token = 0;
         chance = top > -CUDART_INF_F ? 1.0 : 0.0;
     } else {
-        const double kind_t = 1.0 / double(t);
+        constexpr double kLog2e = 1.4426950408889634074;
+        const double per_t = kLog2e / double(t);
         const bool by_k = k > 0 && k < a.n, by_p = top_p < 1.f;
-        if (min_p > 0.f) r.limit = min_p >= 1.f ? 0.0 : -log(double(min_p));
+        // min-p as the least logit kept: the smallest float whose gap is within the limit
+        const double limit = min_p > 0.f ? (min_p >= 1.f ? 0.0 : -log(double(min_p))) : kNoLimit;
+        float least = -CUDART_INF_F;
+        if (top == CUDART_INF_F) {
+            least = top;      // an infinity takes all
+        } else if (limit < kNoLimit) {
+            least = __double2float_ru(double(top) - limit);
+            while (r.gap(least) > limit) least = nextafterf(least, CUDART_INF_F);
+        }
         auto p_goal = [&](unsigned long long total) { return max(1ull, min(total, (unsigned long long)(ceil(double(top_p) * double(total))))); };
         auto u_goal = [&](unsigned long long total) {
-            const double u = double(a.uniform[row]) * double(total);
+            const double u = double(uniform) * double(total);
             return u > 0.0 ? min(total, (unsigned long long)u + 1ull) : 1ull;
         };
-        const double limit = r.limit;
         auto any = [](float) { return true; };
         auto by_gap = [&](float v) { return r.bin(v); };
         bool listed = false;
         unsigned long long total_p = 0;
+        float cut;
+        uint32_t index;
         if (by_k) {
-            r.limit = kNoLimit;
-            histogram(r, -1.0, 0, any, by_gap, [&](unsigned long long) { return (unsigned long long)k; });
+            auto k_goal = [&](unsigned long long) { return (unsigned long long)k; };
+            histogram(r, true, 0.0, 0, [&](float v) { return r.bin(v) < kNearBins; }, by_gap, k_goal);
+            if (s.bin == kBins) histogram(r, true, 0.0, 0, any, by_gap, k_goal);
             if (s.bin < kBins) {
-                listed = s.list_to <= kList;
-                if (!listed) { uint32_t ck, ci; resolve(r, -1.0, (unsigned long long)k, &ck, &ci); r.cut_key = ck; r.cut_index = ci; }
+                listed = s.up_to <= kList;
+                if (!listed) { resolve(r, true, 0.0, (unsigned long long)k, &cut, &index); r.cut = cut; r.cut_index = index; }
             }
         }
         if (by_p && !listed) {
-            r.limit = kNoLimit;
-            histogram(r, 1.0, 0, any, by_gap, p_goal);
+            histogram(r, false, kLog2e, 0, any, by_gap, p_goal);
             total_p = s.total;
-            listed = s.list_to <= kList;
-            if (!listed) { uint32_t ck, ci; resolve(r, 1.0, p_goal(total_p), &ck, &ci); r.cut_key = ck; r.cut_index = ci; }
+            listed = s.up_to <= kList;
+            if (!listed) { resolve(r, false, kLog2e, p_goal(total_p), &cut, &index); r.cut = cut; r.cut_index = index; }
         }
-        r.limit = limit;
         if (listed) {
             const int to = s.bin;
-            r.limit = kNoLimit;
             int n = gather(r, [&](float v, int i) { return r.kept(v, i) && r.bin(v) <= to; });
             if (by_k) n = min(n, k);
             unsigned long long total;
             if (by_p) {
                 const unsigned long long given = total_p;
-                const int at = place_in_list(r, n, 1.0, 0, [&](unsigned long long sum) { return p_goal(given ? given : sum); }, &total);
+                const int at = place_in_list(r, n, false, kLog2e, 0, [&](unsigned long long sum) { return p_goal(given ? given : sum); }, &total);
                 n = min(n, at + 1);
             }
-            if (limit < kNoLimit) n = max(1, min(n, __syncthreads_count(2 * int(threadIdx.x) < n && r.gap(value_of(uint32_t(s.sorted[2 * threadIdx.x] >> 32))) <= limit) +
-                                                      __syncthreads_count(2 * int(threadIdx.x) + 1 < n && r.gap(value_of(uint32_t(s.sorted[2 * threadIdx.x + 1] >> 32))) <= limit)));
-            const int at = min(place_in_list(r, n, kind_t, 0, u_goal, &total), n - 1);
+            n = max(1, min(n, __syncthreads_count(int(threadIdx.x) < n && value_of(uint32_t(s.sorted[threadIdx.x] >> 32)) >= least)));
+            const int at = min(place_in_list(r, n, false, per_t, 0, u_goal, &total), n - 1);
             const unsigned long long e = s.sorted[at];
             token = 0xffffffffu - uint32_t(e);
-            chance = double(r.weight(value_of(uint32_t(e >> 32)), kind_t)) / double(total);
+            chance = double(r.weight(value_of(uint32_t(e >> 32)), per_t)) / double(total);
         } else {
-            histogram(r, kind_t, 0, any, by_gap, u_goal);
+            r.least = least;
+            histogram(r, false, per_t, 0, any, by_gap, u_goal);
             const unsigned long long total = s.total;
-            uint32_t ck, ci;
-            resolve(r, kind_t, u_goal(total), &ck, &ci);
-            token = ci;
-            chance = double(r.weight(value_of(ck), kind_t)) / double(total);
+            resolve(r, false, per_t, u_goal(total), &cut, &token);
+            chance = double(r.weight(cut, per_t)) / double(total);
         }
     }
     if (rank == 0 && threadIdx.x == 0) {
@@ -406,11 +420,11 @@ cudaError_t launch_sample_rows(const float * logits, int64_t stride, int rows, i
     // as many blocks per row as leave each at least 2048 logits
     int blocks = 1;
     while (blocks < kMostBlocks && n > blocks * 2048) blocks *= 2;
-    const int slice = (n + blocks - 1) / blocks;
+    const int slice = ((n + blocks - 1) / blocks + 3) & ~3;      // (whole 16 bytes, so that every block's share begins as the row does)
     if (n < 1 || slice > kMostSlice) return cudaErrorInvalidValue;
-    const int bytes = int(sizeof(Shared)) + slice * 4;
+    const int bytes = int(sizeof(Shared)) + 16 + slice * 4;
     static std::atomic<uint64_t> done{0};
-    cudaError_t e = allow_dynamic_smem(k_sample_rows, int(sizeof(Shared)) + kMostSlice * 4, done);
+    cudaError_t e = allow_dynamic_smem(k_sample_rows, int(sizeof(Shared)) + 16 + kMostSlice * 4, done);
     if (e != cudaSuccess) return e;
     const SampleArgs a{logits, stride, n, slice, temperature, top_p, min_p, uniform, top_k, tokens, probability};
     cudaLaunchConfig_t cfg{};
