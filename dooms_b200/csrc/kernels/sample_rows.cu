@@ -3,11 +3,13 @@
 //   kept by top-k: the first k;  by top-p: while what is in front of a token holds less than top_p of the mass e^-g of what top-k kept;  by min-p: e^-g >= min_p;
 //   the token: the first whose cumulative weight e^(-g / T) exceeds u times the kept tokens' total.
 //
-// A row belongs to a cluster of up to eight blocks; each holds its share of the logits in shared memory, so that they are read once. No sort of the row: a cut
-// ("the first element at which a cumulative weight reaches a goal") is found by a histogram of 1/8 nat per bin over all blocks of the cluster, then by sorting
-// the few elements of the bin where the goal falls (or of all bins up to there, where they are few: then everything else is decided in that list too). A bin of
-// more than kList elements (flat logits, or many equal ones) is divided again by the bits of the logits, down to a single value, whose elements are then
-// counted out in the order of their indices.
+// A row belongs to one block, or to a cluster of up to eight that share it, as many as there are rows for: a batch of many rows is one wave of blocks that stream. The
+// first pass finds the maximum and a bound for a top-k (see there); later passes read the row from L2. A cut ("the first element at which a cumulative weight
+// reaches a goal") is found by a histogram over all blocks of the cluster, of 1/24 nat per bin up to 10 nats below m (what is further down is summed in registers, and
+// divided only if the goal falls there), then by sorting the few elements of the bin where the goal falls. As soon as little enough is left to look at (what
+// is above a top-k's bound or a min-p's limit, or in front of a goal) the blocks list it and work on the lists; and where that is at most kList elements, they
+// are sorted and everything else is decided among them. A bin of more than kList elements is divided again by the bits of the logits, down to a single value,
+// whose elements are counted out in the order of their indices.
 // Weights are 64-bit integers, e^-x 2^45 rounded (x and the exponential in 64-bit floating point): sums do not depend on the order of the atomics, and the blocks of
 // a cluster, which all work out every cut for themselves, agree on it. 2^18 logits of the largest weight still fit. What is rounded off is 2^-46 of
 // the row's largest weight per token.
@@ -28,9 +30,11 @@ using namespace dooms::dev;
 namespace {
 
 constexpr int kThreads = 512, kBins = 256, kList = 512, kMostBlocks = 8;
-constexpr int kMostSlice = 32768;      // logits per block
-constexpr float kBinsPerNat = 8.f;
-constexpr int kNearBins = 48;          // a short top-k is looked for among the logits less than 6 below the largest first
+constexpr int kMostLogits = 1 << 18;
+constexpr float kBinsPerNat = 24.f, kFarBinsPerNat = 8.f;
+constexpr int kFar = 240;              // the bin of everything from 10 nats below the largest logit on
+constexpr int kPowers = 256;
+constexpr int kNearMost = 4096;        // logits a block lists
 constexpr double kNoLimit = 1e300;     // (gaps are below 2^129, or infinite)
 static_assert(kList == kThreads && kBins <= kThreads, "one list element and at most one bin per thread");
 
@@ -46,19 +50,24 @@ struct SampleArgs {
 
 struct Shared {
     uint32_t count[kBins], low[kBins], high[kBins];      // this block's histogram: elements, and their weights in two words
-    double power[64];                                    // 2^(-i / 64)
+    double power[kPowers];                               // 2^(-i / kPowers)
     unsigned long long local[kList];                     // this block's elements of the list
     unsigned long long all[kList], sorted[kList];
     unsigned long long warp_sum[kThreads / 32];
+    float near_value[kNearMost];
+    int near_at[kNearMost];                              // where in the share
+    uint32_t n_near;
+    unsigned long long rest[2];                          // weights of what is not listed
     uint32_t n_local, lo_key, hi_key, index, ties;
-    float top;
+    float top, bound;
     // what a step leaves for all threads
     int bin;
     uint32_t in_bin, up_to;
     unsigned long long before, total;
 };
 
-__device__ __forceinline__ uint32_t key_of(float x) { const uint32_t b = __float_as_uint(x); return b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u); }
+__device__ __forceinline__ uint32_t key_of(float x) { const uint32_t b = __float_as_uint(x + 0.f);      // (one zero)
+    return b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u); }
 __device__ __forceinline__ float value_of(uint32_t k) { return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xffffffffu)); }
 __device__ __forceinline__ uint32_t map_to(uint32_t addr, uint32_t rank) {
     uint32_t at;
@@ -76,9 +85,26 @@ __device__ __forceinline__ unsigned long long ld_remote(const unsigned long long
     return v;
 }
 
+// A word of every block of the cluster, reduced: one lane per block.
+template <class F>
+__device__ __forceinline__ uint32_t of_blocks(const uint32_t * p, uint32_t blocks, uint32_t other, F reduce) {
+    const uint32_t lane = threadIdx.x % 32;
+    return reduce(lane < blocks ? ld_remote(p, lane) : other);
+}
+__device__ __forceinline__ uint32_t least_of_blocks(const uint32_t * p, uint32_t blocks) {
+    return of_blocks(p, blocks, 0xffffffffu, [](uint32_t v) { return __reduce_min_sync(0xffffffffu, v); });
+}
+__device__ __forceinline__ uint32_t most_of_blocks(const uint32_t * p, uint32_t blocks) {
+    return of_blocks(p, blocks, 0u, [](uint32_t v) { return __reduce_max_sync(0xffffffffu, v); });
+}
+
 struct Row {
-    const float * x;              // this block's logits in shared memory
-    int first, here;              // their first index, and how many
+    const float * share;          // this block's logits
+    int first, n_share;           // their first index, and how many
+    bool wide;                    // whether they begin on 16 bytes
+    const float * x;              // those at work: the share (at: nullptr), or the list
+    const int * at;
+    int here;
     uint32_t rank, blocks;
     Shared & s;
     float top;
@@ -88,23 +114,48 @@ struct Row {
     uint32_t cut_index = 0;
     bool histogram_used = false, list_used = false;      // whether other blocks may be reading this block's
 
-    __device__ __forceinline__ bool kept(float v, int i) const { return v >= least && (v > cut || (v == cut && uint32_t(first + i) <= cut_index && v > -CUDART_INF_F)); }
+    __device__ __forceinline__ uint32_t index(int i) const { return uint32_t(first + (at ? at[i] : i)); }
+    __device__ __forceinline__ bool kept(float v, int i) const { return v >= least && (v > cut || (v == cut && index(i) <= cut_index && v > -CUDART_INF_F)); }
     __device__ __forceinline__ double gap(float v) const { return v == top ? 0.0 : top64 - double(v); }
-    __device__ __forceinline__ int bin(float v) const { return v == top ? 0 : int(fminf((top - v) * kBinsPerNat, float(kBins - 1))); }
-    // per: log2(e) / T; the weight 2^(45 - gap * per), rounded. 2^-y = 2^-n 2^(-i / 64) 2^-r with y = n + i / 64 + r: a table and the exponential's series to the
-    // fourth power (|r| <= 1/128: what is left out is 4e-14 of it)
-    __device__ __forceinline__ unsigned long long weight(float v, double per) const {
-        const double y = gap(v) * per;
-        if (!(y < 46.0)) return 0ull;
+    __device__ __forceinline__ int bin(float v) const { return v == top ? 0 : int(fminf((top - v) * kBinsPerNat, float(kFar))); }
+    __device__ __forceinline__ int far_bin(float v) const { return int(fminf(fmaxf((top - v) - float(kFar) / kBinsPerNat, 0.f) * kFarBinsPerNat, float(kBins - 1))); }
+    // per: log2(e) / T; the weight 2^(45 - gap * per), rounded. 2^-y = 2^-n 2^(-i / 256) 2^-r with y = n + i / 256 + r: a table and the exponential's series to the
+    // third power (|r| <= 1/512: what is left out is 1.4e-13 of it)
+    __device__ __forceinline__ unsigned long long weight(float v, double per) const { return weight_of(gap(v) * per); }
+    __device__ __forceinline__ unsigned long long weight_of(double y) const {
         constexpr double kMagic = 6755399441055744.0, kLn2 = 0.69314718055994530942;      // 1.5 2^52: what is added to it is rounded to a whole number in its low bits
-        const double at = fma(y, 64.0, kMagic);
-        const uint32_t k = uint32_t(__double2loint(at));
-        const double r = fma(at - kMagic, -1.0 / 64.0, y) * -kLn2;
-        const double e = fma(fma(fma(fma(r, 1.0 / 24.0, 1.0 / 6.0), r, 0.5), r, 1.0), r, 1.0) * s.power[k & 63u];
-        const double scaled = fma(e, __hiloint2double(int((1023u + 45u - (k >> 6)) << 20), 0), 4503599627370496.0);      // + 2^52
-        return (unsigned long long)(__double_as_longlong(scaled)) & 0xfffffffffffffull;
+        const bool some = y < 46.0;      // (not so for a NaN either)
+        const double at = fma(y, double(kPowers), kMagic);
+        const uint32_t k = some ? uint32_t(__double2loint(at)) : 0u;
+        const double r = fma(at - kMagic, -1.0 / kPowers, y);
+        const double e = fma(fma(fma(r, -kLn2 * kLn2 * kLn2 / 6.0, kLn2 * kLn2 / 2.0), r, -kLn2), r, 1.0) * s.power[k % kPowers];
+        const double scaled = fma(e, __hiloint2double(int((1023u + 45u - k / kPowers) << 20), 0), 4503599627370496.0);      // + 2^52
+        return some ? (unsigned long long)(__double_as_longlong(scaled)) & 0xfffffffffffffull : 0ull;
     }
 };
+
+// f(value, place) for this thread's logits at work: of the share four at a time, with kAhead loads in flight.
+template <int kAhead, class F>
+__device__ __forceinline__ void each(const Row & r, F f) {
+    if (r.at || !r.wide) {
+        #pragma unroll 4
+        for (int i = threadIdx.x; i < r.here; i += kThreads) f(r.x[i], i);
+        return;
+    }
+    const int quads = r.here / 4;
+    const float4 * x4 = reinterpret_cast<const float4 *>(r.x);
+    auto four = [&](float4 v, int i) { f(v.x, 4 * i); f(v.y, 4 * i + 1); f(v.z, 4 * i + 2); f(v.w, 4 * i + 3); };
+    int i = threadIdx.x;
+    for (; i + (kAhead - 1) * kThreads < quads; i += kAhead * kThreads) {
+        float4 v[kAhead];
+        #pragma unroll
+        for (int j = 0; j < kAhead; j++) v[j] = __ldg(x4 + i + j * kThreads);
+        #pragma unroll
+        for (int j = 0; j < kAhead; j++) four(v[j], i + j * kThreads);
+    }
+    for (; i < quads; i += kThreads) four(__ldg(x4 + i), i);
+    if (4 * quads + int(threadIdx.x) < r.here) f(r.x[4 * quads + threadIdx.x], 4 * quads + int(threadIdx.x));
+}
 
 // Inclusive sums over the block of a value per thread; *total: of all.
 __device__ __forceinline__ unsigned long long scan(unsigned long long v, unsigned long long * warp_sum, unsigned long long * total) {
@@ -122,6 +173,36 @@ __device__ __forceinline__ unsigned long long scan(unsigned long long v, unsigne
     return warp ? v + ahead : v;
 }
 
+// One element per thread of what the blocks of the cluster have together, `count` of them in each: thread t's is element *at of block *from, if t is less than the
+// number that comes back.
+__device__ __forceinline__ uint32_t deal(const uint32_t * count, uint32_t blocks, uint32_t * from, uint32_t * at) {
+    const uint32_t lane = threadIdx.x % 32;
+    uint32_t upto = lane < blocks ? ld_remote(count, lane) : 0u;
+    #pragma unroll
+    for (int d = 1; d < kMostBlocks; d <<= 1) { const uint32_t o = __shfl_up_sync(0xffffffffu, upto, d); if (lane >= uint32_t(d)) upto += o; }
+    *from = 0;
+    *at = threadIdx.x;
+    #pragma unroll
+    for (uint32_t b = 0; b < kMostBlocks - 1; b++) {
+        const uint32_t end = __shfl_sync(0xffffffffu, upto, b);
+        if (threadIdx.x >= end) { *from = b + 1; *at = threadIdx.x - end; }
+    }
+    return __shfl_sync(0xffffffffu, upto, kMostBlocks - 1);
+}
+
+// The threads' elements (the first n threads have one), largest first, into s.sorted.
+__device__ __forceinline__ void sort_list(Shared & s, int n, unsigned long long mine) {
+    if (int(threadIdx.x) < n) s.all[threadIdx.x] = mine;
+    __syncthreads();
+    if (int(threadIdx.x) < n) {
+        int ahead = 0;
+        #pragma unroll 8
+        for (int j = 0; j < n; j++) ahead += s.all[j] > mine;
+        s.sorted[ahead] = mine;
+    }
+    __syncthreads();
+}
+
 // All blocks' elements for which take(value, i) holds (at most kList of them over the cluster), sorted, into s.sorted; returns their number.
 template <class Take>
 __device__ int gather(Row & r, Take take) {
@@ -130,28 +211,12 @@ __device__ int gather(Row & r, Take take) {
     r.list_used = true;
     if (threadIdx.x == 0) s.n_local = 0;
     __syncthreads();
-    for (int i = threadIdx.x; i < r.here; i += kThreads) {
-        const float v = r.x[i];
-        if (take(v, i)) s.local[atomicAdd(&s.n_local, 1u)] = (unsigned long long)key_of(v) << 32 | (0xffffffffu - uint32_t(r.first + i));
-    }
+    each<4>(r, [&](float v, int i) { if (take(v, i)) s.local[atomicAdd(&s.n_local, 1u)] = (unsigned long long)key_of(v) << 32 | (0xffffffffu - r.index(i)); });
     cluster_barrier();
-    // one element per thread: where it is, from the blocks' counts
-    uint32_t n = 0, from = 0, at = 0;
-    for (uint32_t b = 0; b < r.blocks; b++) {
-        const uint32_t m = ld_remote(&s.n_local, b);
-        if (threadIdx.x >= n && threadIdx.x < n + m) { from = b; at = threadIdx.x - n; }
-        n += m;
-    }
-    unsigned long long mine = 0;
-    if (threadIdx.x < n) s.all[threadIdx.x] = mine = ld_remote(&s.local[at], from);
-    __syncthreads();
-    if (threadIdx.x < n) {
-        uint32_t ahead = 0;
-        #pragma unroll 8
-        for (uint32_t j = 0; j < n; j++) ahead += s.all[j] > mine;
-        s.sorted[ahead] = mine;
-    }
-    __syncthreads();
+    uint32_t from, at;
+    const uint32_t n = deal(&s.n_local, r.blocks, &from, &at);
+    const unsigned long long mine = threadIdx.x < n ? ld_remote(&s.local[at], from) : 0ull;
+    sort_list(s, int(n), mine);
     return int(n);
 }
 
@@ -174,24 +239,36 @@ __device__ int place_in_list(Row & r, int n, bool by_count, double per, unsigned
 
 // A histogram over the kept elements that in(v) takes, by bin_of(v); leaves in s the first bin where the cumulative weight on top of `before` reaches
 // goal(total), what is in front of it, and how many elements it holds, and it and the bins in front. s.bin = kBins: the goal is not reached.
-template <class In, class BinOf, class Goal>
-__device__ void histogram(Row & r, bool by_count, double per, unsigned long long before, In in, BinOf bin_of, Goal goal) {
+// kSumFar: bin kFar is added up in registers (an atomic per element of the many that lie there would be the longest part of the whole row).
+// beyond: weights that are in none of the bins and behind all of them.
+template <bool kSumFar, class In, class BinOf, class Goal>
+__device__ void histogram(Row & r, bool by_count, double per, unsigned long long before, unsigned long long beyond, In in, BinOf bin_of, Goal goal) {
     Shared & s = r.s;
     if (r.histogram_used) cluster_barrier();      // (others may still read the last one)
     r.histogram_used = true;
     if (threadIdx.x < kBins) s.count[threadIdx.x] = s.low[threadIdx.x] = s.high[threadIdx.x] = 0;
     __syncthreads();
-    #pragma unroll 2
-    for (int i = threadIdx.x; i < r.here; i += kThreads) {
-        const float v = r.x[i];
-        if (!r.kept(v, i) || !in(v)) continue;
-        const int b = bin_of(v);
-        atomicAdd(&s.count[b], 1u);
+    auto add = [&](int b, uint32_t elements, unsigned long long w) {
+        atomicAdd(&s.count[b], elements);
         if (!by_count) {      // two words: the low one's overflow is carried into the high one
-            const unsigned long long w = r.weight(v, per);
             const uint32_t low = uint32_t(w), was = atomicAdd(&s.low[b], low), high = uint32_t(w >> 32) + (was + low < was ? 1u : 0u);
             if (high) atomicAdd(&s.high[b], high);
         }
+    };
+    uint32_t far = 0;
+    unsigned long long far_weight = 0;
+    each<2>(r, [&](float v, int i) {
+        if (!r.kept(v, i) || !in(v)) return;
+        const int b = bin_of(v);
+        const unsigned long long w = by_count ? 0ull : r.weight(v, per);
+        if (kSumFar && b == kFar && !r.at) { far++; far_weight += w; }
+        else add(b, 1u, w);
+    });
+    if (kSumFar) {
+        #pragma unroll
+        for (int d = 16; d; d >>= 1) far_weight += __shfl_xor_sync(0xffffffffu, far_weight, d);
+        far = __reduce_add_sync(0xffffffffu, far);
+        if (threadIdx.x % 32 == 0 && far) add(kFar, far, far_weight);
     }
     cluster_barrier();
     unsigned long long m = 0;
@@ -207,7 +284,7 @@ __device__ void histogram(Row & r, bool by_count, double per, unsigned long long
     }
     unsigned long long total, elements = 0;
     const unsigned long long upto = before + scan(m, s.warp_sum, &total);
-    total += before;
+    total += before + beyond;
     if (threadIdx.x == 0) { s.total = total; s.bin = kBins; }
     const unsigned long long up_to = by_count ? upto - before : scan(c, s.warp_sum, &elements);
     __syncthreads();
@@ -221,33 +298,31 @@ __device__ void histogram(Row & r, bool by_count, double per, unsigned long long
     __syncthreads();
 }
 
-// The element at which the cumulative weight over what is kept, past the histogram that is in s, reaches the goal: as its (value, index). The goal is reached.
-__device__ void resolve(Row & r, bool by_count, double per, unsigned long long goal, float * value, uint32_t * index) {
+// The element at which the cumulative weight over what is kept, past the histogram that is in s, reaches the goal: as its (value, index). The goal is reached in the
+// histogram's bin s.bin, whose elements in_bin takes.
+template <class InBin>
+__device__ void resolve(Row & r, bool by_count, double per, unsigned long long goal, InBin in_bin, float * value, uint32_t * index) {
     Shared & s = r.s;
-    const int bin = s.bin;
     unsigned long long before = s.before;
     uint32_t count = s.in_bin, lo = 0, hi = 0xffffffffu;
-    auto in = [&](float v) { const uint32_t k = key_of(v); return r.bin(v) == bin && k >= lo && k <= hi; };
+    auto in = [&](float v) { const uint32_t k = key_of(v); return k >= lo && k <= hi && in_bin(v); };
     while (count > kList) {
         cluster_barrier();
         if (threadIdx.x == 0) { s.lo_key = 0xffffffffu; s.hi_key = 0; }
         __syncthreads();
         uint32_t l = 0xffffffffu, h = 0;
-        for (int i = threadIdx.x; i < r.here; i += kThreads) {
-            const float v = r.x[i];
-            if (r.kept(v, i) && in(v)) { l = min(l, key_of(v)); h = max(h, key_of(v)); }
-        }
+        each<2>(r, [&](float v, int i) { if (r.kept(v, i) && in(v)) { l = min(l, key_of(v)); h = max(h, key_of(v)); } });
         l = __reduce_min_sync(0xffffffffu, l);
         h = __reduce_max_sync(0xffffffffu, h);
         if (threadIdx.x % 32 == 0) { atomicMin(&s.lo_key, l); atomicMax(&s.hi_key, h); }
         cluster_barrier();
-        lo = 0xffffffffu;
-        hi = 0;
-        for (uint32_t b = 0; b < r.blocks; b++) { lo = min(lo, ld_remote(&s.lo_key, b)); hi = max(hi, ld_remote(&s.hi_key, b)); }
+        lo = least_of_blocks(&s.lo_key, r.blocks);
+        hi = most_of_blocks(&s.hi_key, r.blocks);
         if (lo == hi) {      // one value: the goal falls on its m-th element in the order of the indices
             const unsigned long long w = by_count ? 1ull : r.weight(value_of(lo), per), m = (goal - before + w - 1) / w;
+            r.x = r.share; r.at = nullptr; r.here = r.n_share;      // (in order, as a list is not; the value says which bin)
             uint32_t mine = 0;
-            for (int i = threadIdx.x; i < r.here; i += kThreads) mine += r.kept(r.x[i], i) && key_of(r.x[i]) == lo;
+            each<2>(r, [&](float v, int i) { mine += r.kept(v, i) && key_of(v) == lo; });
             if (threadIdx.x == 0) { s.ties = 0; s.index = 0xffffffffu; }
             __syncthreads();
             mine = __reduce_add_sync(0xffffffffu, mine);
@@ -267,15 +342,13 @@ __device__ void resolve(Row & r, bool by_count, double per, unsigned long long g
                 }
             }
             cluster_barrier();
-            uint32_t found = 0xffffffffu;
-            for (uint32_t b = 0; b < r.blocks; b++) found = min(found, ld_remote(&s.index, b));
             *value = value_of(lo);
-            *index = found;
+            *index = least_of_blocks(&s.index, r.blocks);
             return;
         }
         const int shift = max(0, 32 - __clz(hi - lo) - 8);
         const uint32_t top = hi;
-        histogram(r, by_count, per, before, in, [&](float v) { return int((top - key_of(v)) >> shift); }, [&](unsigned long long) { return goal; });
+        histogram<false>(r, by_count, per, before, 0, in, [&](float v) { return int((top - key_of(v)) >> shift); }, [&](unsigned long long) { return goal; });
         before = s.before;
         count = s.in_bin;
         hi = top - (uint32_t(s.bin) << shift);
@@ -292,66 +365,87 @@ __device__ void resolve(Row & r, bool by_count, double per, unsigned long long g
 __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const SampleArgs a) {
     extern __shared__ __align__(16) uint8_t smem[];
     Shared & s = *reinterpret_cast<Shared *>(smem);
-    float * const x = reinterpret_cast<float *>(smem + (sizeof(Shared) + 15) / 16 * 16);
     uint32_t rank, blocks;
     asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
     asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(blocks));
-    const int row = int(blockIdx.x / blocks);
-    const float * logits = a.logits + int64_t(row) * a.stride;
+    const int row = int(blockIdx.x / blocks), warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const int first = int(rank) * a.slice, here = max(0, min(a.slice, a.n - first));
-    const float * from = logits + first;
-    // the share of the row into shared memory, 16 bytes at a time where it begins on such a boundary
+    const float * from = a.logits + int64_t(row) * a.stride + first;
     const bool wide = (reinterpret_cast<uintptr_t>(from) & 15u) == 0;
-    const int quads = wide ? here / 4 : 0;
-    for (int i = threadIdx.x; i < quads; i += kThreads) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(x + 4 * i)), "l"(from + 4 * i) : "memory");
-    for (int i = 4 * quads + threadIdx.x; i < here; i += kThreads) asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(x + i)), "l"(from + i) : "memory");
-    if (threadIdx.x < 64) s.power[threadIdx.x] = exp2(double(threadIdx.x) * (-1.0 / 64.0));
     const float t = a.temperature ? a.temperature[row] : 1.f, top_p = a.top_p ? a.top_p[row] : 1.f, min_p = a.min_p ? a.min_p[row] : 0.f, uniform = a.uniform[row];
     const int k = a.top_k ? a.top_k[row] : 0;
-    asm volatile("cp.async.wait_all;" ::: "memory");
-    __syncthreads();
-    float top = -CUDART_INF_F;
-    #pragma unroll 4
-    for (int i = threadIdx.x; i < here; i += kThreads) {
-        float v = x[i] + 0.f;                           // (one zero)
-        v = v == v ? v : -CUDART_INF_F;                 // a NaN never wins
-        x[i] = v;
-        top = fmaxf(top, v);
-    }
+    const bool greedy = !(t > 0.f), by_k = k > 0 && k < a.n, by_p = top_p < 1.f, by_m = min_p > 0.f;
+    if (threadIdx.x < kPowers) s.power[threadIdx.x] = exp2(double(threadIdx.x) * (-1.0 / kPowers));
+    if (threadIdx.x == 0) { s.n_near = 0; s.index = 0xffffffffu; }
+
+    // ---- the first pass: every thread's largest logit, and with them the row's ----
+    Row r{from, first, here, wide, from, nullptr, here, rank, blocks, s, 0.f, 0.0};
+    float mine = -CUDART_INF_F;
+    uint32_t mine_at = 0xffffffffu;
+    if (greedy) each<8>(r, [&](float v, int i) { if (v > mine) { mine = v; mine_at = uint32_t(first + i); } });      // (a NaN loses, and the first of equal ones wins)
+    else each<8>(r, [&](float v, int) { mine = fmaxf(mine, v); });
+    float top = mine;
     #pragma unroll
     for (int m = 16; m; m >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, m));
-    float * const tops = reinterpret_cast<float *>(s.warp_sum);
-    if (threadIdx.x % 32 == 0) tops[threadIdx.x / 32] = top;
+    // A bound for a top-k: if every warp has m = k / 16 (rounded up) threads with a logit of at least b, the row has k of them. b: the least of the warps' m-th largest.
+    // Where a total of everything is needed, m = 30: one or two in a hundred of a row of 128256 lie above the bound, whatever the logits are like.
+    const bool open = !greedy && !by_k && (by_p || !by_m), bounded = open || (by_k && k <= kThreads && !greedy);
+    float bound = -CUDART_INF_F;
+    if (bounded) {
+        float v = mine;      // sorted over the lanes, largest first
+        #pragma unroll
+        for (int size = 2; size <= 32; size *= 2) {
+            #pragma unroll
+            for (int d = size / 2; d; d /= 2) {
+                const float o = __shfl_xor_sync(0xffffffffu, v, d);
+                const bool larger_first = ((lane & size & 31) == 0) == ((lane & d) == 0);
+                v = larger_first ? fmaxf(v, o) : fminf(v, o);
+            }
+        }
+        bound = __shfl_sync(0xffffffffu, v, open ? 29 : (k + kThreads / 32 - 1) / (kThreads / 32) - 1);
+    }
+    float2 * const tops = reinterpret_cast<float2 *>(s.warp_sum);
+    if (lane == 0) tops[warp] = make_float2(top, bound);
     __syncthreads();
-    if (threadIdx.x == 0) { for (int w = 1; w < kThreads / 32; w++) top = fmaxf(top, tops[w]); s.top = top; s.index = 0xffffffffu; }
+    if (warp == 0) {
+        const float2 v = tops[lane % (kThreads / 32)];
+        top = v.x;
+        bound = v.y;
+        #pragma unroll
+        for (int m = kThreads / 64; m; m >>= 1) { top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, m)); bound = fminf(bound, __shfl_xor_sync(0xffffffffu, bound, m)); }
+        if (lane == 0) { s.top = top; s.bound = bound; }
+    }
     cluster_barrier();
-    for (uint32_t b = 0; b < blocks; b++) top = fmaxf(top, ld_cluster(smem_u32(&s.top), b));
+    top = lane < int(blocks) ? ld_cluster(smem_u32(&s.top), lane) : -CUDART_INF_F;
+    bound = lane < int(blocks) ? ld_cluster(smem_u32(&s.bound), lane) : -CUDART_INF_F;      // (each block's holds for the row)
+    #pragma unroll
+    for (int m = kMostBlocks / 2; m; m >>= 1) { top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, m)); bound = fmaxf(bound, __shfl_xor_sync(0xffffffffu, bound, m)); }
+    top = __shfl_sync(0xffffffffu, top, 0);
+    bound = __shfl_sync(0xffffffffu, bound, 0);
+    r.top = top;
+    r.top64 = double(top);
 
-    Row r{x, first, here, rank, blocks, s, top, double(top)};
     uint32_t token = 0;
     double chance = 1.0;
-    if (!(top > -CUDART_INF_F) || !(t > 0.f)) {
+    if (!(top > -CUDART_INF_F) || greedy) {
         // the lowest index of the largest logit; a row with nothing above the lowest: the first that is a number, with nothing to draw
-        uint32_t found = 0xffffffffu;
-        if (top > -CUDART_INF_F) { for (int i = threadIdx.x; i < here; i += kThreads) if (x[i] == top) { found = uint32_t(first + i); break; } }
-        else { for (int i = threadIdx.x; i < here; i += kThreads) { const float v = from[i]; if (v == v) { found = uint32_t(first + i); break; } } }
+        uint32_t found = mine == top ? mine_at : 0xffffffffu;
+        if (!(top > -CUDART_INF_F)) { found = 0xffffffffu; each<8>(r, [&](float v, int i) { if (v == v) found = min(found, uint32_t(first + i)); }); }
         found = __reduce_min_sync(0xffffffffu, found);
-        if (threadIdx.x % 32 == 0) atomicMin(&s.index, found);
+        if (lane == 0) atomicMin(&s.index, found);
         cluster_barrier();
-        token = 0xffffffffu;
-        for (uint32_t b = 0; b < blocks; b++) token = min(token, ld_remote(&s.index, b));
+        token = least_of_blocks(&s.index, blocks);
         if (token == 0xffffffffu) token = 0;
         chance = top > -CUDART_INF_F ? 1.0 : 0.0;
     } else {
         constexpr double kLog2e = 1.4426950408889634074;
         const double per_t = kLog2e / double(t);
-        const bool by_k = k > 0 && k < a.n, by_p = top_p < 1.f;
-        // min-p as the least logit kept: the smallest float whose gap is within the limit
-        const double limit = min_p > 0.f ? (min_p >= 1.f ? 0.0 : -log(double(min_p))) : kNoLimit;
+        // min-p as the least logit kept: the smallest float whose gap is within -log(min_p)
         float least = -CUDART_INF_F;
         if (top == CUDART_INF_F) {
             least = top;      // an infinity takes all
-        } else if (limit < kNoLimit) {
+        } else if (by_m) {
+            const double limit = min_p >= 1.f ? 0.0 : -log(double(min_p));
             least = __double2float_ru(double(top) - limit);
             while (r.gap(least) > limit) least = nextafterf(least, CUDART_INF_F);
         }
@@ -360,30 +454,137 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const SampleArgs a)
             const double u = double(uniform) * double(total);
             return u > 0.0 ? min(total, (unsigned long long)u + 1ull) : 1ull;
         };
-        auto any = [](float) { return true; };
-        auto by_gap = [&](float v) { return r.bin(v); };
+        // the block's logits that take(v, i) takes, as the list to work on from here
+        auto list = [&](auto take) {
+            __syncthreads();
+            if (threadIdx.x == 0) s.n_near = 0;
+            __syncthreads();
+            each<4>(r, [&](float v, int i) {
+                if (take(v, i)) {
+                    const uint32_t n = atomicAdd(&s.n_near, 1u);
+                    if (n < kNearMost) { s.near_value[n] = v; s.near_at[n] = i; }
+                }
+            });
+            __syncthreads();
+        };
+        auto use_list = [&] { r.x = s.near_value; r.at = s.near_at; r.here = int(s.n_near); };
+
+        auto sorted_up_to = [&](int to) { return gather(r, [&](float v, int i) { return r.kept(v, i) && r.bin(v) <= to; }); };
         bool listed = false;
+        int n = 0;
         unsigned long long total_p = 0;
         float cut;
         uint32_t index;
-        if (by_k) {
-            auto k_goal = [&](unsigned long long) { return (unsigned long long)k; };
-            histogram(r, true, 0.0, 0, [&](float v) { return r.bin(v) < kNearBins; }, by_gap, k_goal);
-            if (s.bin == kBins) histogram(r, true, 0.0, 0, any, by_gap, k_goal);
+        // ---- a top-k's bound, or a min-p alone, says at once what to look at ----
+        const bool alone = least > -CUDART_INF_F && !by_k && !by_p;
+        // ---- or where a total is needed: what is above the bound is listed, and the weights of the rest added up, in two steps down ----
+        bool totals = false;                          // whether rest[] is that, of weights e^(-gap per_rest / log2 e)
+        const float near = alone ? least : fmaxf(bound, -3.402823466e38f), step = float(2.0 * kLog2e / (by_p ? kLog2e : per_t)), down = near - step;
+        unsigned long long rest[2] = {0, 0};          // of everything below near, and below down
+        if (alone || bounded) {
+            if (!open) {
+                list([&](float v, int) { return v >= near; });
+            } else {
+                const double per = by_p ? kLog2e : per_t;
+                __syncthreads();
+                if (threadIdx.x == 0) { s.n_near = 0; s.rest[0] = s.rest[1] = 0; }
+                __syncthreads();
+                each<2>(r, [&](float v, int i) {
+                    const unsigned long long w = r.weight_of((r.top64 - double(v)) * per);
+                    rest[0] += v < near ? w : 0ull;
+                    rest[1] += v < down ? w : 0ull;
+                    if (v >= near) {
+                        const uint32_t n = atomicAdd(&s.n_near, 1u);
+                        if (n < kNearMost) { s.near_value[n] = v; s.near_at[n] = i; }
+                    }
+                });
+                #pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    #pragma unroll
+                    for (int d = 16; d; d >>= 1) rest[j] += __shfl_xor_sync(0xffffffffu, rest[j], d);
+                    if (lane == 0) atomicAdd(&s.rest[j], rest[j]);
+                }
+            }
+            cluster_barrier();
+            if (open) {
+                #pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    rest[j] = lane < int(blocks) ? ld_remote(&s.rest[j], lane) : 0ull;
+                    #pragma unroll
+                    for (int d = kMostBlocks / 2; d; d >>= 1) rest[j] += __shfl_xor_sync(0xffffffffu, rest[j], d);
+                    rest[j] = __shfl_sync(0xffffffffu, rest[j], 0);
+                }
+            }
+            uint32_t list_from, list_at;
+            const uint32_t n_near = deal(&s.n_near, blocks, &list_from, &list_at);
+            if (n_near <= kList && !(open && rest[0])) {
+                unsigned long long e = 0;
+                if (threadIdx.x < n_near) {
+                    const float v = __uint_as_float(ld_remote(reinterpret_cast<const uint32_t *>(s.near_value) + list_at, list_from));
+                    const uint32_t i = ld_remote(reinterpret_cast<const uint32_t *>(s.near_at) + list_at, list_from);
+                    e = (unsigned long long)key_of(v) << 32 | (0xffffffffu - (list_from * uint32_t(a.slice) + i));
+                }
+                sort_list(s, int(n_near), e);
+                n = int(n_near);
+                listed = true;
+            } else if (most_of_blocks(&s.n_near, blocks) <= kNearMost) {
+                use_list();
+                totals = open;
+            }
+        }
+        // A cut over what is kept: the histogram (of the list, or of the share, the far bin divided if the goal falls there); what is in front of the goal becomes the list
+        // where it is few enough; then the element. With totals, a goal behind the list falls on one of the two steps, which alone is divided.
+        int where = 0;      // what the histogram was of: 0 bins from the largest logit down, 1 the far bin's, 2 a step's
+        float step_top = 0.f, step_scale = 0.f, step_end = 0.f;
+        auto step_bin = [&](float v) { return int(fminf((step_top - v) * step_scale, float(kBins - 1))); };
+        auto divide = [&](bool by_count, double per, auto goal) {
+            where = 0;
+            histogram<true>(r, by_count, per, 0, totals ? rest[0] : 0ull, [](float) { return true; }, [&](float v) { return r.bin(v); }, goal);
+            if (totals && s.bin == kBins) {
+                const unsigned long long all = s.total, g = goal(all), listed_weight = all - rest[0];
+                const bool lower = g > all - rest[1];
+                where = 2;
+                step_top = lower ? down : near;
+                step_end = lower ? -CUDART_INF_F : down;
+                step_scale = lower ? 16.f / step : float(kBins) / step;
+                r.x = r.share; r.at = nullptr; r.here = r.n_share;
+                totals = false;
+                histogram<false>(r, by_count, per, lower ? all - rest[1] : listed_weight, lower ? 0ull : rest[1], [&](float v) { return v < step_top && v >= step_end; }, step_bin, goal);
+                return;
+            }
+            totals = false;
+            if (r.at) return;
+            if (s.bin == kFar) {
+                where = 1;
+                histogram<false>(r, by_count, per, s.before, 0, [&](float v) { return r.bin(v) == kFar; }, [&](float v) { return r.far_bin(v); }, goal);
+            } else if (s.bin < kBins && s.up_to > kList && s.up_to <= kNearMost) {
+                const int to = s.bin;
+                list([&](float v, int i) { return r.kept(v, i) && r.bin(v) <= to; });
+                use_list();
+            }
+        };
+        auto element = [&](bool by_count, double per, unsigned long long goal, float * value, uint32_t * index) {
+            const int bin = s.bin, w = where;
+            resolve(r, by_count, per, goal, [&](float v) {
+                return w == 0 ? r.bin(v) == bin : w == 1 ? r.bin(v) == kFar && r.far_bin(v) == bin : v < step_top && v >= step_end && step_bin(v) == bin;
+            }, value, index);
+        };
+        if (by_k && !listed) {
+            divide(true, 0.0, [&](unsigned long long) { return (unsigned long long)k; });
             if (s.bin < kBins) {
-                listed = s.up_to <= kList;
-                if (!listed) { resolve(r, true, 0.0, (unsigned long long)k, &cut, &index); r.cut = cut; r.cut_index = index; }
+                listed = where == 0 && s.up_to <= kList;
+                if (listed) n = sorted_up_to(s.bin);
+                else { element(true, 0.0, (unsigned long long)k, &cut, &index); r.cut = cut; r.cut_index = index; }
             }
         }
         if (by_p && !listed) {
-            histogram(r, false, kLog2e, 0, any, by_gap, p_goal);
+            divide(false, kLog2e, p_goal);
             total_p = s.total;
-            listed = s.up_to <= kList;
-            if (!listed) { resolve(r, false, kLog2e, p_goal(total_p), &cut, &index); r.cut = cut; r.cut_index = index; }
+            listed = where == 0 && s.up_to <= kList;
+            if (listed) n = sorted_up_to(s.bin);
+            else { element(false, kLog2e, p_goal(total_p), &cut, &index); r.cut = cut; r.cut_index = index; }
         }
         if (listed) {
-            const int to = s.bin;
-            int n = gather(r, [&](float v, int i) { return r.kept(v, i) && r.bin(v) <= to; });
             if (by_k) n = min(n, k);
             unsigned long long total;
             if (by_p) {
@@ -398,9 +599,9 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const SampleArgs a)
             chance = double(r.weight(value_of(uint32_t(e >> 32)), per_t)) / double(total);
         } else {
             r.least = least;
-            histogram(r, false, per_t, 0, any, by_gap, u_goal);
+            divide(false, per_t, u_goal);
             const unsigned long long total = s.total;
-            resolve(r, false, per_t, u_goal(total), &cut, &token);
+            element(false, per_t, u_goal(total), &cut, &token);
             chance = double(r.weight(cut, per_t)) / double(total);
         }
     }
@@ -413,18 +614,20 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const SampleArgs a)
 
 }  // namespace
 
-int sample_rows_most() { return kMostBlocks * kMostSlice; }
+int sample_rows_most() { return kMostLogits; }
 
 cudaError_t launch_sample_rows(const float * logits, int64_t stride, int rows, int n, const float * temperature, const int32_t * top_k, const float * top_p, const float * min_p,
                                const float * uniform, int32_t * tokens, float * probability, cudaStream_t stream) {
-    // as many blocks per row as leave each at least 2048 logits
+    // As many blocks per row, each of at least 2048 logits, as make up to four per SM (two are resident): a cluster costs a row its barriers, a single block leaves the
+    // rows that need a total of everything to themselves. 256 rows of 128256, top-k 40 / a mix of filters: 56 / 503 us with one block, 58 / 287 with two, 92 / 235 with
+    // four, 156 / 287 with eight.
     int blocks = 1;
-    while (blocks < kMostBlocks && n > blocks * 2048) blocks *= 2;
+    while (blocks < kMostBlocks && n > blocks * 2048 && int64_t(rows) * blocks * 2 <= 4 * sm_count()) blocks *= 2;
     const int slice = ((n + blocks - 1) / blocks + 3) & ~3;      // (whole 16 bytes, so that every block's share begins as the row does)
-    if (n < 1 || slice > kMostSlice) return cudaErrorInvalidValue;
-    const int bytes = int(sizeof(Shared)) + 16 + slice * 4;
+    if (n < 1 || n > kMostLogits) return cudaErrorInvalidValue;
+    constexpr int bytes = int(sizeof(Shared));
     static std::atomic<uint64_t> done{0};
-    cudaError_t e = allow_dynamic_smem(k_sample_rows, int(sizeof(Shared)) + 16 + kMostSlice * 4, done);
+    cudaError_t e = allow_dynamic_smem(k_sample_rows, bytes, done);
     if (e != cudaSuccess) return e;
     const SampleArgs a{logits, stride, n, slice, temperature, top_p, min_p, uniform, top_k, tokens, probability};
     cudaLaunchConfig_t cfg{};
