@@ -156,6 +156,14 @@ std::mutex g_argmax_noalloc_mutex;
 
 bool matrix_dtype(int32_t dt) { return dt == DOOMS_F16 || dt == DOOMS_Q4_0 || dt == DOOMS_Q5_0 || dt == DOOMS_Q8_0 || dt == DOOMS_Q4_K || dt == DOOMS_Q6_K; }
 
+// The first call of a process may be made while the thread captures a graph: what it sets up (the error word, a kernel's shared-memory limit, the kernel's own loading)
+// belongs to no stream, but a capture in CUDA's global mode forbids it unless this thread says that it knows.
+struct SetUpUnderCapture {
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    SetUpUnderCapture() { (void)cudaThreadExchangeStreamCaptureMode(&mode); }
+    ~SetUpUnderCapture() { (void)cudaThreadExchangeStreamCaptureMode(&mode); }
+};
+
 // Every pointer has to be memory that kernels of the current device can use: a pointer of another device, or plain host memory, would fault in the kernel.
 int32_t check_device(const char * what, std::initializer_list<const void *> pointers) {
     int dev = 0;
@@ -909,6 +917,7 @@ DOOMS_CUDA_API int32_t dooms_cuda_rope_store_paged(const dooms_cuda_paged_cache 
     if (!d_qkv || !d_sequence || !d_at || !d_positions || !d_q || n_rows < 0 || qkv_stride < row || qkv_stride % 4 != 0 || !aligned16(d_qkv) || !aligned16(d_q)) {
         return fail(DOOMS_INVALID_ARGUMENT, "rope_store_paged: a NULL or unaligned pointer, a negative n_rows, or a qkv_stride that is no multiple of 4 or shorter than a row");
     }
+    const SetUpUnderCapture relaxed;
     code = check_device("rope_store_paged", {c.keys, c.values, c.page_table, d_qkv, d_sequence, d_at, d_positions, d_q});
     if (code != DOOMS_OK) return code;
     return launch_result(cuda::launch_rope_store_paged(c, r, d_qkv, qkv_stride, n_head, n_rows, d_sequence, d_at, d_positions, d_q, q_dtype == DOOMS_F16, kernel_error_word(),
@@ -933,6 +942,7 @@ DOOMS_CUDA_API int32_t dooms_cuda_attention_paged(const dooms_cuda_paged_cache *
         return fail(DOOMS_INVALID_ARGUMENT, "attention_paged: a NULL or unaligned pointer, a negative size, or a scale that is negative or not finite");
     }
     if (scratch_bytes < dooms_cuda_attention_paged_scratch_bytes(n_head, c.n_head_kv, c.head_dim)) return fail(DOOMS_RESOURCE_EXHAUSTED, "attention_paged: the scratch is too small");
+    const SetUpUnderCapture relaxed;
     code = check_device("attention_paged", {c.keys, c.values, c.page_table, d_q, d_sequence, d_lengths, d_out, d_scratch});
     if (code != DOOMS_OK) return code;
     return launch_result(cuda::launch_attention_paged(c, d_q, d_out, dtype == DOOMS_F16, n_head, n_rows, d_sequence, d_lengths, max_length,
@@ -952,6 +962,7 @@ DOOMS_CUDA_API int32_t dooms_cuda_attention_prompt_paged(const dooms_cuda_paged_
         return fail(DOOMS_INVALID_ARGUMENT, "attention_prompt_paged: a NULL or unaligned pointer, one buffer as input and output, a negative size, or a scale that is negative or not finite");
     }
     if (scratch_bytes < dooms_cuda_attention_paged_scratch_bytes(n_head, c.n_head_kv, c.head_dim)) return fail(DOOMS_RESOURCE_EXHAUSTED, "attention_prompt_paged: the scratch is too small");
+    const SetUpUnderCapture relaxed;
     code = check_device("attention_prompt_paged", {c.keys, c.values, c.page_table, d_q, d_sequence, d_start, d_lengths, d_out, d_scratch});
     if (code != DOOMS_OK) return code;
     return launch_result(cuda::launch_attention_prompt_paged(c, d_q, d_out, n_head, n_rows, n_prompts, d_sequence, d_start, d_lengths,
@@ -967,6 +978,7 @@ DOOMS_CUDA_API int32_t dooms_cuda_sample_rows(const float * d_logits, int64_t st
     }
     if (n > cuda::sample_rows_most()) return fail(DOOMS_UNSUPPORTED, "sample_rows: rows of at most " + std::to_string(cuda::sample_rows_most()) + " logits");
     if (rows > (1 << 24)) return fail(DOOMS_INVALID_ARGUMENT, "sample_rows: at most 2^24 rows");
+    const SetUpUnderCapture relaxed;
     const int32_t code = check_device("sample_rows", {d_logits, d_temperature, d_top_k, d_top_p, d_min_p, d_uniform, d_tokens, d_probability});
     if (code != DOOMS_OK) return code;
     return launch_result(cuda::launch_sample_rows(d_logits, stride, rows, n, d_temperature, d_top_k, d_top_p, d_min_p, d_uniform, d_tokens, d_probability,

@@ -405,6 +405,37 @@ def test_attention_captured_replayed_and_on_another_stream():
     assert status() == (L.OK, 0)
 
 
+@gpu
+def test_a_process_whose_first_calls_are_captured():
+    """What the first call sets up is set up under a capture too: in a process of its own, all four calls in a graph, then replayed."""
+    import subprocess
+    import sys
+    from pathlib import Path
+    code = """
+import torch
+from dooms_b200 import paged
+keys, values = (torch.randn(8, 16, 2, 64, device="cuda").half() for _ in range(2))
+cache = paged.PagedCache(keys, values, torch.arange(8, dtype=torch.int32, device="cuda").view(2, 4))
+scratch = torch.empty(cache.scratch_bytes(4), dtype=torch.uint8, device="cuda")
+seq, at, start = torch.arange(2, dtype=torch.int32, device="cuda"), torch.full((2,), 20, dtype=torch.int32, device="cuda"), torch.arange(3, dtype=torch.int32, device="cuda")
+qkv, q, out, q16, out16 = torch.randn(2, 512, device="cuda"), *(torch.zeros(2, 4, 64, device="cuda") for _ in range(2)), *(torch.zeros(2, 4, 64, device="cuda").half() for _ in range(2))
+logits, u, tokens = torch.randn(2, 1000, device="cuda"), torch.rand(2, device="cuda"), torch.full((2,), -1, dtype=torch.int32, device="cuda")
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    s = torch.cuda.current_stream().cuda_stream
+    cache.rope_store(qkv, seq, at, at[None], q, base=1e4, neox=True, stream=s)
+    cache.attention(q, seq, at + 1, 64, out, scratch, stream=s)
+    cache.attention_prompt(q16, seq, start, at + 1, out16, scratch, stream=s)
+    paged.sample_rows(logits, u, tokens, stream=s)
+graph.replay()
+torch.cuda.synchronize()
+assert (q != 0).any() and (out != 0).all() and (out16 != 0).all() and (tokens >= 0).all()
+print("captured")
+"""
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300, cwd=Path(__file__).resolve().parent.parent)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
+
+
 # ---------------------------------------------------------------- packed prompts
 
 def check_prompt(cache, new, lengths, H, gaps=(0, 0), scale=0.0, idle=(), every=1, seed=2, sequences=None):
