@@ -61,6 +61,11 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap * ma
                  ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
 }
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ bool elect_one() {
+    uint32_t one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+    return one != 0;
+}
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_commit(uint32_t bar) {
@@ -87,9 +92,16 @@ __device__ __forceinline__ void tc_st32(uint32_t at, const uint32_t * r) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};"
                  ::W8(r, 0), W8(r, 8), W8(r, 16), W8(r, 24), "r"(at) : "memory");
 }
+__device__ __forceinline__ void tc_st16(uint32_t at, const uint32_t * r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::W8(r, 0), W8(r, 8), "r"(at) : "memory");
+}
 #undef R8
 #undef W8
 __device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// Ties what tc_ld32 loaded to the wait in front of this: nothing that uses it can be moved before it.
+#define T8(r, i) "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]), "+r"(r[i + 6]), "+r"(r[i + 7])
+__device__ __forceinline__ void tie32(uint32_t * r) { asm volatile("" : T8(r, 0), T8(r, 8), T8(r, 16), T8(r, 24)); }
+#undef T8
 __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 // Operand tiles of 128-byte rows in the 128-byte swizzle, groups of 8 rows 1024 bytes apart. K-major (Q, K): a row is 64 values of the reduction, a slice of 16 of
 // them is addressed by its byte offset. N-major (V): a row is one key and 64 of the outputs' columns, the next 64 columns lie a whole tile half further.
@@ -101,6 +113,26 @@ __device__ __forceinline__ uint64_t desc_n(uint32_t at) {
 constexpr uint32_t idesc(int n, bool n_major) { return (1u << 4) | (n_major ? 1u << 16 : 0u) | (uint32_t(n >> 3) << 17) | (uint32_t(kRows >> 4) << 24); }
 
 __device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+
+// Two f32 at a time.
+__device__ __forceinline__ uint64_t pair(float a, float b) { uint64_t r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b)); return r; }
+__device__ __forceinline__ void halves(uint64_t v, float & a, float & b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) { uint64_t r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) { uint64_t r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+// 2^x of a pair without the special function unit: x = n + f, f in [-1/2, 1/2], a polynomial for 2^f (relative error 4e-6, fitted to it), n added to the exponent. Below
+// -120 it stays at 2^-120, which is nothing beside a probability.
+__device__ __forceinline__ void ex2_pair(uint64_t x, float & a, float & b) {
+    float xa, xb;
+    halves(x, xa, xb);
+    const uint64_t y = pair(fmaxf(xa, -120.f), fmaxf(xb, -120.f)), magic = pair(12582912.f, 12582912.f), t = add2(y, magic);      // 1.5 2^23: n is in the low bits
+    const uint64_t f = fma2(add2(t, pair(-12582912.f, -12582912.f)), pair(-1.f, -1.f), y);
+    const uint64_t p = fma2(fma2(fma2(fma2(f, pair(0.009582852013409138f, 0.009582852013409138f), pair(0.055906426161527634f, 0.055906426161527634f)), f, pair(0.24024099111557007f, 0.24024099111557007f)), f, pair(0.6931241750717163f, 0.6931241750717163f)), f, pair(1.f, 1.f));
+    float ta, tb, pa, pb;
+    halves(t, ta, tb);
+    halves(p, pa, pb);
+    a = xa == xa ? __uint_as_float(__float_as_uint(pa) + (__float_as_uint(ta) << 23)) : xa;
+    b = xb == xb ? __uint_as_float(__float_as_uint(pb) + (__float_as_uint(tb) << 23)) : xb;
+}
 
 // ---- the line of units ----
 // The part of prompt i that has something to see: its first row, its queries, the keys in front of its first query; no queries for one that is idle or out of range.
@@ -136,7 +168,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention_prompt(const __grid_c
     const uint32_t bars = smem_u32(sums + kThreads + 16);
     const uint32_t q_full = bars, q_empty = bars + 8, s_full = bars + 16, p_full = bars + 32, o_done = bars + 48, k_full = bars + 64, k_empty = k_full + 8 * S, v_full = k_empty + 8 * S,
                    v_empty = v_full + 8 * S, v_fixed = v_empty + 8 * S, tmem_slot = v_fixed + 8 * S;
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;      // (a warp's number, as something the whole warp has)
     if (threadIdx.x == 0) {
         mbar_init(q_full, 1); mbar_init(q_empty, 1);
         for (int x = 0; x < 2; x++) { mbar_init(s_full + 8 * x, 1); mbar_init(p_full + 8 * x, 4); mbar_init(o_done + 8 * x, 1); }
@@ -182,6 +214,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention_prompt(const __grid_c
     tc_fence_after();
     uint32_t tmem;
     asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(tmem_slot));
+    tmem = __shfl_sync(0xffffffffu, tmem, 0);
 
     const int64_t from = total * blockIdx.x / blocks, to = total * (blockIdx.x + 1) / blocks;
     Unit u;
@@ -285,72 +318,88 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention_prompt(const __grid_c
             next_unit(s);
         }
     } else if (warp == 9) {
-        // ---- the MMAs ----
-        if (lane == 0) {
-            constexpr uint32_t id_s = idesc(kRows, false), id_o = idesc(D, true);
-            int kstage = 0, vstage = 0, units = 0;
-            uint32_t kphase = 0, vphase = 0, fixed = 0, done[2] = {0, 0};      // fixed: the phases of v_fixed, a bit per stage; done: probabilities taken
-            auto scores = [&](int x) {
+        // ---- the MMAs: the whole warp walks the steps, so that what describes them stays uniform; one elected thread issues ----
+        constexpr uint32_t id_s = idesc(kRows, false), id_o = idesc(D, true);
+        int kstage = 0, vstage = 0, units = 0;
+        uint32_t kphase = 0, vphase = 0, fixed = 0, done0 = 0, done1 = 0;      // fixed: the phases of v_fixed, a bit per stage; done: probabilities taken
+        const bool leader = elect_one();
+        auto scores = [&](int x) {
+            const uint32_t q = q_at + x * kTileBytes<D>, k = k_at + kstage * kTileBytes<D>, d = tmem + x * kRows;
+            if (leader) {
                 #pragma unroll
                 for (int kk = 0; kk < D / 16; kk++) {
                     const uint32_t at = (kk / 4) * (kRows * 128) + (kk % 4) * 32;
-                    mma_ss(tmem + x * kRows, desc_k(q_at + x * kTileBytes<D> + at), desc_k(k_at + kstage * kTileBytes<D> + at), id_s, kk != 0);
+                    mma_ss(d, desc_k(q + at), desc_k(k + at), id_s, kk != 0);
                 }
                 tc_commit(s_full + 8 * x);
-            };
-            while (unit_at < to && ok) {
-                const Segment s = segment();
-                const int n = s.t1 - s.t0;
-                if (n > 0) {
-                    const int steps[2] = {steps_of(s, 0), steps_of(s, 1)};
-                    ok = mbar_wait(q_full, uint32_t(units & 1)) && mbar_wait(k_full + 8 * kstage, kphase);
-                    if (!ok) break;
-                    units++;
-                    tc_fence_after();
-                    for (int x = 0; x < 2; x++) if (steps[x] > 0) scores(x);
-                    tc_commit(k_empty + 8 * kstage);
-                    if (n == 1) tc_commit(q_empty);
-                    if (++kstage == S) { kstage = 0; kphase ^= 1u; }
-                    for (int j = 0; j < n && ok; j++) {
-                        bool have_v = false, have_k = false;
-                        for (int x = 0; x < 2 && ok; x++) {
-                            if (j < steps[x]) {
-                                ok = mbar_wait(p_full + 8 * x, done[x] & 1u);
-                                if (ok && !have_v) {
-                                    ok = mbar_wait(v_full + 8 * vstage, vphase);
-                                    if (ok && s.keys - (s.t0 + j) * kRows < kRows) { ok = mbar_wait(v_fixed + 8 * vstage, fixed >> vstage & 1u); fixed ^= 1u << vstage; }
-                                    have_v = true;
-                                }
-                                if (!ok) break;
-                                done[x]++;
-                                tc_fence_after();
-                                #pragma unroll
-                                for (int kk = 0; kk < kRows / 16; kk++) {
-                                    mma_ts(tmem + 256 + x * kRows, tmem + x * kRows + kHalf + kk * 8, desc_n(v_at + vstage * kTileBytes<D> + kk * (16 * 128)), id_o, (j | kk) != 0);
-                                }
-                                tc_commit(o_done + 8 * x);
+            }
+            __syncwarp();
+        };
+        auto outputs = [&](int x, bool add) {
+            const uint32_t v = v_at + vstage * kTileBytes<D>, p16 = tmem + x * kRows + kHalf, d = tmem + 256 + x * kRows;
+            if (leader) {
+                #pragma unroll
+                for (int kk = 0; kk < kRows / 16; kk++) mma_ts(d, p16 + kk * 8, desc_n(v + kk * (16 * 128)), id_o, add || kk != 0);
+                tc_commit(o_done + 8 * x);
+            }
+            __syncwarp();
+        };
+        auto commit = [&](uint32_t bar) {
+            if (leader) tc_commit(bar);
+            __syncwarp();
+        };
+        auto wait = [&](uint32_t bar, uint32_t parity) {
+            ok = mbar_wait(bar, parity);
+            ok = __all_sync(0xffffffffu, ok);
+            return ok;
+        };
+        while (unit_at < to && ok) {
+            const Segment s = segment();
+            const int n = s.t1 - s.t0;
+            if (n > 0) {
+                const int steps0 = steps_of(s, 0), steps1 = steps_of(s, 1);
+                if (!wait(q_full, uint32_t(units & 1)) || !wait(k_full + 8 * kstage, kphase)) break;
+                units++;
+                tc_fence_after();
+                if (steps0 > 0) scores(0);
+                if (steps1 > 0) scores(1);
+                commit(k_empty + 8 * kstage);
+                if (n == 1) commit(q_empty);
+                if (++kstage == S) { kstage = 0; kphase ^= 1u; }
+                for (int j = 0; j < n && ok; j++) {
+                    bool have_v = false, have_k = false;
+                    #pragma unroll
+                    for (int x = 0; x < 2; x++) {
+                        const int steps = x ? steps1 : steps0;
+                        if (ok && j < steps) {
+                            if (!wait(p_full + 8 * x, (x ? done1 : done0) & 1u)) break;
+                            if (!have_v) {
+                                if (!wait(v_full + 8 * vstage, vphase)) break;
+                                if (s.keys - (s.t0 + j) * kRows < kRows) { if (!wait(v_fixed + 8 * vstage, fixed >> vstage & 1u)) break; fixed ^= 1u << vstage; }
+                                have_v = true;
                             }
-                            if (j + 1 < steps[x]) {
-                                if (!have_k) { ok = mbar_wait(k_full + 8 * kstage, kphase); have_k = true; }
-                                if (!ok) break;
-                                tc_fence_after();
-                                scores(x);
-                            }
+                            if (x) done1++; else done0++;
+                            tc_fence_after();
+                            outputs(x, j != 0);
                         }
-                        if (!ok) break;
-                        tc_commit(v_empty + 8 * vstage);
-                        if (++vstage == S) { vstage = 0; vphase ^= 1u; }
-                        if (j + 1 < n) {
-                            tc_commit(k_empty + 8 * kstage);
-                            if (j + 2 == n) tc_commit(q_empty);
-                            if (++kstage == S) { kstage = 0; kphase ^= 1u; }
+                        if (ok && j + 1 < steps) {
+                            if (!have_k) { if (!wait(k_full + 8 * kstage, kphase)) break; have_k = true; }
+                            tc_fence_after();
+                            scores(x);
                         }
                     }
+                    if (!ok) break;
+                    commit(v_empty + 8 * vstage);
+                    if (++vstage == S) { vstage = 0; vphase ^= 1u; }
+                    if (j + 1 < n) {
+                        commit(k_empty + 8 * kstage);
+                        if (j + 2 == n) commit(q_empty);
+                        if (++kstage == S) { kstage = 0; kphase ^= 1u; }
+                    }
                 }
-                next_unit(s);
             }
+            next_unit(s);
         }
-        __syncwarp();
     } else {
         // ---- softmax: group x (four warps) has tile x, a thread has row r of it ----
         const int x = warp / 4, r = threadIdx.x % kRows;
@@ -369,27 +418,34 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention_prompt(const __grid_c
                     ok = ok && mbar_wait(s_full + 8 * x, step & 1u);
                     ok = __all_sync(0xffffffffu, ok);
                     tc_fence_after();
-                    // The scores come in halves of 64, the second of which stays in registers; the first is read again when its turn comes (all 128 held at once
-                    // spill). Probabilities go over the second half's place.
+                    // The scores come in quarters of 32, the last two of which stay in registers; the first two are read again behind the work on those (all 128 held
+                    // at once spill). Probabilities go over the second half's place, last quarter first.
                     const int first = (s.t0 + j) * kRows;
                     const bool masked = first + kRows - 1 > lowest;
                     const int limit = position - first;
-                    uint32_t v[kHalf];
-                    auto load = [&](int half) {
-                        #pragma unroll
-                        for (int c = 0; c < kHalf; c += 32) tc_ld32(s_at + half * kHalf + c, v + c);
-                        tc_wait_ld();
+                    uint32_t va[32], vb[32];
+                    auto mask = [&](uint32_t (&v)[32], int c0) {
                         if (masked) {
                             #pragma unroll
-                            for (int c = 0; c < kHalf; c++) v[c] = half * kHalf + c <= limit ? v[c] : 0xff800000u;
+                            for (int c = 0; c < 32; c++) v[c] = c0 + c <= limit ? v[c] : 0xff800000u;
                         }
                     };
                     float m4[4];
                     #pragma unroll
                     for (int half = 0; half < 2; half++) {
-                        load(half);
+                        tc_ld32(s_at + half * kHalf, va);
+                        tc_ld32(s_at + half * kHalf + 32, vb);
+                        tc_wait_ld();
+                        tie32(va);
+                        tie32(vb);
+                        mask(va, half * kHalf);
+                        mask(vb, half * kHalf + 32);
                         #pragma unroll
-                        for (int c = 0; c < kHalf; c++) m4[c % 4] = half == 0 && c < 4 ? __uint_as_float(v[c]) : fmaxf(m4[c % 4], __uint_as_float(v[c]));
+                        for (int c = 0; c < 32; c += 2) {
+                            const float v0 = fmaxf(__uint_as_float(va[c]), __uint_as_float(va[c + 1])), v1 = fmaxf(__uint_as_float(vb[c]), __uint_as_float(vb[c + 1]));
+                            m4[c / 2 % 2] = half == 0 && c < 4 ? v0 : fmaxf(m4[c / 2 % 2], v0);
+                            m4[2 + c / 2 % 2] = half == 0 && c < 4 ? v1 : fmaxf(m4[2 + c / 2 % 2], v1);
+                        }
                     }
                     const float m = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * a.scale_log2;
                     const bool grows = row_there && m > -CUDART_INF_F && (!seen || m > ref + kRescale);
@@ -404,6 +460,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention_prompt(const __grid_c
                             uint32_t o[32];
                             tc_ld32(o_at + c, o);
                             tc_wait_ld();
+                            tie32(o);
                             #pragma unroll
                             for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * by);
                             tc_st32(o_at + c, o);
@@ -412,20 +469,45 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention_prompt(const __grid_c
                     }
                     if (grows) { ref = m; seen = true; }
                     const float minus = kLift - ref;
-                    float s4[4] = {0.f, 0.f, 0.f, 0.f};
-                    #pragma unroll
-                    for (int half = 1; half >= 0; half--) {
-                        if (half == 0) load(0);
+                    uint64_t sums[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
+                    const uint64_t scale2 = pair(a.scale_log2, a.scale_log2), minus2 = pair(minus, minus);
+                    // 32 probabilities from their scores, as f16 pairs in the first half of v: a quarter of them by the polynomial
+                    auto powers = [&](uint32_t (&v)[32]) {
                         #pragma unroll
-                        for (int c = 0; c < kHalf; c += 2) {
-                            const float e0 = ex2(fmaf(__uint_as_float(v[c]), a.scale_log2, minus)), e1 = ex2(fmaf(__uint_as_float(v[c + 1]), a.scale_log2, minus));
-                            s4[c / 2 % 2 * 2] += e0;
-                            s4[c / 2 % 2 * 2 + 1] += e1;
+                        for (int c = 0; c < 32; c += 2) {
+                            const uint64_t y = fma2(pair(__uint_as_float(v[c]), __uint_as_float(v[c + 1])), scale2, minus2);
+                            float e0, e1;
+                            if (c % 8 == 6) {
+                                ex2_pair(y, e0, e1);
+                            } else {
+                                halves(y, e0, e1);
+                                e0 = ex2(e0);
+                                e1 = ex2(e1);
+                            }
+                            sums[c / 2 % 2] = add2(sums[c / 2 % 2], pair(e0, e1));
                             const __half2 h = __floats2half2_rn(e0, e1);
                             v[c / 2] = *reinterpret_cast<const uint32_t *>(&h);
                         }
-                        tc_st32(s_at + kHalf + half * 32, v);
-                    }
+                    };
+                    powers(vb);
+                    tc_st16(s_at + kHalf + 48, vb);
+                    tc_ld32(s_at + 32, vb);
+                    powers(va);
+                    tc_st16(s_at + kHalf + 32, va);
+                    tc_wait_ld();
+                    tie32(vb);
+                    tc_ld32(s_at, va);
+                    mask(vb, 32);
+                    powers(vb);
+                    tc_st16(s_at + kHalf + 16, vb);
+                    tc_wait_ld();
+                    tie32(va);
+                    mask(va, 0);
+                    powers(va);
+                    tc_st16(s_at + kHalf, va);
+                    float s4[4];
+                    halves(sums[0], s4[0], s4[1]);
+                    halves(sums[1], s4[2], s4[3]);
                     sum += (s4[0] + s4[1]) + (s4[2] + s4[3]);
                     tc_wait_st();
                     tc_fence_before();
@@ -450,6 +532,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention_prompt(const __grid_c
                             uint32_t o[32];
                             tc_ld32(o_at + c, o);
                             tc_wait_ld();
+                            tie32(o);
                             #pragma unroll
                             for (int i = 0; i < 32; i += 2) {
                                 const __half2 h = __floats2half2_rn(__uint_as_float(o[i]) * by, __uint_as_float(o[i + 1]) * by);
@@ -467,6 +550,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention_prompt(const __grid_c
                             uint32_t o[32];
                             tc_ld32(o_at + c, o);
                             tc_wait_ld();
+                            tie32(o);
                             #pragma unroll
                             for (int i = 0; i < 8; i++) {
                                 reinterpret_cast<uint4 *>(part)[(c / 4 + i) * kRows + r] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
