@@ -53,7 +53,7 @@ struct Args {
 template <int D> constexpr int kTilePart = kRows * (D + 2);
 template <int D> constexpr int kTileBytes = kRows * D * 2;
 template <int D> constexpr int kRing = D == 128 ? 2 : 4;          // stages of K, and of V
-template <int D> constexpr int kSmem = 1024 + 2 * kTileBytes<D> + 2 * kRing<D> * kTileBytes<D> + (kThreads + 16) * 8 + 256;
+template <int D> constexpr int kSmem = 1024 + 2 * kTileBytes<D> + 2 * kRing<D> * kTileBytes<D> + (kThreads + 16) * 8 + 256 + 8 * 2048;
 
 // ---- tcgen05 and copies ----
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap * map, int x, int y, int z, uint32_t bar) {
@@ -114,6 +114,7 @@ constexpr uint32_t idesc(int n, bool n_major) { return (1u << 4) | (n_major ? 1u
 
 __device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 
+__device__ __forceinline__ float max3(float a, float b, float c) { float r; asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c)); return r; }
 // Two f32 at a time.
 __device__ __forceinline__ uint64_t pair(float a, float b) { uint64_t r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b)); return r; }
 __device__ __forceinline__ void halves(uint64_t v, float & a, float & b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
@@ -166,12 +167,13 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention_prompt(const __grid_c
     int64_t * const sums = reinterpret_cast<int64_t *>(smem_raw + (v_at + S * kTileBytes<D> - smem_u32(smem_raw)));
     int * const flag = reinterpret_cast<int *>(sums + kThreads + 15);
     const uint32_t bars = smem_u32(sums + kThreads + 16);
-    const uint32_t q_full = bars, q_empty = bars + 8, s_full = bars + 16, p_full = bars + 32, o_done = bars + 48, k_full = bars + 64, k_empty = k_full + 8 * S, v_full = k_empty + 8 * S,
+    const uint32_t q_full = bars, q_empty = bars + 8, s_full = bars + 16, p_full = bars + 32, o_done = bars + 64, k_full = bars + 80, k_empty = k_full + 8 * S, v_full = k_empty + 8 * S,
                    v_empty = v_full + 8 * S, v_fixed = v_empty + 8 * S, tmem_slot = v_fixed + 8 * S;
+    const uint32_t staged = (bars + 256 + 15u) & ~15u;      // 2 KB per softmax warp
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;      // (a warp's number, as something the whole warp has)
     if (threadIdx.x == 0) {
         mbar_init(q_full, 1); mbar_init(q_empty, 1);
-        for (int x = 0; x < 2; x++) { mbar_init(s_full + 8 * x, 1); mbar_init(p_full + 8 * x, 4); mbar_init(o_done + 8 * x, 1); }
+        for (int x = 0; x < 2; x++) { mbar_init(s_full + 8 * x, 1); mbar_init(p_full + 16 * x, 4); mbar_init(p_full + 16 * x + 8, 4); mbar_init(o_done + 8 * x, 1); }
         for (int s = 0; s < S; s++) { mbar_init(k_full + 8 * s, 1); mbar_init(k_empty + 8 * s, 1); mbar_init(v_full + 8 * s, 1); mbar_init(v_empty + 8 * s, 1); mbar_init(v_fixed + 8 * s, 1); }
         mbar_init_fence();
     }
@@ -335,12 +337,13 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention_prompt(const __grid_c
             }
             __syncwarp();
         };
-        auto outputs = [&](int x, bool add) {
-            const uint32_t v = v_at + vstage * kTileBytes<D>, p16 = tmem + x * kRows + kHalf, d = tmem + 256 + x * kRows;
+        // one half of the keys, the upper (half = 1) first
+        auto outputs = [&](int x, int half, bool add) {
+            const uint32_t v = v_at + vstage * kTileBytes<D> + half * (kHalf * 128), p16 = tmem + x * kRows + kHalf + half * 32, d = tmem + 256 + x * kRows;
             if (leader) {
                 #pragma unroll
-                for (int kk = 0; kk < kRows / 16; kk++) mma_ts(d, p16 + kk * 8, desc_n(v + kk * (16 * 128)), id_o, add || kk != 0);
-                tc_commit(o_done + 8 * x);
+                for (int kk = 0; kk < kHalf / 16; kk++) mma_ts(d, p16 + kk * 8, desc_n(v + kk * (16 * 128)), id_o, add || kk != 0);
+                if (half == 0) tc_commit(o_done + 8 * x);
             }
             __syncwarp();
         };
@@ -372,7 +375,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention_prompt(const __grid_c
                     for (int x = 0; x < 2; x++) {
                         const int steps = x ? steps1 : steps0;
                         if (ok && j < steps) {
-                            if (!wait(p_full + 8 * x, (x ? done1 : done0) & 1u)) break;
+                            const uint32_t parity = (x ? done1 : done0) & 1u;
+                            if (!wait(p_full + 16 * x, parity)) break;
                             if (!have_v) {
                                 if (!wait(v_full + 8 * vstage, vphase)) break;
                                 if (s.keys - (s.t0 + j) * kRows < kRows) { if (!wait(v_fixed + 8 * vstage, fixed >> vstage & 1u)) break; fixed ^= 1u << vstage; }
@@ -380,7 +384,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention_prompt(const __grid_c
                             }
                             if (x) done1++; else done0++;
                             tc_fence_after();
-                            outputs(x, j != 0);
+                            outputs(x, 1, j != 0);
+                            if (!wait(p_full + 16 * x + 8, parity)) break;
+                            tc_fence_after();
+                            outputs(x, 0, true);
                         }
                         if (ok && j + 1 < steps) {
                             if (!have_k) { if (!wait(k_full + 8 * kstage, kphase)) break; have_k = true; }
@@ -404,7 +411,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention_prompt(const __grid_c
         // ---- softmax: group x (four warps) has tile x, a thread has row r of it ----
         const int x = warp / 4, r = threadIdx.x % kRows;
         const uint32_t lanes = uint32_t((warp % 4) * 32) << 16, s_at = tmem + lanes + x * kRows, o_at = tmem + lanes + 256 + x * kRows;
-        const int query = x * a.tile_queries + r / a.group, head = r % a.group;      // of the unit
+        const int query = x * a.tile_queries + r / a.group;      // of the unit
         const bool row_there = r < a.tile_queries * a.group;
         uint32_t step = 0;      // scores taken
         while (unit_at < to) {
@@ -442,9 +449,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention_prompt(const __grid_c
                         mask(vb, half * kHalf + 32);
                         #pragma unroll
                         for (int c = 0; c < 32; c += 2) {
-                            const float v0 = fmaxf(__uint_as_float(va[c]), __uint_as_float(va[c + 1])), v1 = fmaxf(__uint_as_float(vb[c]), __uint_as_float(vb[c + 1]));
-                            m4[c / 2 % 2] = half == 0 && c < 4 ? v0 : fmaxf(m4[c / 2 % 2], v0);
-                            m4[2 + c / 2 % 2] = half == 0 && c < 4 ? v1 : fmaxf(m4[2 + c / 2 % 2], v1);
+                            float & m0 = m4[c / 2 % 2], & m1 = m4[2 + c / 2 % 2];
+                            m0 = half == 0 && c < 4 ? fmaxf(__uint_as_float(va[c]), __uint_as_float(va[c + 1])) : max3(m0, __uint_as_float(va[c]), __uint_as_float(va[c + 1]));
+                            m1 = half == 0 && c < 4 ? fmaxf(__uint_as_float(vb[c]), __uint_as_float(vb[c + 1])) : max3(m1, __uint_as_float(vb[c]), __uint_as_float(vb[c + 1]));
                         }
                     }
                     const float m = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * a.scale_log2;
@@ -471,13 +478,13 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention_prompt(const __grid_c
                     const float minus = kLift - ref;
                     uint64_t sums[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
                     const uint64_t scale2 = pair(a.scale_log2, a.scale_log2), minus2 = pair(minus, minus);
-                    // 32 probabilities from their scores, as f16 pairs in the first half of v: a quarter of them by the polynomial
+                    // 32 probabilities from their scores, as f16 pairs in the first half of v: one in eight by the polynomial
                     auto powers = [&](uint32_t (&v)[32]) {
                         #pragma unroll
                         for (int c = 0; c < 32; c += 2) {
                             const uint64_t y = fma2(pair(__uint_as_float(v[c]), __uint_as_float(v[c + 1])), scale2, minus2);
                             float e0, e1;
-                            if (c % 8 == 6) {
+                            if (c % 16 == 14) {
                                 ex2_pair(y, e0, e1);
                             } else {
                                 halves(y, e0, e1);
@@ -494,6 +501,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention_prompt(const __grid_c
                     tc_ld32(s_at + 32, vb);
                     powers(va);
                     tc_st16(s_at + kHalf + 32, va);
+                    tc_wait_st();      // the upper half's probabilities go ahead
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(p_full + 16 * x);
                     tc_wait_ld();
                     tie32(vb);
                     tc_ld32(s_at, va);
@@ -512,7 +523,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention_prompt(const __grid_c
                     tc_wait_st();
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(p_full + 8 * x);
+                    if (lane == 0) mbar_arrive(p_full + 16 * x + 8);
                     step++;
                 }
                 // ---- the unit's outputs, or the segment's part of them ----
@@ -522,10 +533,29 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention_prompt(const __grid_c
                     tc_fence_after();
                 }
                 const bool whole = s.t0 == 0 && s.t1 == s.tiles;
+                // 32 columns of the warp's 32 rows, from a thread per row: through shared memory, so that a store is eight rows of 64 bytes and not 32 pieces of 16
+                const int last = min(a.tile_queries, s.queries - x * a.tile_queries) * a.group;      // rows of the tile that are there
+                __half * const out = a.out + ((int64_t(s.row) + x * a.tile_queries) * a.n_head + u.kvh * a.group) * D;
+                auto write_rows = [&](const uint32_t * o, int c) {
+                    const uint32_t at = staged + warp * 2048u;
+                    #pragma unroll
+                    for (uint32_t i = 0; i < 4; i++) {
+                        asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at + lane * 64u + ((i ^ (uint32_t(lane) >> 1 & 3u)) << 4)), "r"(o[4 * i]), "r"(o[4 * i + 1]), "r"(o[4 * i + 2]),
+                                     "r"(o[4 * i + 3]) : "memory");
+                    }
+                    __syncwarp();
+                    #pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const uint32_t row = uint32_t(lane / 4 + 8 * i), piece = uint32_t(lane % 4);
+                        uint4 w;
+                        asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(at + row * 64u + ((piece ^ (row >> 1 & 3u)) << 4)) : "memory");
+                        const int rr = (warp % 4) * 32 + int(row);
+                        if (rr < last) *reinterpret_cast<uint4 *>(out + (int64_t(rr / a.group) * a.n_head + rr % a.group) * D + c + piece * 8) = w;
+                    }
+                    __syncwarp();
+                };
                 if (whole) {
-                    const bool mine = row_there && query < s.queries;
                     const float by = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
-                    __half * const out = a.out + ((int64_t(s.row) + query) * a.n_head + u.kvh * a.group + head) * D;
                     if (n > 0) {
                         #pragma unroll
                         for (int c = 0; c < D; c += 32) {
@@ -538,8 +568,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention_prompt(const __grid_c
                                 const __half2 h = __floats2half2_rn(__uint_as_float(o[i]) * by, __uint_as_float(o[i + 1]) * by);
                                 o[i / 2] = *reinterpret_cast<const uint32_t *>(&h);
                             }
-                            #pragma unroll
-                            for (int i = 0; i < 4; i++) if (mine) reinterpret_cast<uint4 *>(out + c)[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                            write_rows(o, c);
                         }
                     }
                 } else {
@@ -574,12 +603,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention_prompt(const __grid_c
                         float top = -CUDART_INF_F, l = 0.f;
                         for (int b = b0; b <= b1; b++) top = fmaxf(top, __ldcg(reinterpret_cast<const float2 *>(part_of(b) + kRows * D) + r).x);
                         const float minus = top == -CUDART_INF_F ? 0.f : top;
-                        const bool mine = row_there && query < s.queries;
                         for (int b = b0; b <= b1; b++) { const float2 st = __ldcg(reinterpret_cast<const float2 *>(part_of(b) + kRows * D) + r); l = fmaf(st.y, ex2(st.x - minus), l); }
                         const float by = l > 0.f || l != l ? 1.f / l : 0.f;
-                        __half * const out = a.out + ((int64_t(s.row) + query) * a.n_head + u.kvh * a.group + head) * D;
                         for (int c = 0; c < D / 4; c += 8) {
                             float4 o[8] = {};
+                            uint32_t half_row[16];
                             for (int b = b0; b <= b1; b++) {
                                 const float * pt = part_of(b);
                                 const float st = __ldcg(reinterpret_cast<const float2 *>(pt + kRows * D) + r).x, share = ex2(st - minus);
@@ -596,8 +624,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention_prompt(const __grid_c
                             for (int i = 0; i < 8; i += 2) {
                                 const __half2 h[4] = {__floats2half2_rn(o[i].x * by, o[i].y * by), __floats2half2_rn(o[i].z * by, o[i].w * by),
                                                       __floats2half2_rn(o[i + 1].x * by, o[i + 1].y * by), __floats2half2_rn(o[i + 1].z * by, o[i + 1].w * by)};
-                                if (mine) *reinterpret_cast<uint4 *>(out + (c + i) * 4) = *reinterpret_cast<const uint4 *>(h);
+                                const uint4 w = *reinterpret_cast<const uint4 *>(h);
+                                half_row[2 * i] = w.x; half_row[2 * i + 1] = w.y; half_row[2 * i + 2] = w.z; half_row[2 * i + 3] = w.w;
                             }
+                            write_rows(half_row, c * 4);
                         }
                     }
                 }
