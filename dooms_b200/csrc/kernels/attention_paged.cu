@@ -8,7 +8,9 @@
 // block leaves (max, sum, output), and the last of them to arrive adds them up in the order of the blocks. A block has at most two cut items, so the scratch memory
 // depends on the grid alone, and its contents at the start do not matter.
 //
-// The G query heads are rows of m16n8k16 MMAs (f16 operands, f32 accumulators; more than 16 are several items). With f32 queries, query and probabilities enter as f16
+// The G query heads are the eight columns (G > 8: twice eight; more than 16 are several items) of m16n8k16 MMAs, S^T = K Q^T and O^T = V^T P^T, f16 operands, f32
+// accumulators: keys and values are their 16-row operands, so that no row is spent on heads that are not there (with the heads as rows a step was twice the
+// MMAs, and heads of 128 spilled: 118 against 100 us for one row of 131071 keys). With f32 queries, query and probabilities enter as f16
 // value + f16 rounding error (2^-22 together), the query after its row was scaled by a power of two, and each tile's products are added to the outputs in f32
 // (round to nearest; the tensor core's own accumulation truncates): as exact as f32 arithmetic. Probabilities are kept times 2^10, so that their second part
 // stays in f16's normal range.
@@ -60,6 +62,12 @@ __device__ __forceinline__ void ldsm4_t(uint32_t addr, uint32_t (&r)[4]) {
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// The transpose of an 8 x 8 matrix of f16, a row's two neighbours per lane.
+__device__ __forceinline__ uint32_t transposed(uint32_t v) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
 }
 __device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 // (a, b) as f16 pairs; `rest`: what the rounding left, rounded to f16 too
@@ -162,10 +170,9 @@ template <int D, bool HALF, bool WIDE>      // WIDE: items of more than 8 query 
 struct Kernel {
     static constexpr int kStages = D == 128 ? 3 : 6;
     static constexpr int kStageBytes = kTile * D * 2 * 2;
-    static constexpr int kPairs = WIDE ? 2 : 1;
-    static constexpr int kMergeBytes = 3 * (D / 8) * 32 * 8;       // three warps' halves of 8 rows
-    static constexpr int kSmem = 1024 + kStages * kStageBytes + kMergeBytes + 3 * kHeads * 8 + (kThreads + 8) * 8 + 16 * kStages + 32;
-    static constexpr int KK = D / 16, NN = D / 8;
+    static constexpr int NT = WIDE ? 2 : 1, KK = D / 16;
+    static constexpr int kMergeBytes = 3 * KK * 32 * 16;       // three warps' results for eight heads
+    static constexpr int kSmem = 1024 + kStages * kStageBytes + kMergeBytes + 3 * 8 * 8 + (kThreads + 8) * 8 + 16 * kStages + 32;
 };
 
 template <int D, bool HALF, bool WIDE>
@@ -174,9 +181,9 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) k_attention_paged(cons
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     const uint32_t ring = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t * const base = smem_raw + (ring - smem_u32(smem_raw));
-    float2 * const merge = reinterpret_cast<float2 *>(base + K::kStages * K::kStageBytes);                       // [3][NN][32]
-    float2 * const stats = reinterpret_cast<float2 *>(reinterpret_cast<uint8_t *>(merge) + K::kMergeBytes);     // [3][kHeads] (max, sum)
-    int64_t * const sums = reinterpret_cast<int64_t *>(stats + 3 * kHeads);
+    float4 * const merge = reinterpret_cast<float4 *>(base + K::kStages * K::kStageBytes);                       // [3][KK][32]
+    float2 * const stats = reinterpret_cast<float2 *>(reinterpret_cast<uint8_t *>(merge) + K::kMergeBytes);     // [3][8] (max, sum)
+    int64_t * const sums = reinterpret_cast<int64_t *>(stats + 3 * 8);
     const uint32_t full = smem_u32(sums + kThreads + 8), empty = full + 8 * K::kStages;
     int * const last = reinterpret_cast<int *>(sums + kThreads + 7);
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
@@ -184,24 +191,27 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) k_attention_paged(cons
         for (int s = 0; s < K::kStages; s++) { mbar_init(full + 8 * s, 1); mbar_init(empty + 8 * s, kWarps); }
         mbar_init_fence();
     }
+    if (warp == kWarps && lane < 2) asm volatile("prefetch.tensormap [%0];" ::"l"(lane == 0 ? &kmap : &vmap) : "memory");
     pdl_wait();
-    // rows without positions are zero; entries out of range are reported
-    for (int r = blockIdx.x; r < a.n_rows; r += gridDim.x) {
-        const int n = row_length(a, r);
-        if (n < 0 && a.sequence[r] >= 0 && threadIdx.x == 0) a.c.fail();
-        if (n == 0) {
-            for (int i = threadIdx.x; i < a.n_head * D; i += kThreads) {
-                if (HALF) static_cast<__half *>(a.out)[int64_t(r) * a.n_head * D + i] = __half(0.f);
-                else static_cast<float *>(a.out)[int64_t(r) * a.n_head * D + i] = 0.f;
-            }
-        }
-    }
     const int items = a.c.n_kv * a.parts;
     const int64_t total = count_tiles(a, sums) * items;
-    const int64_t blocks = min(int64_t(gridDim.x), total);
-    if (int64_t(blockIdx.x) >= blocks) return;
-    paged_counter_begin(a.arrived + blockIdx.x, a.call);      // of the item that this block's span may end in
-    const int64_t from = total * blockIdx.x / blocks, to = total * (blockIdx.x + 1) / blocks;
+    const int blocks = int(min(int64_t(gridDim.x), total));
+    // rows without positions are zero; entries out of range are reported (by the last warp, which has the least to do at the end)
+    auto rows_without = [&](int thread, int threads) {
+        for (int r = blockIdx.x; r < a.n_rows; r += gridDim.x) {
+            const int n = row_length(a, r);
+            if (n < 0 && a.sequence[r] >= 0 && thread == 0) a.c.fail();
+            if (n == 0) {
+                for (int i = thread; i < a.n_head * D; i += threads) {
+                    if (HALF) static_cast<__half *>(a.out)[int64_t(r) * a.n_head * D + i] = __half(0.f);
+                    else static_cast<float *>(a.out)[int64_t(r) * a.n_head * D + i] = 0.f;
+                }
+            }
+        }
+    };
+    if (int(blockIdx.x) >= blocks) { rows_without(threadIdx.x, kThreads); return; }
+    const int64_t each = quotient(total, blocks);
+    const int64_t from = part_of(total, each, blockIdx.x, blocks), to = part_of(total, each, blockIdx.x + 1, blocks);
     Place p;
     int64_t item_at;      // the first tile of the item at hand
     {
@@ -212,7 +222,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) k_attention_paged(cons
         int r = th * per;
         int64_t t = row_tiles(a, r);
         while (at + t * items <= from) { at += t * items; t = row_tiles(a, ++r); }
-        p.row = r; p.tiles = int(t); p.part = int((from - at) / t); p.tile = int((from - at) % t);
+        p.row = r; p.tiles = int(t); p.part = int(quotient(from - at, t)); p.tile = int(from - at - p.part * t);
         item_at = at + int64_t(p.part) * t;
     }
     auto next_item = [&] {
@@ -224,11 +234,11 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) k_attention_paged(cons
     int stage = 0;
     uint32_t phase = 0;
     auto advance = [&] { if (++stage == K::kStages) { stage = 0; phase ^= 1u; } };
-    int64_t left = to - from;
+    int left = int(to - from);
 
     if (warp == kWarps) {
         // ---- the copies: lane i brings piece i of a tile (the rows of one page, or 64 of them; half a head of 128), keys and values ----
-        const int box = min(kTile, 1 << a.c.page_shift), pieces = kTile / box;
+        const int box = min(kTile, 1 << a.c.page_shift);
         while (left > 0) {
             const int n = row_length(a, p.row), kvh = p.part / a.parts;
             const int32_t * table = a.c.table + int64_t(a.sequence[p.row]) * a.c.max_pages;
@@ -257,31 +267,32 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) k_attention_paged(cons
             if (!ok) break;
             if (left > 0) next_item();
         }
-        (void)pieces;
+        rows_without(lane, 32);
     } else {
+        paged_counter_begin(a.arrived + blockIdx.x, a.call);      // of the item that this block's span may end in
         const int g = lane >> 2, t = lane & 3;
-        // where this lane's ldmatrix rows lie in a stage: keys 16 warp + ..
-        const int krow = warp * 16 + (lane & 7) + ((lane >> 4) & 1) * 8, kchunk = (lane >> 3) & 1;
-        const int vrow = warp * 16 + (lane & 7) + ((lane >> 3) & 1) * 8, vchunk = lane >> 4;
+        // where this lane's ldmatrix rows lie in a stage: keys 16 warp + .., as rows of the A operand (S^T = K Q^T), and as its columns (O^T = V^T P^T)
+        const int krow = warp * 16 + (lane & 7) + ((lane >> 3) & 1) * 8, kchunk = lane >> 4;
+        const int vrow = warp * 16 + (lane & 7) + ((lane >> 4) & 1) * 8, vchunk = (lane >> 3) & 1;
         const uint32_t kat = uint32_t(krow) * 128u, vat = uint32_t(vrow) * 128u + kTile * D * 2, sw = uint32_t(lane & 7);
         while (left > 0) {
             const int n = row_length(a, p.row), kvh = p.part / a.parts, head0 = kvh * a.group + (p.part % a.parts) * kHeads;
             const int heads = min(kHeads, a.group - (p.part % a.parts) * kHeads);
-            // the item's queries as A operands: rows g and (WIDE) g + 8
-            uint32_t qh[K::KK][4], ql[HALF ? 1 : K::KK][4];
-            float f[K::kPairs];
+            // the item's queries as B operands: this lane has two times two neighbouring values of head g (+ 8 e) in each slice of 16; f: the scale of heads 2t and 2t + 1
+            uint32_t qh[K::NT][K::KK][2], ql[HALF ? 1 : K::NT][HALF ? 1 : K::KK][2];
+            float f[K::NT][2];
             #pragma unroll
-            for (int e = 0; e < 2; e++) {
-                const bool there = e < K::kPairs && g + 8 * e < heads;
+            for (int e = 0; e < K::NT; e++) {
+                const bool there = g + 8 * e < heads;
                 const int64_t at = (int64_t(p.row) * a.n_head + head0 + g + 8 * e) * D + 2 * t;
                 if (HALF) {
                     #pragma unroll
                     for (int kk = 0; kk < K::KK; kk++) {
                         const uint32_t * q = reinterpret_cast<const uint32_t *>(static_cast<const __half *>(a.q) + at + 16 * kk);
-                        qh[kk][e] = there ? __ldg(q) : 0u;
-                        qh[kk][2 + e] = there ? __ldg(q + 4) : 0u;
+                        qh[e][kk][0] = there ? __ldg(q) : 0u;
+                        qh[e][kk][1] = there ? __ldg(q + 4) : 0u;
                     }
-                    if (e < K::kPairs) f[e] = a.scale_log2;
+                    f[e][0] = f[e][1] = a.scale_log2;
                 } else {
                     float2 v[K::KK][2];
                     float most = 0.f;
@@ -294,23 +305,27 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) k_attention_paged(cons
                     }
                     most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
                     most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-                    // a power of two that brings the row's largest value into [1, 2); rows of zeros, of subnormals and with infinities go as they are
+                    // a power of two that brings the head's largest value into [1, 2); zeros, subnormals and infinities go as they are
                     const uint32_t ex = __float_as_uint(most) >> 23;
                     const bool fit = ex > 1 && ex < 253;
-                    const float down = fit ? __uint_as_float((254u - ex) << 23) : 1.f;
-                    if (e < K::kPairs) f[e] = a.scale_log2 * (fit ? __uint_as_float(ex << 23) : 1.f);
+                    const float down = fit ? __uint_as_float((254u - ex) << 23) : 1.f, up = a.scale_log2 * (fit ? __uint_as_float(ex << 23) : 1.f);
+                    f[e][0] = __shfl_sync(0xffffffffu, up, 8 * t);
+                    f[e][1] = __shfl_sync(0xffffffffu, up, 8 * t + 4);
                     #pragma unroll
                     for (int kk = 0; kk < K::KK; kk++) {
-                        qh[kk][e] = split2(v[kk][0].x * down, v[kk][0].y * down, &ql[HALF ? 0 : kk][e]);
-                        qh[kk][2 + e] = split2(v[kk][1].x * down, v[kk][1].y * down, &ql[HALF ? 0 : kk][2 + e]);
+                        #pragma unroll
+                        for (int i = 0; i < 2; i++) qh[e][kk][i] = split2(v[kk][i].x * down, v[kk][i].y * down, &ql[HALF ? 0 : e][HALF ? 0 : kk][i]);
                     }
                 }
             }
-            float o[K::NN][2 * K::kPairs], top[K::kPairs], sum[K::kPairs];
+            float o[K::NT][K::KK][4], top[K::NT][2], sum[K::NT][2];
             #pragma unroll
-            for (int j = 0; j < K::NN; j++) { o[j][0] = o[j][1] = 0.f; if (WIDE) o[j][2 * K::kPairs - 2] = o[j][2 * K::kPairs - 1] = 0.f; }
-            #pragma unroll
-            for (int e = 0; e < K::kPairs; e++) { top[e] = -CUDART_INF_F; sum[e] = 0.f; }
+            for (int e = 0; e < K::NT; e++) {
+                #pragma unroll
+                for (int j = 0; j < K::KK; j++) o[e][j][0] = o[e][j][1] = o[e][j][2] = o[e][j][3] = 0.f;
+                top[e][0] = top[e][1] = -CUDART_INF_F;
+                sum[e][0] = sum[e][1] = 0.f;
+            }
             const bool starts = p.tile == 0;
             for (; p.tile < p.tiles && left > 0; p.tile++, left--) {
                 const int valid = min(kTile, n - p.tile * kTile) - warp * 16;      // of this warp's 16 keys
@@ -318,75 +333,83 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) k_attention_paged(cons
                 ok = __all_sync(0xffffffffu, ok);
                 if (valid > 0) {
                     const uint32_t st = ring + stage * K::kStageBytes;
-                    float s[2][4] = {};
-                    [[maybe_unused]] float rest[2][4] = {};
+                    // scores of keys g, g + 8 and heads 2t, 2t + 1. f32: sixteen products at a time, added up in f32 (a chain through the accumulator loses 1e-6 of a probability
+                    // on heads of 128), the queries' second parts in an accumulator of their own
+                    float s[K::NT][4] = {};
+                    [[maybe_unused]] float rest[K::NT][4] = {};
                     #pragma unroll
                     for (int kk = 0; kk < K::KK; kk++) {
-                        uint32_t b[4];
-                        ldsm4(st + kat + (kk / 4) * (kTile * 128) + (((uint32_t(kk % 4) * 2 + kchunk) ^ sw) << 4), b);
-                        if (HALF) {
-                            mma_f16(s[0], qh[kk], b[0], b[1]);
-                            mma_f16(s[1], qh[kk], b[2], b[3]);
-                        } else {      // sixteen products at a time, added up in f32: a chain through the accumulator loses 1e-6 of a probability on heads of 128
-                            #pragma unroll
-                            for (int j = 0; j < 2; j++) {
+                        uint32_t k[4];
+                        ldsm4(st + kat + (kk / 4) * (kTile * 128) + (((uint32_t(kk % 4) * 2 + kchunk) ^ sw) << 4), k);
+                        #pragma unroll
+                        for (int e = 0; e < K::NT; e++) {
+                            if (HALF) {
+                                mma_f16(s[e], k, qh[e][kk][0], qh[e][kk][1]);
+                            } else {
                                 float c[4] = {0.f, 0.f, 0.f, 0.f};
-                                mma_f16(c, qh[kk], b[2 * j], b[2 * j + 1]);
-                                mma_f16(rest[j], ql[HALF ? 0 : kk], b[2 * j], b[2 * j + 1]);
+                                mma_f16(c, k, qh[e][kk][0], qh[e][kk][1]);
+                                mma_f16(rest[e], k, ql[HALF ? 0 : e][HALF ? 0 : kk][0], ql[HALF ? 0 : e][HALF ? 0 : kk][1]);
                                 #pragma unroll
-                                for (int i = 0; i < 2 * K::kPairs; i++) s[j][i] += c[i];
+                                for (int i = 0; i < 4; i++) s[e][i] += c[i];
                             }
                         }
                     }
-                    if (!HALF) {
-                        #pragma unroll
-                        for (int j = 0; j < 2; j++) {
-                            #pragma unroll
-                            for (int i = 0; i < 2 * K::kPairs; i++) s[j][i] += rest[j][i];
-                        }
-                    }
-                    if (valid < 16) {      // the last page's rest: no score, and no value (a page may hold anything there)
-                        #pragma unroll
-                        for (int j = 0; j < 2; j++) {
-                            #pragma unroll
-                            for (int i = 0; i < 4; i++) if (8 * j + 2 * t + (i & 1) >= valid) s[j][i] = -CUDART_INF_F;
-                        }
+                    if (valid < 16) {      // the last page's rest: no value (a page may hold anything there), and below no score
                         for (int i = lane; i < (16 - valid) * (D / 8); i += 32) {
                             const uint32_t row = uint32_t(warp * 16 + valid + i / (D / 8)), c = uint32_t(i % (D / 8));
                             asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(st + kTile * D * 2 + (c / 8) * (kTile * 128) + row * 128u + (c % 8) * 16u), "r"(0u) : "memory");
                         }
                         __syncwarp();
                     }
-                    uint32_t ph[4] = {0u, 0u, 0u, 0u}, pl[4] = {0u, 0u, 0u, 0u};
-                    float keep[K::kPairs];
+                    uint32_t ph[K::NT][2], pl[K::NT][2];
+                    float keep[K::NT][2];
                     #pragma unroll
-                    for (int e = 0; e < K::kPairs; e++) {
-                        const float f_e = f[e];
-                        float m = fmaxf(fmaxf(s[0][2 * e], s[0][2 * e + 1]), fmaxf(s[1][2 * e], s[1][2 * e + 1])) * f_e;
-                        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-                        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-                        m = fmaxf(m, top[e]);
-                        const float minus = m == -CUDART_INF_F ? 0.f : kLift - m;
-                        keep[e] = ex2(top[e] + (m == -CUDART_INF_F ? 0.f : -m));
-                        top[e] = m;
-                        float x[2][2];
+                    for (int e = 0; e < K::NT; e++) {
+                        if (!HALF) {
+                            #pragma unroll
+                            for (int i = 0; i < 4; i++) s[e][i] += rest[e][i];
+                        }
+                        if (valid < 16) {
+                            #pragma unroll
+                            for (int i = 0; i < 4; i++) if (g + 8 * (i / 2) >= valid) s[e][i] = -CUDART_INF_F;
+                        }
+                        float x[4];
                         #pragma unroll
-                        for (int j = 0; j < 2; j++) { x[j][0] = ex2(fmaf(s[j][2 * e], f_e, minus)); x[j][1] = ex2(fmaf(s[j][2 * e + 1], f_e, minus)); }
-                        sum[e] = sum[e] * keep[e] + ((x[0][0] + x[0][1]) + (x[1][0] + x[1][1]));
-                        ph[e] = HALF ? split2(x[0][0], x[0][1], nullptr) : split_p(x[0][0], x[0][1], &pl[e]);
-                        ph[2 + e] = HALF ? split2(x[1][0], x[1][1], nullptr) : split_p(x[1][0], x[1][1], &pl[2 + e]);
-                    }
-                    #pragma unroll
-                    for (int j = 0; j < K::NN; j += 2) {
-                        uint32_t b[4];
-                        ldsm4_t(st + vat + (j / 8) * (kTile * 128) + (((uint32_t(j % 8) + vchunk) ^ sw) << 4), b);
+                        for (int h = 0; h < 2; h++) {
+                            const float f_h = f[e][h];
+                            float m = fmaxf(s[e][h], s[e][2 + h]) * f_h;
+                            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+                            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+                            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+                            m = fmaxf(m, top[e][h]);
+                            const bool none = m == -CUDART_INF_F;
+                            const float minus = none ? 0.f : kLift - m;
+                            keep[e][h] = ex2(top[e][h] - (none ? 0.f : m));
+                            top[e][h] = m;
+                            x[h] = ex2(fmaf(s[e][h], f_h, minus));
+                            x[2 + h] = ex2(fmaf(s[e][2 + h], f_h, minus));
+                            sum[e][h] = fmaf(sum[e][h], keep[e][h], x[h] + x[2 + h]);
+                        }
+                        // probabilities of key g (+ 8) and heads 2t, 2t + 1 -> of keys 2t, 2t + 1 (+ 8) and head g: the B operand
                         #pragma unroll
                         for (int i = 0; i < 2; i++) {
+                            uint32_t low = 0;
+                            const uint32_t high = HALF ? split2(x[2 * i], x[2 * i + 1], nullptr) : split_p(x[2 * i], x[2 * i + 1], &low);
+                            ph[e][i] = transposed(high);
+                            if (!HALF) pl[e][i] = transposed(low);
+                        }
+                    }
+                    #pragma unroll
+                    for (int j = 0; j < K::KK; j++) {
+                        uint32_t v[4];
+                        ldsm4_t(st + vat + (j / 4) * (kTile * 128) + (((uint32_t(j % 4) * 2 + vchunk) ^ sw) << 4), v);
+                        #pragma unroll
+                        for (int e = 0; e < K::NT; e++) {
                             float c[4] = {0.f, 0.f, 0.f, 0.f};
-                            mma_f16(c, ph, b[2 * i], b[2 * i + 1]);
-                            if (!HALF) mma_f16(c, pl, b[2 * i], b[2 * i + 1]);
+                            mma_f16(c, v, ph[e][0], ph[e][1]);
+                            if (!HALF) mma_f16(c, v, pl[e][0], pl[e][1]);
                             #pragma unroll
-                            for (int e = 0; e < 2 * K::kPairs; e++) o[j + i][e] = fmaf(o[j + i][e], keep[e / 2], c[e]);
+                            for (int i = 0; i < 4; i++) o[e][j][i] = fmaf(o[e][j][i], keep[e][i % 2], c[i]);
                         }
                     }
                     if (valid < 16) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");      // (the zeros, before a copy may land on them)
@@ -396,54 +419,67 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) k_attention_paged(cons
                 advance();
             }
             const bool ends = p.tile == p.tiles;
-            // ---- the four warps' results: warps 1 to 3 hand theirs to warp 0, eight rows at a time ----
+            // ---- the four warps' results: warps 1 to 3 hand theirs to warp 0, eight heads at a time ----
             #pragma unroll
-            for (int e = 0; e < K::kPairs; e++) {
-                sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], 1);
-                sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], 2);
+            for (int e = 0; e < K::NT; e++) {
+                #pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    #pragma unroll
+                    for (int d = 4; d < 32; d *= 2) sum[e][h] += __shfl_xor_sync(0xffffffffu, sum[e][h], d);
+                }
                 asm volatile("bar.sync 1, 128;" ::: "memory");      // warp 0 is done with the last hand-over
                 if (warp > 0) {
-                    if (t == 0) stats[(warp - 1) * kHeads + g] = make_float2(top[e], sum[e]);
+                    if (g == 0) {
+                        stats[(warp - 1) * 8 + 2 * t] = make_float2(top[e][0], sum[e][0]);
+                        stats[(warp - 1) * 8 + 2 * t + 1] = make_float2(top[e][1], sum[e][1]);
+                    }
                     #pragma unroll
-                    for (int j = 0; j < K::NN; j++) merge[((warp - 1) * K::NN + j) * 32 + lane] = make_float2(o[j][2 * e], o[j][2 * e + 1]);
+                    for (int j = 0; j < K::KK; j++) merge[((warp - 1) * K::KK + j) * 32 + lane] = make_float4(o[e][j][0], o[e][j][1], o[e][j][2], o[e][j][3]);
                 }
                 asm volatile("bar.sync 1, 128;" ::: "memory");
                 if (warp == 0) {
-                    float m = top[e], share[4], l;
-                    #pragma unroll
-                    for (int w = 0; w < 3; w++) m = fmaxf(m, stats[w * kHeads + g].x);
-                    const float minus = m == -CUDART_INF_F ? 0.f : m;
-                    share[0] = ex2(top[e] - minus);
-                    l = sum[e] * share[0];
-                    #pragma unroll
-                    for (int w = 0; w < 3; w++) { const float2 x = stats[w * kHeads + g]; share[w + 1] = ex2(x.x - minus); l += x.y * share[w + 1]; }
                     const bool whole = starts && ends;
-                    const float by = whole ? (l > 0.f || l != l ? 1.f / l : 0.f) : 1.f;
-                    const int h = g + 8 * e;
                     float * const part = a.part + (int64_t(blockIdx.x) * 2 + (starts ? 1 : 0)) * kSlot<D>;
-                    const int64_t at = (int64_t(p.row) * a.n_head + head0 + h) * D + 2 * t;
-                    if (h < heads) {
-                        if (!whole && t == 0) *reinterpret_cast<float2 *>(part + kHeads * D + 2 * h) = make_float2(m, l);
+                    float share[2][4], by[2];
+                    #pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        float m = top[e][h];
                         #pragma unroll
-                        for (int j = 0; j < K::NN; j++) {
-                            float2 v = make_float2(o[j][2 * e] * share[0], o[j][2 * e + 1] * share[0]);
-                            #pragma unroll
-                            for (int w = 0; w < 3; w++) {
-                                const float2 x = merge[(w * K::NN + j) * 32 + lane];
-                                v.x = fmaf(x.x, share[w + 1], v.x);
-                                v.y = fmaf(x.y, share[w + 1], v.y);
+                        for (int w = 0; w < 3; w++) m = fmaxf(m, stats[w * 8 + 2 * t + h].x);
+                        const float minus = m == -CUDART_INF_F ? 0.f : m;
+                        share[h][0] = ex2(top[e][h] - minus);
+                        float l = sum[e][h] * share[h][0];
+                        #pragma unroll
+                        for (int w = 0; w < 3; w++) { const float2 x = stats[w * 8 + 2 * t + h]; share[h][w + 1] = ex2(x.x - minus); l += x.y * share[h][w + 1]; }
+                        by[h] = whole ? (l > 0.f || l != l ? 1.f / l : 0.f) : 1.f;
+                        const int head = 2 * t + h + 8 * e;
+                        if (!whole && g == 0 && head < heads) *reinterpret_cast<float2 *>(part + kHeads * D + 2 * head) = make_float2(m, l);
+                    }
+                    #pragma unroll
+                    for (int j = 0; j < K::KK; j++) {
+                        float y[4] = {o[e][j][0] * share[0][0], o[e][j][1] * share[1][0], o[e][j][2] * share[0][0], o[e][j][3] * share[1][0]};
+                        #pragma unroll
+                        for (int w = 0; w < 3; w++) {
+                            const float4 x = merge[(w * K::KK + j) * 32 + lane];
+                            y[0] = fmaf(x.x, share[0][w + 1], y[0]); y[1] = fmaf(x.y, share[1][w + 1], y[1]);
+                            y[2] = fmaf(x.z, share[0][w + 1], y[2]); y[3] = fmaf(x.w, share[1][w + 1], y[3]);
+                        }
+                        #pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const int head = 2 * t + i % 2 + 8 * e, d = 16 * j + g + 8 * (i / 2);
+                            if (head < heads) {
+                                const float v = y[i] * by[i % 2];
+                                const int64_t at = (int64_t(p.row) * a.n_head + head0 + head) * D + d;
+                                if (!whole) part[head * D + d] = v;
+                                else if (HALF) static_cast<__half *>(a.out)[at] = __float2half_rn(v);
+                                else static_cast<float *>(a.out)[at] = v;
                             }
-                            v.x *= by;
-                            v.y *= by;
-                            if (!whole) *reinterpret_cast<float2 *>(part + h * D + 8 * j + 2 * t) = v;
-                            else if (HALF) *reinterpret_cast<__half2 *>(static_cast<__half *>(a.out) + at + 8 * j) = __floats2half2_rn(v.x, v.y);
-                            else *reinterpret_cast<float2 *>(static_cast<float *>(a.out) + at + 8 * j) = v;
                         }
                     }
                 }
             }
             if (!(starts && ends)) {
-                const int first = int(((item_at + 1) * blocks - 1) / total), count = int(((item_at + p.tiles) * blocks - 1) / total) - first + 1;
+                const int first = int(quotient((item_at + 1) * blocks - 1, total)), count = int(quotient((item_at + p.tiles) * blocks - 1, total)) - first + 1;
                 if (warp == 0) {
                     __threadfence();
                     __syncwarp();

@@ -158,6 +158,73 @@ __device__ __forceinline__ int64_t prompt_length(const Args & a, const Prompt & 
     return p.queries ? a.c.n_kv * units_length(p, wide, (p.queries + wide - 1) / wide) : 0;
 }
 
+// Adds up the parts that blocks b0 to b1 left of a unit, with the eight softmax warps: rows0 and rows1 rows of its tiles A and B; out: its first query's first head. A warp
+// takes four rows at a time of two groups of rows, so that the loads of two parts' 2 x D / 32 pieces of 16 bytes are in flight together.
+template <int D>
+__device__ __forceinline__ void join(const Args & a, int b0, int b1, int rows0, int rows1, __half * out, int warp, int lane) {
+    constexpr int kPieces = D / 32, kSets = 2 * kRows / 4;
+    const int sub = lane % 4, piece = lane / 4;
+    for (int set = warp; set < kSets / 2; set += 8) {      // rows 4 set + sub of tile A, and of tile B
+        float4 o[2][kPieces];
+        float m[2] = {-CUDART_INF_F, -CUDART_INF_F}, l[2] = {0.f, 0.f};
+        const int row = 4 * set + sub;
+        const bool there[2] = {row < rows0, row < rows1};
+        if (!__any_sync(0xffffffffu, there[0] || there[1])) continue;
+        #pragma unroll
+        for (int x = 0; x < 2; x++) {
+            #pragma unroll
+            for (int i = 0; i < kPieces; i++) o[x][i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+        for (int b = b0; b <= b1; b += 2) {
+            float2 st[2][2];
+            float4 w[2][2][kPieces];
+            #pragma unroll
+            for (int k = 0; k < 2; k++) {
+                #pragma unroll
+                for (int x = 0; x < 2; x++) {
+                    const float * part = a.part + ((int64_t(b + k) * 2 + (b + k == b0 ? 1 : 0)) * 2 + x) * kTilePart<D>;
+                    const bool load = there[x] && b + k <= b1;
+                    st[k][x] = load ? __ldcg(reinterpret_cast<const float2 *>(part + kRows * D) + row) : make_float2(-CUDART_INF_F, 0.f);
+                    #pragma unroll
+                    for (int i = 0; i < kPieces; i++) w[k][x][i] = load ? __ldcg(reinterpret_cast<const float4 *>(part) + (piece + 8 * i) * kRows + row) : make_float4(0.f, 0.f, 0.f, 0.f);
+                }
+            }
+            #pragma unroll
+            for (int x = 0; x < 2; x++) {
+                const float top = max3(m[x], st[0][x].x, st[1][x].x), minus = top == -CUDART_INF_F ? 0.f : top, keep = ex2(m[x] - minus);
+                l[x] *= keep;
+                #pragma unroll
+                for (int i = 0; i < kPieces; i++) { o[x][i].x *= keep; o[x][i].y *= keep; o[x][i].z *= keep; o[x][i].w *= keep; }
+                #pragma unroll
+                for (int k = 0; k < 2; k++) {
+                    const bool some = st[k][x].x > -CUDART_INF_F;      // (a tile without a step in a part left no outputs there, only that)
+                    const float share = ex2(st[k][x].x - minus);
+                    l[x] = some ? fmaf(st[k][x].y, share, l[x]) : l[x];
+                    #pragma unroll
+                    for (int i = 0; i < kPieces; i++) {
+                        if (some) {
+                            o[x][i].x = fmaf(w[k][x][i].x, share, o[x][i].x); o[x][i].y = fmaf(w[k][x][i].y, share, o[x][i].y);
+                            o[x][i].z = fmaf(w[k][x][i].z, share, o[x][i].z); o[x][i].w = fmaf(w[k][x][i].w, share, o[x][i].w);
+                        }
+                    }
+                }
+                m[x] = top;
+            }
+        }
+        #pragma unroll
+        for (int x = 0; x < 2; x++) {
+            if (!there[x]) continue;
+            const float by = l[x] > 0.f || l[x] != l[x] ? 1.f / l[x] : 0.f;
+            __half * const to = out + ((int64_t(x) * a.tile_queries + row / a.group) * a.n_head + row % a.group) * D;
+            #pragma unroll
+            for (int i = 0; i < kPieces; i++) {
+                const __half2 h[2] = {__floats2half2_rn(o[x][i].x * by, o[x][i].y * by), __floats2half2_rn(o[x][i].z * by, o[x][i].w * by)};
+                *reinterpret_cast<uint2 *>(to + (piece + 8 * i) * 4) = *reinterpret_cast<const uint2 *>(h);
+            }
+        }
+    }
+}
+
 template <int D>
 __global__ void __launch_bounds__(kThreads, 1) k_attention_prompt(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
                                                                   const __grid_constant__ CUtensorMap vmap, const Args a) {
@@ -177,19 +244,16 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention_prompt(const __grid_c
         for (int s = 0; s < S; s++) { mbar_init(k_full + 8 * s, 1); mbar_init(k_empty + 8 * s, 1); mbar_init(v_full + 8 * s, 1); mbar_init(v_empty + 8 * s, 1); mbar_init(v_fixed + 8 * s, 1); }
         mbar_init_fence();
     }
+    if (warp == 9) {      // the MMAs' warp owns the tensor memory
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(tmem_slot) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    } else if (warp == 8 && lane < 3) {
+        asm volatile("prefetch.tensormap [%0];" ::"l"(lane == 0 ? &qmap : lane == 1 ? &kmap : &vmap) : "memory");
+    }
     pdl_wait();
 
-    // ---- what is out of range is reported, queries that see nothing are zero; then the line ----
-    const int wide = 2 * a.tile_queries;
-    for (int i = blockIdx.x; i < a.n_prompts; i += gridDim.x) {
-        bool bad = false;
-        const Prompt p = prompt_at(a, i, &bad);
-        if (bad && threadIdx.x == 0) a.c.fail();
-        if (bad || p.seq < 0) continue;
-        const int b = a.start[i], unseen = (a.start[i + 1] - b) - p.queries;
-        for (int64_t u = threadIdx.x; u < int64_t(unseen) * a.n_head * D; u += kThreads) a.out[int64_t(b) * a.n_head * D + u] = __half(0.f);
-    }
-    const int per = (a.n_prompts + kThreads - 1) / kThreads;
+    // ---- the line: every thread adds up a run of prompts, the block scans the runs ----
+    const int wide = 2 * a.tile_queries, per = (a.n_prompts + kThreads - 1) / kThreads;
     {
         const int i0 = min(a.n_prompts, int(threadIdx.x) * per), i1 = min(a.n_prompts, i0 + per);
         int64_t mine = 0;
@@ -201,40 +265,36 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention_prompt(const __grid_c
         for (int w = 0; w < warp; w++) run += sums[kThreads + w];
         sums[threadIdx.x] = run - mine;
         if (threadIdx.x == kThreads - 1) sums[kThreads + 14] = run;
+        tc_fence_before();
         __syncthreads();
+        tc_fence_after();
     }
-    const int64_t total = sums[kThreads + 14];
-    const int64_t blocks = max(int64_t(1), min(int64_t(gridDim.x), total / kShortestSpan));
-    if (total == 0 || int64_t(blockIdx.x) >= blocks) return;
-    paged_counter_begin(a.arrived + blockIdx.x, a.call);
-    if (warp == 9) {      // the MMAs' warp owns the tensor memory
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(tmem_slot) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    }
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
     uint32_t tmem;
     asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(tmem_slot));
     tmem = __shfl_sync(0xffffffffu, tmem, 0);
-
-    const int64_t from = total * blockIdx.x / blocks, to = total * (blockIdx.x + 1) / blocks;
-    Unit u;
-    Prompt p;
-    int64_t unit_at;      // where unit u begins
-    {
+    const int64_t total = sums[kThreads + 14];
+    const int blocks = max(1, int(min(int64_t(gridDim.x), total / kShortestSpan)));
+    const int64_t each = quotient(total, blocks);
+    auto part_at = [&](int b) { return part_of(total, each, b, blocks); };
+    const bool idle = total == 0 || int(blockIdx.x) >= blocks;
+    const int64_t from = idle ? 0 : part_at(blockIdx.x), to = idle ? 0 : part_at(blockIdx.x + 1);
+    Unit u{0, 0, 0};
+    Prompt p{0, 0, 0, 0};
+    int64_t unit_at = 0;      // where unit u begins
+    if (!idle) {
         int th = 0;
+        #pragma unroll
         for (int step = 256; step; step >>= 1) if (th + step < kThreads && sums[th + step] <= from) th += step;
         int64_t at = sums[th];
         int i = th * per;
         int64_t n;
         for (;; i++) { p = prompt_at(a, i); n = prompt_length(a, p); if (at + n > from) break; at += n; }
         const int tiles = (p.queries + wide - 1) / wide;
-        const int64_t head = n / a.c.n_kv;
-        const int kvh = int((from - at) / head);
+        const int64_t head = units_length(p, wide, tiles);
+        const int kvh = int(quotient(from - at, head));
         at += kvh * head;
         int t = 0;
-        for (int step = 1 << 30; step; step >>= 1) if (t + step < tiles && at + units_length(p, wide, t + step) <= from) t += step;
+        for (int step = 1 << (31 - __clz(tiles)); step; step >>= 1) if (t + step < tiles && at + units_length(p, wide, t + step) <= from) t += step;
         u = {i, kvh, t};
         unit_at = at + units_length(p, wide, t);
     }
@@ -262,7 +322,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention_prompt(const __grid_c
     };
     bool ok = true;
 
-    if (warp == 8) {
+    if (idle) {
+        // (nothing but the end)
+    } else if (warp == 8) {
         // ---- the copies ----
         const int box = min(kRows, 1 << a.c.page_shift), piece = lane / (D / 64), half = lane % (D / 64);
         int stage = 0, units = 0;
@@ -414,6 +476,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention_prompt(const __grid_c
         const int query = x * a.tile_queries + r / a.group;      // of the unit
         const bool row_there = r < a.tile_queries * a.group;
         uint32_t step = 0;      // scores taken
+        paged_counter_begin(a.arrived + blockIdx.x, a.call);      // of the unit that this block's part of the line may end in
         while (unit_at < to) {
             const Segment s = segment();
             if (s.t0 < s.t1) {
@@ -592,43 +655,15 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention_prompt(const __grid_c
                     __threadfence();
                     asm volatile("bar.sync 1, 256;" ::: "memory");
                     // the blocks that share the unit: those whose tiles are not none
-                    int b0 = int(((unit_at + 1) * blocks - 1) / total), b1 = int((s.next * blocks - 1) / total);
-                    if (tile_of(total * (b0 + 1) / blocks - unit_at, s.tiles) == 0) b0++;
-                    if (tile_of(total * b1 / blocks - unit_at, s.tiles) == s.tiles) b1--;
+                    int b0 = int(quotient((unit_at + 1) * blocks - 1, total)), b1 = int(quotient(s.next * blocks - 1, total));
+                    if (tile_of(part_at(b0 + 1) - unit_at, s.tiles) == 0) b0++;
+                    if (tile_of(part_at(b1) - unit_at, s.tiles) == s.tiles) b1--;
                     if (threadIdx.x == 0) *flag = paged_counter_arrive(a.arrived + b0, a.call, b1 - b0 + 1, &ok);
                     asm volatile("bar.sync 1, 256;" ::: "memory");
                     if (*flag) {
                         __threadfence();
-                        auto part_of = [&](int b) { return a.part + ((int64_t(b) * 2 + (b == b0 ? 1 : 0)) * 2 + x) * kTilePart<D>; };
-                        float top = -CUDART_INF_F, l = 0.f;
-                        for (int b = b0; b <= b1; b++) top = fmaxf(top, __ldcg(reinterpret_cast<const float2 *>(part_of(b) + kRows * D) + r).x);
-                        const float minus = top == -CUDART_INF_F ? 0.f : top;
-                        for (int b = b0; b <= b1; b++) { const float2 st = __ldcg(reinterpret_cast<const float2 *>(part_of(b) + kRows * D) + r); l = fmaf(st.y, ex2(st.x - minus), l); }
-                        const float by = l > 0.f || l != l ? 1.f / l : 0.f;
-                        for (int c = 0; c < D / 4; c += 8) {
-                            float4 o[8] = {};
-                            uint32_t half_row[16];
-                            for (int b = b0; b <= b1; b++) {
-                                const float * pt = part_of(b);
-                                const float st = __ldcg(reinterpret_cast<const float2 *>(pt + kRows * D) + r).x, share = ex2(st - minus);
-                                float4 w[8];
-                                #pragma unroll
-                                for (int i = 0; i < 8; i++) w[i] = st > -CUDART_INF_F ? __ldcg(reinterpret_cast<const float4 *>(pt) + (c + i) * kRows + r) : make_float4(0.f, 0.f, 0.f, 0.f);
-                                #pragma unroll
-                                for (int i = 0; i < 8; i++) {
-                                    o[i].x = fmaf(w[i].x, share, o[i].x); o[i].y = fmaf(w[i].y, share, o[i].y);
-                                    o[i].z = fmaf(w[i].z, share, o[i].z); o[i].w = fmaf(w[i].w, share, o[i].w);
-                                }
-                            }
-                            #pragma unroll
-                            for (int i = 0; i < 8; i += 2) {
-                                const __half2 h[4] = {__floats2half2_rn(o[i].x * by, o[i].y * by), __floats2half2_rn(o[i].z * by, o[i].w * by),
-                                                      __floats2half2_rn(o[i + 1].x * by, o[i + 1].y * by), __floats2half2_rn(o[i + 1].z * by, o[i + 1].w * by)};
-                                const uint4 w = *reinterpret_cast<const uint4 *>(h);
-                                half_row[2 * i] = w.x; half_row[2 * i + 1] = w.y; half_row[2 * i + 2] = w.z; half_row[2 * i + 3] = w.w;
-                            }
-                            write_rows(half_row, c * 4);
-                        }
+                        join<D>(a, b0, b1, x == 0 ? last : min(a.tile_queries, s.queries) * a.group, x == 1 ? last : max(0, s.queries - a.tile_queries) * a.group,
+                                a.out + (int64_t(s.row) * a.n_head + u.kvh * a.group) * D, warp, lane);
                     }
                 }
                 tc_fence_before();
@@ -637,6 +672,15 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention_prompt(const __grid_c
         }
     }
     if (!ok && lane == 0 && a.c.error) *reinterpret_cast<volatile int *>(a.c.error) = kErrorPagedWait;
+    // ---- what is out of range is reported, queries that see nothing are zero ----
+    for (int i = blockIdx.x; i < a.n_prompts; i += gridDim.x) {
+        bool bad = false;
+        const Prompt q = prompt_at(a, i, &bad);
+        if (bad && threadIdx.x == 0) a.c.fail();
+        if (bad || q.seq < 0) continue;
+        const int b = a.start[i], unseen = (a.start[i + 1] - b) - q.queries;
+        for (int64_t v = threadIdx.x; v < int64_t(unseen) * a.n_head * D; v += kThreads) a.out[int64_t(b) * a.n_head * D + v] = __half(0.f);
+    }
     tc_fence_before();
     __syncthreads();
     if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");

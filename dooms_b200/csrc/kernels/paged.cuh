@@ -28,6 +28,13 @@ struct PagedView {
     }
 };
 
+// a / b for a >= 0, b > 0: in 32 bits where they fit (a 64-bit division is some hundred cycles, and stands in front of everything else a block does).
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+    return ((a | b) >> 32) == 0 ? int64_t(uint32_t(a) / uint32_t(b)) : a / b;
+}
+// Where the b-th of n equal parts of `total` begins.
+__device__ __forceinline__ int64_t part_of(int64_t total, int64_t each, int b, int n) { return each * b + int64_t(uint64_t(total - each * n) * uint32_t(b) / uint32_t(n)); }
+
 // Arrival counters in scratch memory whose contents at the start do not matter: a counter is (a call's own number, 48 bits, not zero) << 16 | blocks that have
 // arrived. The block that owns the counter sets it up when it begins; others (behind it in the grid) wait until it carries the call's number. The last
 // one to arrive leaves zero, so that a replayed call, whose number is the same, finds no count of its own; one that nobody arrived at stays set up for the replay.
