@@ -706,9 +706,10 @@ cudaError_t make_heads_map(TensorMap * out, const void * base, int head_dim, int
     const cuuint64_t dims[3] = {cuuint64_t(head_dim), cuuint64_t(heads), cuuint64_t(rows)};
     const cuuint64_t strides[2] = {cuuint64_t(head_dim) * 2, cuuint64_t(head_dim) * 2 * cuuint64_t(heads)};
     const cuuint32_t box[3] = {64u, cuuint32_t(box_heads), cuuint32_t(box_rows)};
+    // (a head of 64 is one line of 128 bytes: fetching its neighbour's along with it ran 1024 rows on two heads at 4.3 instead of 5.7 TB/s)
     const cuuint32_t estr[3] = {1u, 1u, 1u};
     const CUresult r = fn(reinterpret_cast<CUtensorMap *>(out), CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void *>(base), dims, strides, box, estr,
-                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, head_dim >= 128 ? CU_TENSOR_MAP_L2_PROMOTION_L2_256B : CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
