@@ -4,87 +4,134 @@
 //   pair i of a head, axis x(i) (the sections deal the pairs over the axes in order):  a = position[x(i)] * base^(-2 i / d)
 //   (u, w) -> (u cos a - w sin a, u sin a + w cos a), the pair being elements (i, i + d/2) or (2i, 2i + 1)
 //
-// Angles, sines and cosines are 64-bit (a position of 100 000 leaves an f32 angle two correct decimals) and rounded once to f32; the rotation is f32 and each
-// result is rounded once to the type it is stored as.
+// An angle is reduced to a turn's fraction in 64 bits (a position of 100 000 leaves an f32 angle two correct decimals); its sine and cosine are those of the fraction
+// rounded to f32, corrected by what the rounding left, 1e-7 off at most. The rotation is f32 and each result is rounded once to the type it is stored as.
+#include <cmath>
+
 #include "launch.cuh"
 #include "paged.cuh"
 
 namespace dooms {
 namespace cuda {
 
+using namespace dooms::dev;
+
 namespace {
 
-constexpr int kThreads = 256, kMostTokens = 4;
+constexpr int kThreads = 256, kAtOnce = 4;      // kAtOnce: units of a thread whose loads are in flight together
 
 struct RopeArgs {
-    double log2_base;
+    double turns[64];                   // base^(-2 i / d) / (2 pi): turns per position
     int neox, n_axes, axis_end[4];      // axis x has the pairs [axis_end[x - 1], axis_end[x])
 };
 
 __device__ __forceinline__ uint32_t pack(float a, float b) { const __half2 h = __floats2half2_rn(a, b); return *reinterpret_cast<const uint32_t *>(&h); }
 
-// A block takes `per_block` rows (1 to 4) and, of their heads, the share blockIdx.y of gridDim.y. It first makes the rows' (cos, sin) in shared memory, one
-// thread per pair, then every thread turns units of eight values (four pairs).
-template <int D, bool HALF_Q>
-__global__ void __launch_bounds__(kThreads) k_rope_store_paged(const PagedView c, const RopeArgs r, const float * __restrict__ qkv, int64_t stride, int n_head, int n_rows,
-                                                               const int32_t * __restrict__ sequence, const int32_t * __restrict__ at, const int32_t * __restrict__ positions,
-                                                               void * __restrict__ q_out, int per_block) {
-    constexpr int kPairs = D / 2, kUnits = D / 8;
-    __shared__ float2 cs[kMostTokens][kPairs];
-    __shared__ int64_t line[kMostTokens];
-    const int row0 = int(blockIdx.x) * per_block, rows = min(per_block, n_rows - row0);
-    if (int(threadIdx.x) < rows) {
+// Bound by device memory, and close to being bound by instructions: a row has TPR threads, each of which has the same eight values (four pairs) of every head it takes, so
+// that its sines and cosines stay in registers and its addresses are a step apart. (With rows and heads dealt by division and the pairs chosen at run time a unit
+// was 325 instructions: 68 us for 6000 rows of 40 + 8 heads of 128 instead of what the table in the design notes has.) Every thread asks for its first units,
+// then the block makes its rows' (cos, sin) in shared memory, one thread per pair, and looks the rows' places up, while those are on their way.
+template <int D, bool HALF_Q, bool NEOX, int TPR>
+__global__ void __launch_bounds__(kThreads, 4) k_rope_store_paged(const PagedView c, const __grid_constant__ RopeArgs r, const float * __restrict__ qkv, int64_t stride, int n_head,
+                                                               int n_rows, const int32_t * __restrict__ sequence, const int32_t * __restrict__ at,
+                                                               const int32_t * __restrict__ positions, void * __restrict__ q_out) {
+    constexpr int kPairs = D / 2, kUnits = D / 8, kRows = kThreads / TPR, kStep = TPR / kUnits;      // kStep heads apart: a thread's units
+    __shared__ __align__(16) float2 cs[kRows][kPairs];
+    __shared__ int64_t line[kRows];
+    pdl_wait();
+    const int row0 = int(blockIdx.x) * kRows, mine = threadIdx.x / TPR, row = row0 + mine, unit = threadIdx.x % TPR, part = unit % kUnits, head0 = unit / kUnits;
+    const int heads = n_head + 2 * c.n_kv;
+    // where in a head the unit's two times four values begin (a value head is taken the same way, and copied)
+    constexpr int kGap = NEOX ? kPairs : 4;
+    const int first = NEOX ? part * 4 : part * 8;
+    const bool there = row < n_rows;
+    const float * from = qkv + int64_t(row) * stride + int64_t(head0) * D + first;
+    float4 lo[kAtOnce], hi[kAtOnce];
+    auto load = [&](int h0) {
+        #pragma unroll
+        for (int k = 0; k < kAtOnce; k++) {
+            if (there && h0 + k * kStep < heads) {
+                lo[k] = __ldg(reinterpret_cast<const float4 *>(from + k * kStep * D));
+                hi[k] = __ldg(reinterpret_cast<const float4 *>(from + k * kStep * D + kGap));
+            }
+        }
+        from += kAtOnce * kStep * D;
+    };
+    load(head0);
+    if (threadIdx.x < kRows && row0 + int(threadIdx.x) < n_rows) {
         const int t = row0 + threadIdx.x, s = sequence[t];
         int64_t where = -1;
         if (s >= 0) {
             const int p = at[t];
             if (s < c.n_sequences && p >= 0 && p < c.capacity()) where = c.row(s, p);
-            if (where < 0 && blockIdx.y == 0) c.fail();
+            if (where < 0) c.fail();
         }
         line[threadIdx.x] = where;
     }
-    for (int i = threadIdx.x; i < rows * kPairs; i += kThreads) {
+    for (int i = threadIdx.x; i < kRows * kPairs; i += kThreads) {
         const int t = row0 + i / kPairs, pair = i % kPairs;
+        if (t >= n_rows) break;
         int axis = 0;
         while (axis < r.n_axes - 1 && pair >= r.axis_end[axis]) axis++;
-        const double a = double(positions[int64_t(axis) * n_rows + t]) * exp2(r.log2_base * (double(pair) * (-2.0 / D)));
-        double s, co;
-        sincos(a, &s, &co);
-        cs[i / kPairs][pair] = make_float2(float(co), float(s));
+        const double turns = double(positions[int64_t(axis) * n_rows + t]) * r.turns[pair], f = turns - rint(turns);
+        const float f32 = float(f), rest = float(f - double(f32)) * 6.28318530717958647693f;
+        float s, co;
+        sincospif(2.f * f32, &s, &co);
+        cs[i / kPairs][pair] = make_float2(fmaf(-s, rest, co), fmaf(co, rest, s));
     }
     __syncthreads();
-    const int heads = n_head + 2 * c.n_kv, units = rows * heads * kUnits;
-    for (int u = int(blockIdx.y) * kThreads + threadIdx.x; u < units; u += int(gridDim.y) * kThreads) {
-        const int part = u % kUnits, h = (u / kUnits) % heads, b = u / (kUnits * heads);
-        const int64_t where = line[b];
-        if (where < 0) continue;
-        const float * x = qkv + int64_t(row0 + b) * stride + int64_t(h) * D;
-        const bool value = h >= n_head + c.n_kv, halves = r.neox && !value;      // (values are taken in order)
-        const float4 lo = __ldg(reinterpret_cast<const float4 *>(x + (halves ? part * 4 : part * 8)));
-        const float4 hi = __ldg(reinterpret_cast<const float4 *>(x + (halves ? kPairs + part * 4 : part * 8 + 4)));
-        float y[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-        if (!value) {
-            #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const float2 e = cs[b][part * 4 + i];
-                const int iu = halves ? i : 2 * i, iw = halves ? 4 + i : 2 * i + 1;
-                const float uu = y[iu], ww = y[iw];
-                y[iu] = uu * e.x - ww * e.y;
-                y[iw] = uu * e.y + ww * e.x;
+    if (!there) return;
+    const int64_t where = line[mine];
+    if (where < 0) return;
+    const float4 e01 = *reinterpret_cast<const float4 *>(&cs[mine][part * 4]), e23 = *reinterpret_cast<const float4 *>(&cs[mine][part * 4 + 2]);
+    const float co[4] = {e01.x, e01.z, e23.x, e23.z}, si[4] = {e01.y, e01.w, e23.y, e23.w};
+    __half * const k_to = c.k + where * c.n_kv * D + first, * const v_to = c.v + where * c.n_kv * D + first;
+    const int64_t q_at = int64_t(row) * n_head * D + first;
+    for (int h0 = head0; h0 < heads; h0 += kAtOnce * kStep) {
+        if (h0 != head0) load(h0);
+        #pragma unroll
+        for (int k = 0; k < kAtOnce; k++) {
+            const int h = h0 + k * kStep;
+            if (h >= heads) break;
+            float a[4], b[4];      // the pairs, and then what they become
+            if (NEOX) {
+                a[0] = lo[k].x; a[1] = lo[k].y; a[2] = lo[k].z; a[3] = lo[k].w; b[0] = hi[k].x; b[1] = hi[k].y; b[2] = hi[k].z; b[3] = hi[k].w;
+            } else {
+                a[0] = lo[k].x; b[0] = lo[k].y; a[1] = lo[k].z; b[1] = lo[k].w; a[2] = hi[k].x; b[2] = hi[k].y; a[3] = hi[k].z; b[3] = hi[k].w;
+            }
+            if (h < n_head + c.n_kv) {
+                #pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const float u = a[i], w = b[i];
+                    a[i] = u * co[i] - w * si[i];
+                    b[i] = u * si[i] + w * co[i];
+                }
+            }
+            if (!HALF_Q && h < n_head) {
+                float * to = static_cast<float *>(q_out) + q_at + h * D;
+                *reinterpret_cast<float4 *>(to) = NEOX ? make_float4(a[0], a[1], a[2], a[3]) : make_float4(a[0], b[0], a[1], b[1]);
+                *reinterpret_cast<float4 *>(to + kGap) = NEOX ? make_float4(b[0], b[1], b[2], b[3]) : make_float4(a[2], b[2], a[3], b[3]);
+            } else {
+                __half * to = h < n_head ? static_cast<__half *>(q_out) + q_at + h * D : h < n_head + c.n_kv ? k_to + (h - n_head) * D : v_to + (h - n_head - c.n_kv) * D;
+                if (NEOX) {
+                    *reinterpret_cast<uint2 *>(to) = make_uint2(pack(a[0], a[1]), pack(a[2], a[3]));
+                    *reinterpret_cast<uint2 *>(to + kGap) = make_uint2(pack(b[0], b[1]), pack(b[2], b[3]));
+                } else {
+                    *reinterpret_cast<uint4 *>(to) = make_uint4(pack(a[0], b[0]), pack(a[1], b[1]), pack(a[2], b[2]), pack(a[3], b[3]));
+                }
             }
         }
-        const int first = halves ? part * 4 : part * 8, second = halves ? kPairs + part * 4 : part * 8 + 4;
-        if (h < n_head && !HALF_Q) {
-            float * q = static_cast<float *>(q_out) + (int64_t(row0 + b) * n_head + h) * D;
-            *reinterpret_cast<float4 *>(q + first) = make_float4(y[0], y[1], y[2], y[3]);
-            *reinterpret_cast<float4 *>(q + second) = make_float4(y[4], y[5], y[6], y[7]);
-        } else {
-            __half * o = h < n_head ? static_cast<__half *>(q_out) + (int64_t(row0 + b) * n_head + h) * D
-                                    : (value ? c.v : c.k) + (where * c.n_kv + (h - n_head - (value ? c.n_kv : 0))) * D;
-            *reinterpret_cast<uint2 *>(o + first) = make_uint2(pack(y[0], y[1]), pack(y[2], y[3]));
-            *reinterpret_cast<uint2 *>(o + second) = make_uint2(pack(y[4], y[5]), pack(y[6], y[7]));
-        }
     }
+}
+
+template <int D, bool HALF_Q, bool NEOX, class... Args>
+cudaError_t launch(int heads, int n_rows, cudaStream_t stream, Args... args) {
+    // threads per row: so many that a thread has at most four units or so, whose loads all go out at once
+    const int units = heads * (D / 8);
+    auto go = [&](auto kernel, int rows) { return launch_pdl(kernel, dim3(unsigned((n_rows + rows - 1) / rows)), dim3(kThreads), 0, stream, args...); };
+    if (units > 512) return go(k_rope_store_paged<D, HALF_Q, NEOX, 256>, 1);
+    if (units > 256) return go(k_rope_store_paged<D, HALF_Q, NEOX, 128>, 2);
+    return go(k_rope_store_paged<D, HALF_Q, NEOX, 64>, 4);
 }
 
 }  // namespace
@@ -92,15 +139,28 @@ __global__ void __launch_bounds__(kThreads) k_rope_store_paged(const PagedView c
 cudaError_t launch_rope_store_paged(const PagedCache & cache, const RopeSections & rope, const float * qkv, int64_t stride, int n_head, int n_rows, const int32_t * sequence,
                                     const int32_t * at, const int32_t * positions, void * q_out, bool half_q, int * error, cudaStream_t stream) {
     const PagedView c = paged_view(cache, error);
-    RopeArgs r{log2(rope.base), rope.neox, rope.n_axes, {0, 0, 0, 0}};
+    // the table of the last base and head size that this thread used: a program has one
+    struct Table { double base = 0.0; int head_dim = 0; RopeArgs args; };
+    static thread_local Table table;
+    if (table.base != rope.base || table.head_dim != cache.head_dim) {
+        for (int i = 0; i < cache.head_dim / 2; i++) table.args.turns[i] = std::pow(rope.base, -2.0 * i / cache.head_dim) / 6.28318530717958647693;
+        table.base = rope.base;
+        table.head_dim = cache.head_dim;
+    }
+    RopeArgs r = table.args;
+    r.neox = rope.neox;
+    r.n_axes = rope.n_axes;
     for (int x = 0, end = 0; x < 4; x++) r.axis_end[x] = end += rope.sections[x];
-    const int per_block = n_rows >= kMostTokens * 2 * sm_count() ? kMostTokens : 1;
-    const dim3 grid(unsigned((n_rows + per_block - 1) / per_block), 1u);
-    auto go = [&](auto kernel) { kernel<<<grid, kThreads, 0, stream>>>(c, r, qkv, stride, n_head, n_rows, sequence, at, positions, q_out, per_block); };
-    if (cache.head_dim == 128) half_q ? go(k_rope_store_paged<128, true>) : go(k_rope_store_paged<128, false>);
-    else if (cache.head_dim == 64) half_q ? go(k_rope_store_paged<64, true>) : go(k_rope_store_paged<64, false>);
-    else return cudaErrorInvalidValue;
-    return cudaGetLastError();
+    const int heads = n_head + 2 * cache.n_head_kv;
+    auto go = [&]<int D>() {
+        auto with = [&](auto launcher) { return launcher(heads, n_rows, stream, c, r, qkv, stride, n_head, n_rows, sequence, at, positions, q_out); };
+        using L = cudaError_t (*)(int, int, cudaStream_t, PagedView, RopeArgs, const float *, int64_t, int, int, const int32_t *, const int32_t *, const int32_t *, void *);
+        const L launchers[4] = {launch<D, false, false>, launch<D, false, true>, launch<D, true, false>, launch<D, true, true>};
+        return with(launchers[2 * half_q + (rope.neox != 0)]);
+    };
+    if (cache.head_dim == 128) return go.template operator()<128>();
+    if (cache.head_dim == 64) return go.template operator()<64>();
+    return cudaErrorInvalidValue;
 }
 
 }  // namespace cuda

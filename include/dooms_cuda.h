@@ -271,8 +271,8 @@ typedef struct dooms_cuda_rope {
 } dooms_cuda_rope;
 /* rope_store (llama_kernels.h:521-545) for rows of many sequences: of row r of d_qkv (n_head query heads, n_head_kv key heads, n_head_kv value heads of f32, rows
  * qkv_stride floats apart, a multiple of 4; 16-byte aligned) the queries are turned into d_q [n_rows][n_head][head_dim] (q_dtype DOOMS_F32 or DOOMS_F16; 16-byte
- * aligned, apart from d_qkv), keys (turned) and values are rounded to f16 and written to position d_at[r] of sequence d_sequence[r] (negative: an idle row, nothing
- * of which is read or written). d_positions: int32 [n_axes][n_rows]. No position twice in one call. n_head: a multiple of n_head_kv, at most 64 times. */
+ * aligned, apart from d_qkv), keys (turned) and values are rounded to f16 and written to position d_at[r] of sequence d_sequence[r] (negative: an idle row, of which
+ * nothing is written). d_positions: int32 [n_axes][n_rows]. No position twice in one call. n_head: a multiple of n_head_kv, at most 64 times. */
 DOOMS_CUDA_API int32_t dooms_cuda_rope_store_paged(const dooms_cuda_paged_cache * cache, const dooms_cuda_rope * rope, const float * d_qkv, int64_t qkv_stride, int32_t n_head,
                                                    int32_t n_rows, const int32_t * d_sequence, const int32_t * d_at, const int32_t * d_positions, int32_t q_dtype, void * d_q,
                                                    void * stream);
