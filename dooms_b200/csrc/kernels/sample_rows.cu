@@ -3,13 +3,15 @@
 //   kept by top-k: the first k;  by top-p: while what is in front of a token holds less than top_p of the mass e^-g of what top-k kept;  by min-p: e^-g >= min_p;
 //   the token: the first whose cumulative weight e^(-g / T) exceeds u times the kept tokens' total.
 //
-// A row belongs to one block, or to a cluster of up to eight that share it, as many as there are rows for: a batch of many rows is one wave of blocks that stream. The
-// first pass finds the maximum and a bound for a top-k (see there); later passes read the row from L2. A cut ("the first element at which a cumulative weight
-// reaches a goal") is found by a histogram over all blocks of the cluster, of 1/24 nat per bin up to 10 nats below m (what is further down is summed in registers, and
-// divided only if the goal falls there), then by sorting the few elements of the bin where the goal falls. As soon as little enough is left to look at (what
-// is above a top-k's bound or a min-p's limit, or in front of a goal) the blocks list it and work on the lists; and where that is at most kList elements, they
-// are sorted and everything else is decided among them. A bin of more than kList elements is divided again by the bits of the logits, down to a single value,
-// whose elements are counted out in the order of their indices.
+// A row belongs to one block, or to a cluster of up to eight that share it. The first pass finds the maximum and a bound (see there): for a top-k one that the k largest
+// lie above, where a total of everything is needed one that a tenth of the row does; later passes read the row from L2. A cut ("the first element at which a
+// cumulative weight reaches a goal") is found by a histogram over all blocks of the cluster, of 1/24 nat per bin, then by sorting the few elements of the bin where
+// the goal falls. Histograms are of lists wherever there is one to make (what is above the bound or a min-p's limit, a step below the bound, or in front of a goal):
+// an element costs a histogram some hundred instructions, a list two votes, and the sum of the weights that are in no list some fifty. Where at most kList
+// elements are left to look at, they are sorted and everything else is decided among them. A bin of more than kList elements is divided again by the bits of the
+// logits, down to a single value, whose elements are counted out in the order of their indices.
+// Bound by instructions where a total is needed (256 rows of 128256, B200: 290 to 500 us), else by latencies and memory (top-k 40: 63 us, the largest alone: 34 us of
+// the 20 that reading the 131 MB takes).
 // Weights are 64-bit integers, e^-x 2^45 rounded (x and the exponential in 64-bit floating point): sums do not depend on the order of the atomics, and the blocks of
 // a cluster, which all work out every cut for themselves, agree on it. 2^18 logits of the largest weight still fit. What is rounded off is 2^-46 of
 // the row's largest weight per token.
@@ -34,7 +36,8 @@ constexpr int kMostLogits = 1 << 18;
 constexpr float kBinsPerNat = 24.f, kFarBinsPerNat = 8.f;
 constexpr int kFar = 240;              // the bin of everything from 10 nats below the largest logit on
 constexpr int kPowers = 256;
-constexpr int kNearMost = 4096;        // logits a block lists
+constexpr int kNearMost = 8192, kPerWarp = kNearMost / (kThreads / 32);      // logits a block lists, and each of its warps
+constexpr int kSamples = 8;            // logits per thread that say how far down a list goes
 constexpr double kNoLimit = 1e300;     // (gaps are below 2^129, or infinite)
 static_assert(kList == kThreads && kBins <= kThreads, "one list element and at most one bin per thread");
 
@@ -42,11 +45,14 @@ struct SampleArgs {
     const float * logits;
     int64_t stride;
     int n, slice;
+    int sample_every, sample_rank;      // of a thread's groups of four logits one in so many (a power of two) is sampled; m (see the kernel)
     const float * temperature, * top_p, * min_p, * uniform;
     const int32_t * top_k;
     int32_t * tokens;
     float * probability;
+    int rows_of;
 };
+enum { kAllRows, kBoundedRows, kOpenRows };
 
 struct Shared {
     uint32_t count[kBins], low[kBins], high[kBins];      // this block's histogram: elements, and their weights in two words
@@ -56,8 +62,9 @@ struct Shared {
     unsigned long long warp_sum[kThreads / 32];
     float near_value[kNearMost];
     int near_at[kNearMost];                              // where in the share
-    uint32_t n_near;
-    unsigned long long rest[2];                          // weights of what is not listed
+    uint32_t n_near;                                     // all of them; kNearMost + 1 where a warp's did not fit
+    int warp_near[kThreads / 32];
+    unsigned long long rest[3];                          // weights of what is not listed
     uint32_t n_local, lo_key, hi_key, index, ties;
     float top, bound;
     // what a step leaves for all threads
@@ -134,27 +141,31 @@ struct Row {
     }
 };
 
-// f(value, place) for this thread's logits at work: of the share four at a time, with kAhead loads in flight.
+// f(value, place) for this thread's logits at work: of the share four at a time, with kAhead loads in flight; of a list, what the thread's warp has of it. All lanes
+// of a warp make the same calls: what is not there is a NaN, which is larger than nothing, equal to nothing and weighs nothing.
 template <int kAhead, class F>
 __device__ __forceinline__ void each(const Row & r, F f) {
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const float none = __int_as_float(0x7fffffff);
     if (r.at || !r.wide) {
-        #pragma unroll 4
-        for (int i = threadIdx.x; i < r.here; i += kThreads) f(r.x[i], i);
+        const int step = r.at ? 32 : kThreads, begin = r.at ? warp * kPerWarp : warp * 32, end = r.at ? begin + r.here : r.here;
+        #pragma unroll 2
+        for (int i = begin; i < end; i += step) f(i + lane < end ? r.x[i + lane] : none, i + lane);
         return;
     }
     const int quads = r.here / 4;
     const float4 * x4 = reinterpret_cast<const float4 *>(r.x);
     auto four = [&](float4 v, int i) { f(v.x, 4 * i); f(v.y, 4 * i + 1); f(v.z, 4 * i + 2); f(v.w, 4 * i + 3); };
-    int i = threadIdx.x;
-    for (; i + (kAhead - 1) * kThreads < quads; i += kAhead * kThreads) {
+    int i = warp * 32;
+    for (; i + (kAhead - 1) * kThreads + 31 < quads; i += kAhead * kThreads) {
         float4 v[kAhead];
         #pragma unroll
-        for (int j = 0; j < kAhead; j++) v[j] = __ldg(x4 + i + j * kThreads);
+        for (int j = 0; j < kAhead; j++) v[j] = __ldg(x4 + i + lane + j * kThreads);
         #pragma unroll
-        for (int j = 0; j < kAhead; j++) four(v[j], i + j * kThreads);
+        for (int j = 0; j < kAhead; j++) four(v[j], i + lane + j * kThreads);
     }
-    for (; i < quads; i += kThreads) four(__ldg(x4 + i), i);
-    if (4 * quads + int(threadIdx.x) < r.here) f(r.x[4 * quads + threadIdx.x], 4 * quads + int(threadIdx.x));
+    for (; i < quads; i += kThreads) four(i + lane < quads ? __ldg(x4 + i + lane) : make_float4(none, none, none, none), i + lane);
+    if (warp == 0 && 4 * quads < r.here) f(4 * quads + lane < r.here ? r.x[4 * quads + lane] : none, 4 * quads + lane);
 }
 
 // Inclusive sums over the block of a value per thread; *total: of all.
@@ -211,7 +222,12 @@ __device__ int gather(Row & r, Take take) {
     r.list_used = true;
     if (threadIdx.x == 0) s.n_local = 0;
     __syncthreads();
-    each<4>(r, [&](float v, int i) { if (take(v, i)) s.local[atomicAdd(&s.n_local, 1u)] = (unsigned long long)key_of(v) << 32 | (0xffffffffu - r.index(i)); });
+    each<4>(r, [&](float v, int i) {
+        if (take(v, i)) {
+            const uint32_t n = atomicAdd(&s.n_local, 1u);
+            if (n < kList) s.local[n] = (unsigned long long)key_of(v) << 32 | (0xffffffffu - r.index(i));
+        }
+    });
     cluster_barrier();
     uint32_t from, at;
     const uint32_t n = deal(&s.n_local, r.blocks, &from, &at);
@@ -365,6 +381,8 @@ __device__ void resolve(Row & r, bool by_count, double per, unsigned long long g
 __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const SampleArgs a) {
     extern __shared__ __align__(16) uint8_t smem[];
     Shared & s = *reinterpret_cast<Shared *>(smem);
+    // With two launches the second may start as soon as the first's blocks have, which is when what both read is there; it waits for the first at its end.
+    if (a.rows_of != kOpenRows) { pdl_wait(); pdl_trigger(); }
     uint32_t rank, blocks;
     asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
     asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(blocks));
@@ -375,24 +393,31 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const SampleArgs a)
     const float t = a.temperature ? a.temperature[row] : 1.f, top_p = a.top_p ? a.top_p[row] : 1.f, min_p = a.min_p ? a.min_p[row] : 0.f, uniform = a.uniform[row];
     const int k = a.top_k ? a.top_k[row] : 0;
     const bool greedy = !(t > 0.f), by_k = k > 0 && k < a.n, by_p = top_p < 1.f, by_m = min_p > 0.f;
+    // open: a total of everything is needed. What is listed there is what lies above the least of the warps' m-th largest of the threads' largest of kSamples logits each: a
+    // share of the row that does not depend on what its logits are like.
+    const bool open = !greedy && !by_k && (by_p || !by_m), bounded = open || (by_k && k <= kThreads && !greedy);
+    // (rows of the other launch: their clusters leave at once)
+    if (a.rows_of != kAllRows && open != (a.rows_of == kOpenRows)) { if (a.rows_of == kOpenRows) pdl_wait(); return; }
     if (threadIdx.x < kPowers) s.power[threadIdx.x] = exp2(double(threadIdx.x) * (-1.0 / kPowers));
     if (threadIdx.x == 0) { s.n_near = 0; s.index = 0xffffffffu; }
 
     // ---- the first pass: every thread's largest logit, and with them the row's ----
     Row r{from, first, here, wide, from, nullptr, here, rank, blocks, s, 0.f, 0.0};
-    float mine = -CUDART_INF_F;
+    float mine = -CUDART_INF_F, sample = -CUDART_INF_F;
     uint32_t mine_at = 0xffffffffu;
     if (greedy) each<8>(r, [&](float v, int i) { if (v > mine) { mine = v; mine_at = uint32_t(first + i); } });      // (a NaN loses, and the first of equal ones wins)
-    else each<8>(r, [&](float v, int) { mine = fmaxf(mine, v); });
+    else if (!open) each<8>(r, [&](float v, int) { mine = fmaxf(mine, v); });
+    else each<8>(r, [&](float v, int i) {
+        mine = fmaxf(mine, v);
+        if (i % 4 == 0 && (i / (4 * kThreads) & (a.sample_every - 1)) == 0) sample = fmaxf(sample, v);
+    });
     float top = mine;
     #pragma unroll
     for (int m = 16; m; m >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, m));
     // A bound for a top-k: if every warp has m = k / 16 (rounded up) threads with a logit of at least b, the row has k of them. b: the least of the warps' m-th largest.
-    // Where a total of everything is needed, m = 30: one or two in a hundred of a row of 128256 lie above the bound, whatever the logits are like.
-    const bool open = !greedy && !by_k && (by_p || !by_m), bounded = open || (by_k && k <= kThreads && !greedy);
     float bound = -CUDART_INF_F;
     if (bounded) {
-        float v = mine;      // sorted over the lanes, largest first
+        float v = open ? sample : mine;      // sorted over the lanes, largest first
         #pragma unroll
         for (int size = 2; size <= 32; size *= 2) {
             #pragma unroll
@@ -402,7 +427,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const SampleArgs a)
                 v = larger_first ? fmaxf(v, o) : fminf(v, o);
             }
         }
-        bound = __shfl_sync(0xffffffffu, v, open ? 29 : (k + kThreads / 32 - 1) / (kThreads / 32) - 1);
+        bound = __shfl_sync(0xffffffffu, v, open ? a.sample_rank - 1 : (k + kThreads / 32 - 1) / (kThreads / 32) - 1);
     }
     float2 * const tops = reinterpret_cast<float2 *>(s.warp_sum);
     if (lane == 0) tops[warp] = make_float2(top, bound);
@@ -454,20 +479,30 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const SampleArgs a)
             const double u = double(uniform) * double(total);
             return u > 0.0 ? min(total, (unsigned long long)u + 1ull) : 1ull;
         };
-        // the block's logits that take(v, i) takes, as the list to work on from here
-        auto list = [&](auto take) {
+        // The list: every warp appends to a piece of its own, so that no counter is shared.
+        int listed_here = 0;
+        auto append = [&](bool take, float v, int i) {
+            const uint32_t m = __ballot_sync(0xffffffffu, take);
+            if (m) {
+                const int at = listed_here + __popc(m & ((1u << lane) - 1u));
+                if (take && at < kPerWarp) { s.near_value[warp * kPerWarp + at] = v; s.near_at[warp * kPerWarp + at] = i; }
+                listed_here += __popc(m);
+            }
+        };
+        bool lists_made = false;
+        auto list_begin = [&] {
+            if (lists_made) cluster_barrier();      // (others may still read the last one's number)
+            lists_made = true;
             __syncthreads();
             if (threadIdx.x == 0) s.n_near = 0;
             __syncthreads();
-            each<4>(r, [&](float v, int i) {
-                if (take(v, i)) {
-                    const uint32_t n = atomicAdd(&s.n_near, 1u);
-                    if (n < kNearMost) { s.near_value[n] = v; s.near_at[n] = i; }
-                }
-            });
-            __syncthreads();
+            listed_here = 0;
         };
-        auto use_list = [&] { r.x = s.near_value; r.at = s.near_at; r.here = int(s.n_near); };
+        auto list_end = [&] {
+            if (lane == 0) atomicAdd(&s.n_near, listed_here > kPerWarp ? uint32_t(kNearMost + 1) : uint32_t(listed_here));
+            listed_here = min(listed_here, kPerWarp);
+        };
+        auto use_list = [&] { r.x = s.near_value; r.at = s.near_at; r.here = listed_here; };
 
         auto sorted_up_to = [&](int to) { return gather(r, [&](float v, int i) { return r.kept(v, i) && r.bin(v) <= to; }); };
         bool listed = false;
@@ -475,92 +510,102 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const SampleArgs a)
         unsigned long long total_p = 0;
         float cut;
         uint32_t index;
+        auto use_share = [&] { r.x = r.share; r.at = nullptr; r.here = r.n_share; };
+        auto fits = [&] { return most_of_blocks(&s.n_near, blocks) <= kNearMost; };
+
         // ---- a top-k's bound, or a min-p alone, says at once what to look at ----
         const bool alone = least > -CUDART_INF_F && !by_k && !by_p;
-        // ---- or where a total is needed: what is above the bound is listed, and the weights of the rest added up, in two steps down ----
-        bool totals = false;                          // whether rest[] is that, of weights e^(-gap per_rest / log2 e)
-        const float near = alone ? least : fmaxf(bound, -3.402823466e38f), step = float(2.0 * kLog2e / (by_p ? kLog2e : per_t)), down = near - step;
-        unsigned long long rest[2] = {0, 0};          // of everything below near, and below down
-        if (alone || bounded) {
-            if (!open) {
-                list([&](float v, int) { return v >= near; });
-            } else {
-                const double per = by_p ? kLog2e : per_t;
-                __syncthreads();
-                if (threadIdx.x == 0) { s.n_near = 0; s.rest[0] = s.rest[1] = 0; }
-                __syncthreads();
+        const float near = alone ? least : fmaxf(bound, -3.402823466e38f);
+        if (alone || (by_k && bounded)) {
+            list_begin();
+            each<4>(r, [&](float v, int i) { append(v >= near, v, i); });
+            list_end();
+            cluster_barrier();
+            const uint32_t n_near = of_blocks(&s.n_near, blocks, 0u, [](uint32_t v) { return __reduce_add_sync(0xffffffffu, v); });
+            if (fits()) use_list();
+            if (n_near <= kList) {
+                n = gather(r, [](float v, int) { return v == v; });
+                listed = true;
+            }
+        }
+
+        // A cut over what is kept. Of a list: the histogram. Of the share, by count: the histogram, its far bin divided if the goal falls there; what is in front of the goal
+        // becomes the list where it fits. Of the share, by weight: one pass without a branch adds up the weights below three steps down from the bound and lists what
+        // is above it; if the goal is in front of the end of one of the steps, that step is listed; if not (or if a list does not fit), the histogram of the share. Then
+        // the element.
+        int where = 0;      // what the histogram was of: 0 bins from the largest logit down, 1 the far bin's, 2 a step's
+        float step_top = 0.f, step_scale = 0.f, step_end = 0.f;
+        auto step_bin = [&](float v) { return int(fminf((step_top - v) * step_scale, float(kBins - 1))); };
+        auto every = [](float) { return true; };
+        auto from_top = [&](float v) { return r.bin(v); };
+        auto divide = [&](bool by_count, double per, auto goal) {
+            where = 0;
+            if (!r.at && !by_count) {
+                const float nat = float(kLog2e / per), down1 = near - 0.7f * nat, down2 = near - 1.6f * nat;
+                unsigned long long rest[3] = {0, 0, 0};       // the weights below near, down1, down2
+                list_begin();
+                if (threadIdx.x < 3) s.rest[threadIdx.x] = 0;
                 each<2>(r, [&](float v, int i) {
-                    const unsigned long long w = r.weight_of((r.top64 - double(v)) * per);
+                    const bool kept = r.kept(v, i);
+                    const unsigned long long w = r.weight_of(kept ? (r.top64 - double(v)) * per : 64.0);
                     rest[0] += v < near ? w : 0ull;
-                    rest[1] += v < down ? w : 0ull;
-                    if (v >= near) {
-                        const uint32_t n = atomicAdd(&s.n_near, 1u);
-                        if (n < kNearMost) { s.near_value[n] = v; s.near_at[n] = i; }
-                    }
+                    rest[1] += v < down1 ? w : 0ull;
+                    rest[2] += v < down2 ? w : 0ull;
+                    append(kept && v >= near, v, i);
                 });
+                __syncthreads();
                 #pragma unroll
-                for (int j = 0; j < 2; j++) {
+                for (int j = 0; j < 3; j++) {
                     #pragma unroll
                     for (int d = 16; d; d >>= 1) rest[j] += __shfl_xor_sync(0xffffffffu, rest[j], d);
                     if (lane == 0) atomicAdd(&s.rest[j], rest[j]);
                 }
-            }
-            cluster_barrier();
-            if (open) {
+                list_end();
+                cluster_barrier();
                 #pragma unroll
-                for (int j = 0; j < 2; j++) {
+                for (int j = 0; j < 3; j++) {
                     rest[j] = lane < int(blocks) ? ld_remote(&s.rest[j], lane) : 0ull;
                     #pragma unroll
                     for (int d = kMostBlocks / 2; d; d >>= 1) rest[j] += __shfl_xor_sync(0xffffffffu, rest[j], d);
                     rest[j] = __shfl_sync(0xffffffffu, rest[j], 0);
                 }
-            }
-            uint32_t list_from, list_at;
-            const uint32_t n_near = deal(&s.n_near, blocks, &list_from, &list_at);
-            if (n_near <= kList && !(open && rest[0])) {
-                unsigned long long e = 0;
-                if (threadIdx.x < n_near) {
-                    const float v = __uint_as_float(ld_remote(reinterpret_cast<const uint32_t *>(s.near_value) + list_at, list_from));
-                    const uint32_t i = ld_remote(reinterpret_cast<const uint32_t *>(s.near_at) + list_at, list_from);
-                    e = (unsigned long long)key_of(v) << 32 | (0xffffffffu - (list_from * uint32_t(a.slice) + i));
+                if (fits()) {
+                    use_list();
+                    histogram<false>(r, false, per, 0, rest[0], every, from_top, goal);
+                    if (s.bin < kBins) return;
+                    const unsigned long long all = s.total, g = goal(all);
+                    use_share();
+                    if (g <= all - rest[2]) {
+                        const bool second = g > all - rest[1];
+                        where = 2;
+                        step_top = second ? down1 : near;
+                        step_end = second ? down2 : down1;
+                        step_scale = float(kBins) / (step_top - step_end);
+                        list_begin();
+                        each<4>(r, [&](float v, int i) { append(v < step_top && v >= step_end && r.kept(v, i), v, i); });
+                        list_end();
+                        cluster_barrier();
+                        if (fits()) use_list();
+                        histogram<false>(r, false, per, second ? all - rest[1] : all - rest[0], second ? rest[2] : rest[1], [&](float v) { return v < step_top && v >= step_end; }, step_bin, goal);
+                        return;
+                    }
                 }
-                sort_list(s, int(n_near), e);
-                n = int(n_near);
-                listed = true;
-            } else if (most_of_blocks(&s.n_near, blocks) <= kNearMost) {
-                use_list();
-                totals = open;
             }
-        }
-        // A cut over what is kept: the histogram (of the list, or of the share, the far bin divided if the goal falls there); what is in front of the goal becomes the list
-        // where it is few enough; then the element. With totals, a goal behind the list falls on one of the two steps, which alone is divided.
-        int where = 0;      // what the histogram was of: 0 bins from the largest logit down, 1 the far bin's, 2 a step's
-        float step_top = 0.f, step_scale = 0.f, step_end = 0.f;
-        auto step_bin = [&](float v) { return int(fminf((step_top - v) * step_scale, float(kBins - 1))); };
-        auto divide = [&](bool by_count, double per, auto goal) {
-            where = 0;
-            histogram<true>(r, by_count, per, 0, totals ? rest[0] : 0ull, [](float) { return true; }, [&](float v) { return r.bin(v); }, goal);
-            if (totals && s.bin == kBins) {
-                const unsigned long long all = s.total, g = goal(all), listed_weight = all - rest[0];
-                const bool lower = g > all - rest[1];
-                where = 2;
-                step_top = lower ? down : near;
-                step_end = lower ? -CUDART_INF_F : down;
-                step_scale = lower ? 16.f / step : float(kBins) / step;
-                r.x = r.share; r.at = nullptr; r.here = r.n_share;
-                totals = false;
-                histogram<false>(r, by_count, per, lower ? all - rest[1] : listed_weight, lower ? 0ull : rest[1], [&](float v) { return v < step_top && v >= step_end; }, step_bin, goal);
+            if (r.at) {
+                histogram<false>(r, by_count, per, 0, 0, every, from_top, goal);
                 return;
             }
-            totals = false;
-            if (r.at) return;
+            histogram<true>(r, by_count, per, 0, 0, every, from_top, goal);
             if (s.bin == kFar) {
                 where = 1;
                 histogram<false>(r, by_count, per, s.before, 0, [&](float v) { return r.bin(v) == kFar; }, [&](float v) { return r.far_bin(v); }, goal);
             } else if (s.bin < kBins && s.up_to > kList && s.up_to <= kNearMost) {
                 const int to = s.bin;
-                list([&](float v, int i) { return r.kept(v, i) && r.bin(v) <= to; });
-                use_list();
+                list_begin();
+                each<4>(r, [&](float v, int i) { append(r.kept(v, i) && r.bin(v) <= to, v, i); });
+                list_end();
+                cluster_barrier();
+                if (fits()) use_list();
             }
         };
         auto element = [&](bool by_count, double per, unsigned long long goal, float * value, uint32_t * index) {
@@ -568,6 +613,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const SampleArgs a)
             resolve(r, by_count, per, goal, [&](float v) {
                 return w == 0 ? r.bin(v) == bin : w == 1 ? r.bin(v) == kFar && r.far_bin(v) == bin : v < step_top && v >= step_end && step_bin(v) == bin;
             }, value, index);
+            if (w != 0) use_share();      // (a step's list is not all that is kept)
         };
         if (by_k && !listed) {
             divide(true, 0.0, [&](unsigned long long) { return (unsigned long long)k; });
@@ -610,6 +656,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const SampleArgs a)
         if (a.probability) a.probability[row] = float(chance);
     }
     cluster_barrier();      // no block leaves while another reads its shared memory
+    if (a.rows_of == kOpenRows) pdl_wait();      // the first launch's rows are done when this one is
 }
 
 }  // namespace
@@ -618,30 +665,46 @@ int sample_rows_most() { return kMostLogits; }
 
 cudaError_t launch_sample_rows(const float * logits, int64_t stride, int rows, int n, const float * temperature, const int32_t * top_k, const float * top_p, const float * min_p,
                                const float * uniform, int32_t * tokens, float * probability, cudaStream_t stream) {
-    // As many blocks per row, each of at least 2048 logits, as make up to four per SM (two are resident): a cluster costs a row its barriers, a single block leaves the
-    // rows that need a total of everything to themselves. 256 rows of 128256, top-k 40 / a mix of filters: 56 / 503 us with one block, 58 / 287 with two, 92 / 235 with
-    // four, 156 / 287 with eight.
-    int blocks = 1;
-    while (blocks < kMostBlocks && n > blocks * 2048 && int64_t(rows) * blocks * 2 <= 4 * sm_count()) blocks *= 2;
-    const int slice = ((n + blocks - 1) / blocks + 3) & ~3;      // (whole 16 bytes, so that every block's share begins as the row does)
     if (n < 1 || n > kMostLogits) return cudaErrorInvalidValue;
     constexpr int bytes = int(sizeof(Shared));
     static std::atomic<uint64_t> done{0};
     cudaError_t e = allow_dynamic_smem(k_sample_rows, bytes, done);
     if (e != cudaSuccess) return e;
-    const SampleArgs a{logits, stride, n, slice, temperature, top_p, min_p, uniform, top_k, tokens, probability};
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(unsigned(rows) * unsigned(blocks));
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = size_t(bytes);
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = unsigned(blocks);
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, k_sample_rows, a);
+    // As many blocks per row, each of at least 2048 logits, as make up to `most` in all: a cluster costs a row its barriers, but a block alone leaves a row that needs a total
+    // of everything to itself.
+    auto blocks_for = [&](int64_t most) {
+        int blocks = 1;
+        while (blocks < kMostBlocks && n > blocks * 2048 && int64_t(rows) * blocks * 2 <= most) blocks *= 2;
+        return blocks;
+    };
+    auto go = [&](int rows_of, int blocks) {
+        const int slice = ((n + blocks - 1) / blocks + 3) & ~3;      // (whole 16 bytes, so that every block's share begins as the row does)
+        const double groups = slice / 4.0 / kThreads, share = std::min(0.1, 0.5 * kNearMost / slice);
+        int every = 1;
+        while (every * 2 * kSamples <= groups) every *= 2;
+        const int samples = std::max(1, int(groups / every)), rank = std::clamp(int(32.0 * (1.0 - std::pow(1.0 - share, samples))), 1, 32);
+        const SampleArgs a{logits, stride, n, slice, every, rank, temperature, top_p, min_p, uniform, top_k, tokens, probability, rows_of};
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3(unsigned(rows) * unsigned(blocks));
+        cfg.blockDim = dim3(kThreads);
+        cfg.dynamicSmemBytes = size_t(bytes);
+        cfg.stream = stream;
+        cudaLaunchAttribute attr[2];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = unsigned(blocks);
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[1].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = pdl_enabled() ? 2 : 1;
+        return cudaLaunchKernelEx(&cfg, k_sample_rows, a);
+    };
+    const int all = blocks_for(4 * sm_count());
+    if (all == blocks_for(INT64_MAX)) return go(kAllRows, all);
+    // Too many rows for that: those that a bound leaves little of with few blocks each, the others with as many as there can be, in two launches that overlap. 256 rows of
+    // 128256, top-k 40 / a mix of filters: one launch with two blocks a row 59 / 300 us, with four 95 / 244, with eight 159 / 289; two launches 63 / 257.
+    e = go(kBoundedRows, all);
+    return e == cudaSuccess ? go(kOpenRows, blocks_for(INT64_MAX)) : e;
 }
 
 }  // namespace cuda

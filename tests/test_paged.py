@@ -692,6 +692,30 @@ def test_sampling_twice_gives_the_same_and_rows_do_not_touch_one_another():
     assert torch.equal(out[0], out[1]) and torch.equal(out[0][::7], out[2][::7])
 
 
+@gpu
+@pytest.mark.parametrize("rows, n", [(75, 20000), (160, 17000), (400, 5000)])
+def test_sampling_batches_of_mixed_rows(rows, n):
+    """More rows than there are blocks for eight each: rows that a bound leaves little of and rows that need a total go in two launches, also under a capture."""
+    g = np.random.default_rng(rows)
+    names = list(FILTERS)
+    kind = [names[i] for i in g.integers(0, len(names), rows)]
+    x = (g.standard_normal((rows, n)) * g.choice([0.05, 1.0, 2.5, 6.0], rows)[:, None]).astype(np.float32)
+    t, p, m = (np.array([FILTERS[name][i] for name in kind], dtype=np.float32) for i in (0, 2, 3))
+    k, u = np.array([FILTERS[name][1] for name in kind], dtype=np.int32), g.random(rows).astype(np.float32)
+    check_sample(x, t, k, p, m, u)
+    d = [cuda(a) for a in (x, u, t, k, p, m)]
+    tokens, prob = torch.full((rows,), -9, dtype=torch.int32, device="cuda"), torch.zeros(rows, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        d[0].mul_(1.0)                         # what the sampling reads is made by the kernel in front of it, and read by the one behind it
+        paged.sample_rows(d[0], d[1], tokens, prob, *d[2:], stream=torch.cuda.current_stream().cuda_stream)
+        copy = tokens.clone()
+    for _ in range(3):
+        tokens.fill_(-9)
+        graph.replay()
+    assert copy.tolist() == [chain(x[r], t[r], k[r], p[r], m[r], u[r])[0] for r in range(rows)]
+
+
 # ---------------------------------------------------------------- together
 
 @gpu
