@@ -10,7 +10,7 @@
 // an element costs a histogram some hundred instructions, a list two votes, and the sum of the weights that are in no list some fifty. Where at most kList
 // elements are left to look at, they are sorted and everything else is decided among them. A bin of more than kList elements is divided again by the bits of the
 // logits, down to a single value, whose elements are counted out in the order of their indices.
-// Bound by instructions where a total is needed (256 rows of 128256, B200: 290 to 500 us), else by latencies and memory (top-k 40: 63 us, the largest alone: 34 us of
+// Bound by instructions where a total is needed (256 rows of 128256, B200: 231 us at no filter, 291 at a nucleus), else by latencies and memory (top-k 40: 60 us, the largest alone: 34 us of
 // the 20 that reading the 131 MB takes).
 // Weights are 64-bit integers, e^-x 2^45 rounded (x and the exponential in 64-bit floating point): sums do not depend on the order of the atomics, and the blocks of
 // a cluster, which all work out every cut for themselves, agree on it. 2^18 logits of the largest weight still fit. What is rounded off is 2^-46 of
@@ -699,12 +699,13 @@ cudaError_t launch_sample_rows(const float * logits, int64_t stride, int rows, i
         cfg.numAttrs = pdl_enabled() ? 2 : 1;
         return cudaLaunchKernelEx(&cfg, k_sample_rows, a);
     };
-    const int all = blocks_for(4 * sm_count());
-    if (all == blocks_for(INT64_MAX)) return go(kAllRows, all);
-    // Too many rows for that: those that a bound leaves little of with few blocks each, the others with as many as there can be, in two launches that overlap. 256 rows of
-    // 128256, top-k 40 / a mix of filters: one launch with two blocks a row 59 / 300 us, with four 95 / 244, with eight 159 / 289; two launches 63 / 257.
+    const int all = blocks_for(4 * sm_count()), open = std::max(all, std::min(blocks_for(INT64_MAX), 4));
+    if (all == open) return go(kAllRows, all);
+    // Too many rows for four blocks each: those that a bound leaves little of get fewer, the others four, in two launches that overlap. Rows x logits, mix of filters /
+    // nucleus alone, with eight blocks for the open rows against four, in us: 256 x 32000 143 / 321 against 105 / 143, 256 x 128256 257 / 499 against 244 / 291,
+    // 128 x 151936 (four fit all rows, one launch) 178 / 267 against 178 / 194. One launch of two blocks for all 256 rows: 300 for the mix, of four: 95 for top-k 40 alone (two: 59).
     e = go(kBoundedRows, all);
-    return e == cudaSuccess ? go(kOpenRows, blocks_for(INT64_MAX)) : e;
+    return e == cudaSuccess ? go(kOpenRows, open) : e;
 }
 
 }  // namespace cuda
