@@ -164,8 +164,12 @@ struct SetUpUnderCapture {
     ~SetUpUnderCapture() { (void)cudaThreadExchangeStreamCaptureMode(&mode); }
 };
 
-// Every pointer has to be memory that kernels of the current device can use: a pointer of another device, or plain host memory, would fault in the kernel.
+// Every pointer has to be memory that kernels of the current device can use: a pointer of another device, or plain host memory, would fault in the kernel, and so would one
+// that is not on a 4-byte boundary.
 int32_t check_device(const char * what, std::initializer_list<const void *> pointers) {
+    for (const void * p : pointers) {
+        if (reinterpret_cast<uintptr_t>(p) & 3u) return fail(DOOMS_INVALID_ARGUMENT, std::string(what) + ": a pointer is not on a boundary of 4 bytes");
+    }
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) { (void)cudaGetLastError(); return fail(DOOMS_UNSUPPORTED, std::string(what) + ": no CUDA device"); }
     for (const void * p : pointers) {
@@ -177,6 +181,12 @@ int32_t check_device(const char * what, std::initializer_list<const void *> poin
         if (!here) return fail(DOOMS_INVALID_ARGUMENT, std::string(what) + ": a pointer is not memory of the current device");
     }
     return DOOMS_OK;
+}
+
+// Whether two pieces of memory have a byte in common.
+bool overlap(const void * a, int64_t a_bytes, const void * b, int64_t b_bytes) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return x < y + uintptr_t(b_bytes) && y < x + uintptr_t(a_bytes);
 }
 
 bool aligned16(const void * p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -917,6 +927,9 @@ DOOMS_CUDA_API int32_t dooms_cuda_rope_store_paged(const dooms_cuda_paged_cache 
     if (!d_qkv || !d_sequence || !d_at || !d_positions || !d_q || n_rows < 0 || qkv_stride < row || qkv_stride % 4 != 0 || !aligned16(d_qkv) || !aligned16(d_q)) {
         return fail(DOOMS_INVALID_ARGUMENT, "rope_store_paged: a NULL or unaligned pointer, a negative n_rows, or a qkv_stride that is no multiple of 4 or shorter than a row");
     }
+    if (overlap(d_q, int64_t(n_rows) * n_head * c.head_dim * (q_dtype == DOOMS_F16 ? 2 : 4), d_qkv, ((int64_t(n_rows) - 1) * qkv_stride + row) * 4)) {
+        return fail(DOOMS_INVALID_ARGUMENT, "rope_store_paged: d_q overlaps d_qkv");
+    }
     const SetUpUnderCapture relaxed;
     code = check_device("rope_store_paged", {c.keys, c.values, c.page_table, d_qkv, d_sequence, d_at, d_positions, d_q});
     if (code != DOOMS_OK) return code;
@@ -941,7 +954,11 @@ DOOMS_CUDA_API int32_t dooms_cuda_attention_paged(const dooms_cuda_paged_cache *
         !(scale >= 0.f) || !(scale < 1e30f)) {
         return fail(DOOMS_INVALID_ARGUMENT, "attention_paged: a NULL or unaligned pointer, a negative size, or a scale that is negative or not finite");
     }
-    if (scratch_bytes < dooms_cuda_attention_paged_scratch_bytes(n_head, c.n_head_kv, c.head_dim)) return fail(DOOMS_RESOURCE_EXHAUSTED, "attention_paged: the scratch is too small");
+    const int64_t needed = dooms_cuda_attention_paged_scratch_bytes(n_head, c.n_head_kv, c.head_dim), io = int64_t(n_rows) * n_head * c.head_dim * (dtype == DOOMS_F16 ? 2 : 4);
+    if (scratch_bytes < needed) return fail(DOOMS_RESOURCE_EXHAUSTED, "attention_paged: the scratch is too small");
+    if (overlap(d_q, io, d_out, io) || overlap(d_scratch, needed, d_q, io) || overlap(d_scratch, needed, d_out, io)) {
+        return fail(DOOMS_INVALID_ARGUMENT, "attention_paged: d_q, d_out and d_scratch may not overlap");
+    }
     const SetUpUnderCapture relaxed;
     code = check_device("attention_paged", {c.keys, c.values, c.page_table, d_q, d_sequence, d_lengths, d_out, d_scratch});
     if (code != DOOMS_OK) return code;
@@ -957,11 +974,15 @@ DOOMS_CUDA_API int32_t dooms_cuda_attention_prompt_paged(const dooms_cuda_paged_
     int32_t code = check_paged("attention_prompt_paged", cache, n_head, &c);
     if (code != DOOMS_OK) return code;
     if (n_rows == 0 || n_prompts == 0) return DOOMS_OK;
-    if (!d_q || !d_sequence || !d_start || !d_lengths || !d_out || !d_scratch || d_q == d_out || n_rows < 0 || n_prompts < 0 || !aligned16(d_q) || !aligned16(d_out) ||
+    if (!d_q || !d_sequence || !d_start || !d_lengths || !d_out || !d_scratch || n_rows < 0 || n_prompts < 0 || !aligned16(d_q) || !aligned16(d_out) ||
         !aligned16(d_scratch) || !(scale >= 0.f) || !(scale < 1e30f)) {
-        return fail(DOOMS_INVALID_ARGUMENT, "attention_prompt_paged: a NULL or unaligned pointer, one buffer as input and output, a negative size, or a scale that is negative or not finite");
+        return fail(DOOMS_INVALID_ARGUMENT, "attention_prompt_paged: a NULL or unaligned pointer, a negative size, or a scale that is negative or not finite");
     }
-    if (scratch_bytes < dooms_cuda_attention_paged_scratch_bytes(n_head, c.n_head_kv, c.head_dim)) return fail(DOOMS_RESOURCE_EXHAUSTED, "attention_prompt_paged: the scratch is too small");
+    const int64_t needed = dooms_cuda_attention_paged_scratch_bytes(n_head, c.n_head_kv, c.head_dim), io = int64_t(n_rows) * n_head * c.head_dim * 2;
+    if (scratch_bytes < needed) return fail(DOOMS_RESOURCE_EXHAUSTED, "attention_prompt_paged: the scratch is too small");
+    if (overlap(d_q, io, d_out, io) || overlap(d_scratch, needed, d_q, io) || overlap(d_scratch, needed, d_out, io)) {
+        return fail(DOOMS_INVALID_ARGUMENT, "attention_prompt_paged: d_q, d_out and d_scratch may not overlap");
+    }
     const SetUpUnderCapture relaxed;
     code = check_device("attention_prompt_paged", {c.keys, c.values, c.page_table, d_q, d_sequence, d_start, d_lengths, d_out, d_scratch});
     if (code != DOOMS_OK) return code;

@@ -1,5 +1,6 @@
 """Python face of the operators of a serving step over a key / value cache in pages (include/dooms_cuda.h: dooms_cuda_paged_cache): rotary positions with the cache
-write, attention of single tokens and of packed prompts over the pages, and sampling. Tensors are device tensors (torch's); outputs are written in place and nothing is allocated. `stream` is a cudaStream_t as an integer (0: the default stream)."""
+write, attention of single tokens and of packed prompts over the pages, and sampling. Tensors are device tensors (torch's); outputs are written in place and nothing is
+allocated. `stream` is a cudaStream_t as an integer (0: the default stream)."""
 from __future__ import annotations
 
 import ctypes as C
@@ -25,6 +26,13 @@ def _dtype(name: str, t) -> int:
     if dt is None:
         raise L.DoomsError(L.UNSUPPORTED, f"{name}: float32 or float16 expected, got {t.dtype}")
     return dt
+
+
+def _scratch(t) -> tuple[int, int]:
+    """The scratch tensor's address and bytes."""
+    if not t.is_contiguous():
+        raise L.DoomsError(L.INVALID_ARGUMENT, "scratch: expected a contiguous tensor")
+    return t.data_ptr(), t.numel() * t.element_size()
 
 
 class PagedCache:
@@ -73,7 +81,7 @@ class PagedCache:
         shape = (n, n_head, self._c.head_dim)
         L.check(L.lib().dooms_cuda_attention_paged(self._ref, _dtype("q", q), _pointer("q", q, q.dtype, shape), _pointer("sequence", sequence, _I32, (n,)),
                                                    _pointer("lengths", lengths, _I32, (n,)), max_length, _pointer("out", out, q.dtype, shape), n_head, n, scale,
-                                                   scratch.data_ptr(), scratch.numel() * scratch.element_size(), stream))
+                                                   *_scratch(scratch), stream))
 
     def attention_prompt(self, q, sequence, start, lengths, out, scratch, scale: float = 0.0, stream: int = 0) -> None:
         """Packed prompts, causal: q, out f16 [rows][n_head][head_dim]; prompt i has rows start[i] .. start[i + 1] - 1, the last of lengths[i] positions of sequence[i]."""
@@ -81,8 +89,7 @@ class PagedCache:
         shape, n = (rows, n_head, self._c.head_dim), sequence.shape[0]
         L.check(L.lib().dooms_cuda_attention_prompt_paged(self._ref, _pointer("q", q, _F16, shape), _pointer("sequence", sequence, _I32, (n,)),
                                                           _pointer("start", start, _I32, (n + 1,)), _pointer("lengths", lengths, _I32, (n,)),
-                                                          _pointer("out", out, _F16, shape), n_head, n, rows, scale, scratch.data_ptr(),
-                                                          scratch.numel() * scratch.element_size(), stream))
+                                                          _pointer("out", out, _F16, shape), n_head, n, rows, scale, *_scratch(scratch), stream))
 
 
 def sample_rows(logits, uniform, tokens, probability=None, temperature=None, top_k=None, top_p=None, min_p=None, stream: int = 0) -> None:

@@ -276,11 +276,12 @@ typedef struct dooms_cuda_rope {
 DOOMS_CUDA_API int32_t dooms_cuda_rope_store_paged(const dooms_cuda_paged_cache * cache, const dooms_cuda_rope * rope, const float * d_qkv, int64_t qkv_stride, int32_t n_head,
                                                    int32_t n_rows, const int32_t * d_sequence, const int32_t * d_at, const int32_t * d_positions, int32_t q_dtype, void * d_q,
                                                    void * stream);
-/* Bytes of scratch memory (16-byte aligned) that attention_paged and attention_prompt_paged work in, for any number of rows; 0: bad arguments. */
+/* Bytes of scratch memory (16-byte aligned) that attention_paged and attention_prompt_paged work in, for any number of rows; 0: bad arguments. What it holds before a call
+ * does not matter; calls (and captured graphs) that can run at the same time need one each, calls one after another may share it. */
 DOOMS_CUDA_API int64_t dooms_cuda_attention_paged_scratch_bytes(int32_t n_head, int32_t n_head_kv, int32_t head_dim);
 /* attention_split + attention_combine (llama_kernels.h:860-929) for one new token of each of many sequences: row r of d_q [n_rows][n_head][head_dim] (turned) attends to
  * the first d_lengths[r] positions of sequence d_sequence[r] (negative: an idle row, whose output is left as it is; length 0: zeros). d_q and d_out: dtype DOOMS_F32 or
- * DOOMS_F16, 16-byte aligned; with f32 the products are as exact as f32 arithmetic. max_length: at least every length (a longer one is out of range); it may be generous.
+ * DOOMS_F16, 16-byte aligned, apart from one another and from the scratch; with f32 the products are as exact as f32 arithmetic. max_length: at least every length (a longer one is out of range); it may be generous.
  * scale: of the scores; 0: 1 / sqrt(head_dim). */
 DOOMS_CUDA_API int32_t dooms_cuda_attention_paged(const dooms_cuda_paged_cache * cache, int32_t dtype, const void * d_q, const int32_t * d_sequence, const int32_t * d_lengths,
                                                   int32_t max_length, void * d_out, int32_t n_head, int32_t n_rows, float scale, void * d_scratch, int64_t scratch_bytes,
@@ -288,7 +289,7 @@ DOOMS_CUDA_API int32_t dooms_cuda_attention_paged(const dooms_cuda_paged_cache *
 /* attention_prefill<64 / 128> (llama_kernels.h:640-769) for the packed prompts of many sequences: d_q [n_rows][n_head][head_dim] f16; prompt i has rows d_start[i] to
  * d_start[i + 1] - 1 (d_start: int32 [n_prompts + 1], not descending, d_start[0] >= 0, d_start[n_prompts] <= n_rows), which are the last positions of the d_lengths[i]
  * that sequence d_sequence[i] (negative: an idle prompt) has: a prompt may go on behind what is cached, and its own keys and values are in the cache already. A row
- * sees the positions up to its own; one that sees none (a prompt longer than its length) gives zeros. d_out [n_rows][n_head][head_dim] f16, apart from d_q; rows of no
+ * sees the positions up to its own; one that sees none (a prompt longer than its length) gives zeros. d_out [n_rows][n_head][head_dim] f16, apart from d_q and the scratch; rows of no
  * prompt are left as they are. Queries and probabilities enter the products as f16, as in the reference's tiles (:660, 708-713). */
 DOOMS_CUDA_API int32_t dooms_cuda_attention_prompt_paged(const dooms_cuda_paged_cache * cache, const void * d_q, const int32_t * d_sequence, const int32_t * d_start,
                                                          const int32_t * d_lengths, void * d_out, int32_t n_head, int32_t n_prompts, int32_t n_rows, float scale,

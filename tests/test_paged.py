@@ -117,6 +117,33 @@ def test_the_python_face_refuses_other_tensors():
         paged.sample_rows(torch.zeros(3, 8, dtype=torch.float16), torch.zeros(3), ids)
 
 
+def test_overlapping_and_unaligned_memory_is_refused():
+    """Blocks read their inputs while others write: what is written may not overlap what is read. An int32 or float off its boundary would fault in the kernel."""
+    c, rope, big = fake_cache(), fake_rope(), 1 << 32
+    for q, out, scratch in ((16, 16, big), (16, 32, big), (big + 2 * 4 * 64 * 4 - 16, big, 16), (big, 2 * big, big), (2 * big, big + 4096, big)):
+        assert attention_code(c, q=q, out=out, scratch=scratch) == L.INVALID_ARGUMENT, (q, out, scratch)
+        assert b"overlap" in L.lib().dooms_cuda_last_error()
+    for q, out, scratch in ((16, 16, big), (big + 5 * 4 * 64 * 2 - 16, big, 16), (big, 2 * big, big), (2 * big, big + 4096, big)):
+        assert prompt_code(c, q=q, out=out, scratch=scratch) == L.INVALID_ARGUMENT, (q, out, scratch)
+        assert b"overlap" in L.lib().dooms_cuda_last_error()
+    for qkv, q in ((16, 16), (big, big + (512 + 8 * 64) * 4 - 16), (big + 2 * 4 * 64 * 4 - 16, big)):
+        assert store_code(c, rope, qkv=qkv, q=q) == L.INVALID_ARGUMENT, (qkv, q)
+        assert b"overlap" in L.lib().dooms_cuda_last_error()
+    for code in (store_code(c, rope, q=1 << 20, at=18), attention_code(c, q=big, out=2 * big, seq=17), attention_code(fake_cache(page_table=4097), q=big, out=2 * big),
+                 prompt_code(c, q=big, out=2 * big, start=22), sample_code(logits=18), sample_code(tokens=17), sample_code(t=33)):
+        assert code == L.INVALID_ARGUMENT and b"4 bytes" in L.lib().dooms_cuda_last_error()
+
+
+def test_the_python_face_refuses_a_scratch_with_gaps():
+    keys = torch.zeros(4, 16, 2, 64, dtype=torch.float16)
+    cache, ids, q = paged.PagedCache(keys, keys.clone(), torch.zeros(2, 2, dtype=torch.int32)), torch.zeros(3, dtype=torch.int32), torch.zeros(3, 4, 64)
+    for scratch in (torch.zeros(1).expand(1 << 24), torch.zeros(1 << 22, 2)[:, 0]):
+        with pytest.raises(L.DoomsError, match="scratch"):
+            cache.attention(q, ids, ids, 5, q.clone(), scratch)
+        with pytest.raises(L.DoomsError, match="scratch"):
+            cache.attention_prompt(q.half(), ids, torch.zeros(4, dtype=torch.int32), ids, q.half(), scratch)
+
+
 # ---------------------------------------------------------------- plain forms in 64 bits
 
 def status():
