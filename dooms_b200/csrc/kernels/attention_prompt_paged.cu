@@ -42,6 +42,7 @@ constexpr float kLift = 6.f;                // probabilities are kept times 2^kL
 
 struct Args {
     PagedView c;
+    const __half * q;
     __half * out;
     int n_head, group, tile_queries, n_prompts, n_rows;      // tile_queries: queries per tile
     const int32_t * sequence, * start, * lengths;
@@ -225,9 +226,55 @@ __device__ __forceinline__ void join(const Args & a, int b0, int b1, int rows0, 
     }
 }
 
+// Outputs of rows that a value they do not see has spoilt: positions of a unit's later queries lie in the same tiles, and their probability of zero times an infinity
+// or NaN is NaN. A warp's rows of one tile, of those in `rows` (a NaN among their outputs, of a finite sum); key0, key1: the segment's keys that the tile had. Such a row whose
+// unseen values are at fault is worked out once more, key by key over the segment, against the reference its sum stands for.
+struct Spoilt { uint32_t rows; int seq, kvh, q_row, row0, first, key0, key1, queries; };      // row0: the warp's first row; first: the position of the tile's first query
+// out: the tile's outputs, f16, times by; else part: the tile's part.
+template <int D>
+__device__ __noinline__ void mend_rows(const Args & a, const Spoilt w, float ref, float by, __half * out, float * part) {
+    constexpr int kMine = D / 32;
+    const int lane = threadIdx.x % 32;
+    auto line = [&](int key) { return max(a.c.row(w.seq, key), int64_t(0)) * a.c.n_kv + w.kvh; };
+    for (uint32_t rest = w.rows; rest; rest &= rest - 1) {
+        const int i = __ffs(rest) - 1, r = w.row0 + i, position = w.first + min(r / a.group, w.queries - 1);
+        bool odd = false;
+        for (int key = max(position + 1, w.key0); key < w.key1; key++) {
+            const __half * v = a.c.v + line(key) * D + lane * kMine;
+            for (int d = 0; d < kMine; d++) odd = odd || !(fabsf(__half2float(v[d])) <= 65504.f);
+        }
+        if (!__any_sync(0xffffffffu, odd)) continue;
+        const float minus = kLift - __shfl_sync(0xffffffffu, ref, i);
+        const __half * q = a.q + ((int64_t(w.q_row) + r / a.group) * a.n_head + w.kvh * a.group + r % a.group) * D;
+        float o[kMine] = {};
+        const int end = min(w.key1, position + 1);
+        for (int k0 = w.key0; k0 < end; k0 += 32) {
+            float p = 0.f;
+            if (k0 + lane < end) {
+                const __half * k = a.c.k + line(k0 + lane) * D;
+                float s = 0.f;
+                for (int d = 0; d < D; d++) s = fmaf(__half2float(q[d]), __half2float(k[d]), s);
+                p = __half2float(__float2half_rn(ex2(fmaf(s, a.scale_log2, minus))));      // (as the other rows' enter the products)
+            }
+            for (int j = 0; j < min(32, end - k0); j++) {
+                const float pj = __shfl_sync(0xffffffffu, p, j);
+                const __half * v = a.c.v + line(k0 + j) * D + lane * kMine;
+                for (int d = 0; d < kMine; d++) o[d] = fmaf(pj, __half2float(v[d]), o[d]);
+            }
+        }
+        const float by_row = __shfl_sync(0xffffffffu, by, i);
+        for (int d = 0; d < kMine; d++) {
+            const int c = lane * kMine + d;
+            if (out) out[(int64_t(r / a.group) * a.n_head + r % a.group) * D + c] = __float2half_rn(o[d] * by_row);
+            else part[((c / 4) * kRows + r) * 4 + c % 4] = o[d];
+        }
+    }
+    __syncwarp();
+}
+
 template <int D>
 __global__ void __launch_bounds__(kThreads, 1) k_attention_prompt(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
-                                                                  const __grid_constant__ CUtensorMap vmap, const Args a) {
+                                                                  const __grid_constant__ CUtensorMap vmap, const __grid_constant__ Args a) {
     constexpr int S = kRing<D>;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     const uint32_t q_at = (smem_u32(smem_raw) + 1023u) & ~1023u, k_at = q_at + 2 * kTileBytes<D>, v_at = k_at + S * kTileBytes<D>;
@@ -596,6 +643,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention_prompt(const __grid_c
                     tc_fence_after();
                 }
                 const bool whole = s.t0 == 0 && s.t1 == s.tiles;
+                uint64_t odd[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};      // the outputs' sum: NaN if one is
                 // 32 columns of the warp's 32 rows, from a thread per row: through shared memory, so that a store is eight rows of 64 bytes and not 32 pieces of 16
                 const int last = min(a.tile_queries, s.queries - x * a.tile_queries) * a.group;      // rows of the tile that are there
                 __half * const out = a.out + ((int64_t(s.row) + x * a.tile_queries) * a.n_head + u.kvh * a.group) * D;
@@ -617,6 +665,15 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention_prompt(const __grid_c
                     }
                     __syncwarp();
                 };
+                auto spoilt = [&](float sum) {
+                    float a0, a1;
+                    halves(add2(odd[0], odd[1]), a0, a1);
+                    a0 += a1;
+                    const uint32_t rows = __ballot_sync(0xffffffffu, a0 != a0 && sum - sum == 0.f && r < last);
+                    const int key0 = s.t0 * kRows;
+                    return Spoilt{rows, rows ? __ldg(a.sequence + u.prompt) : 0, u.kvh, s.row + x * a.tile_queries, (warp % 4) * 32, s.first + x * a.tile_queries, key0, min(s.keys, key0 + n * kRows),
+                                  s.queries - x * a.tile_queries};
+                };
                 if (whole) {
                     const float by = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
                     if (n > 0) {
@@ -627,12 +684,16 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention_prompt(const __grid_c
                             tc_wait_ld();
                             tie32(o);
                             #pragma unroll
+                            for (int i = 0; i < 32; i += 2) odd[i / 2 % 2] = add2(odd[i / 2 % 2], pair(__uint_as_float(o[i]), __uint_as_float(o[i + 1])));
+                            #pragma unroll
                             for (int i = 0; i < 32; i += 2) {
                                 const __half2 h = __floats2half2_rn(__uint_as_float(o[i]) * by, __uint_as_float(o[i + 1]) * by);
                                 o[i / 2] = *reinterpret_cast<const uint32_t *>(&h);
                             }
                             write_rows(o, c);
                         }
+                        const Spoilt w = spoilt(sum);
+                        if (w.rows) mend_rows<D>(a, w, ref, by, out, nullptr);
                     }
                 } else {
                     float * const part = a.part + ((int64_t(blockIdx.x) * 2 + (s.t0 == 0 ? 1 : 0)) * 2 + x) * kTilePart<D>;
@@ -644,10 +705,16 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention_prompt(const __grid_c
                             tc_wait_ld();
                             tie32(o);
                             #pragma unroll
+                            for (int i = 0; i < 32; i += 2) odd[i / 2 % 2] = add2(odd[i / 2 % 2], pair(__uint_as_float(o[i]), __uint_as_float(o[i + 1])));
+                            #pragma unroll
                             for (int i = 0; i < 8; i++) {
                                 reinterpret_cast<uint4 *>(part)[(c / 4 + i) * kRows + r] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
                             }
                         }
+                    }
+                    if (n > 0) {
+                        const Spoilt w = spoilt(sum);
+                        if (w.rows) mend_rows<D>(a, w, ref, 1.f, nullptr, part);
                     }
                     // (a tile without a step in this segment leaves no outputs, and a maximum that says so)
                     reinterpret_cast<float2 *>(part + kRows * D)[r] = make_float2(n > 0 && seen ? ref : -CUDART_INF_F, n > 0 ? sum : 0.f);
@@ -703,6 +770,7 @@ cudaError_t launch_attention_prompt_paged(const PagedCache & cache, const void *
                                           const int32_t * start, const int32_t * lengths, float scale, void * scratch, int * error, cudaStream_t stream) {
     Args a{};
     a.c = paged_view(cache, error);
+    a.q = static_cast<const __half *>(q);
     a.out = static_cast<__half *>(out);
     a.n_head = n_head; a.group = n_head / cache.n_head_kv; a.tile_queries = kRows / a.group; a.n_prompts = n_prompts; a.n_rows = n_rows;
     a.sequence = sequence; a.start = start; a.lengths = lengths;

@@ -525,6 +525,44 @@ def test_attention_of_prompts_scales_and_shared_sequences():
 
 
 @gpu
+@pytest.mark.parametrize("heads, head_dim, page", [((14, 2), 64, 16), ((8, 2), 128, 64), ((3, 3), 64, 256)])
+@pytest.mark.parametrize("what", [math.nan, math.inf, -math.inf])
+def test_attention_of_prompts_values_that_are_not_finite(heads, head_dim, page, what):
+    """Positions that are not finite are no concern of the rows in front of them, whole units or cut ones; of keys NaN and infinity, of values one column or all of them. A
+    row that sees such a value has it in its output: NaN, or the infinity (an infinite value's probability is far above zero here)."""
+    H, K = heads
+    new, cached = [90, 300, 33, 1], [30, 20000, 0, 128]
+    lengths = [a + b for a, b in zip(new, cached)]
+    for at, column in ((40, 5), (1, None), (85, head_dim - 1)):
+        cache = Cache(lengths, K, head_dim, page, seed=H)
+        spoilt = [lengths[i] - n + min(at, n - 1) for i, n in enumerate(new)]      # the position of each sequence
+        for i, j in enumerate(spoilt):
+            cache.rows(cache.host[1], i)[cache.line(i, lengths[i])[j], :, slice(None) if column is None else column] = what
+        cache.upload()
+        g = np.random.default_rng(at)
+        start = np.concatenate([[0], np.cumsum(new)])
+        q = g.standard_normal((start[-1], H, head_dim)).astype(np.float16)
+        out = torch.full(q.shape, 77.0, dtype=torch.float16, device="cuda")
+        cache.cache.attention_prompt(cuda(q), cuda(np.arange(4, dtype=np.int32)), cuda(start.astype(np.int32)), cuda(np.array(lengths, np.int32)), out, cache.scratch(H))
+        assert status() == (L.OK, 0)
+        got = out.cpu().numpy().astype(np.float64)
+        s = 1 / math.sqrt(head_dim)
+        for i, n in enumerate(new):
+            k, v = cache.sequence(i, lengths[i])
+            sane = np.where(np.isfinite(v), v, 0.0)
+            for j in sorted({0, min(1, n - 1), max(0, min(at, n - 1) - 1), min(at, n - 1), n - 1}):
+                seen = lengths[i] - n + j + 1
+                want, mass, reach = attend(q[start[i] + j].astype(np.float64), k[:seen], sane[:seen], s)
+                tol = bound(want, mass, reach, head_dim, s, True)
+                r = got[start[i] + j]
+                if seen > spoilt[i]:
+                    hit = np.s_[:, :] if column is None else np.s_[:, column]
+                    assert (np.isnan(r[hit]) if math.isnan(what) else ~np.isfinite(r[hit]) if cached[i] > 1000 else r[hit] == what).all(), (i, j)
+                    want[hit] = r[hit] = 0.0
+                assert (np.abs(r - want) <= tol).all(), (i, j, seen)
+
+
+@gpu
 def test_a_long_prompt_in_one_call_is_its_pieces():
     """2100 positions at once, and as pieces behind what is cached: the same rows up to the roundings of two results."""
     H, D, n = 10, 128, 2100
