@@ -528,8 +528,8 @@ def test_attention_of_prompts_scales_and_shared_sequences():
 @pytest.mark.parametrize("heads, head_dim, page", [((14, 2), 64, 16), ((8, 2), 128, 64), ((3, 3), 64, 256)])
 @pytest.mark.parametrize("what", [math.nan, math.inf, -math.inf])
 def test_attention_of_prompts_values_that_are_not_finite(heads, head_dim, page, what):
-    """Positions that are not finite are no concern of the rows in front of them, whole units or cut ones; of keys NaN and infinity, of values one column or all of them. A
-    row that sees such a value has it in its output: NaN, or the infinity (an infinite value's probability is far above zero here)."""
+    """Values that are not finite are no concern of the rows in front of their position, in whole units or cut ones, in one column or all of them. A row that sees such a value
+    has it in its output: NaN, or the infinity where its probability is far above zero."""
     H, K = heads
     new, cached = [90, 300, 33, 1], [30, 20000, 0, 128]
     lengths = [a + b for a, b in zip(new, cached)]
@@ -779,6 +779,106 @@ def test_sampling_batches_of_mixed_rows(rows, n):
         tokens.fill_(-9)
         graph.replay()
     assert copy.tolist() == [chain(x[r], t[r], k[r], p[r], m[r], u[r])[0] for r in range(rows)]
+
+
+@gpu
+@pytest.mark.parametrize("offset", [1, 2, 3, 4])
+def test_sampling_rows_that_do_not_begin_on_16_bytes(offset):
+    g = np.random.default_rng(offset)
+    x = g.standard_normal((6, 5001)).astype(np.float32) * 3
+    flat = torch.full((offset + 6 * 5003,), math.inf, device="cuda")
+    rows = flat[offset:].view(6, 5003)[:, :5001]
+    rows.copy_(cuda(x))
+    t, k, p, m, u = (np.array(a) for a in zip(*[FILTERS[n] + (g.uniform(),) for n in ("chat", "open", "nucleus", "wide", "min_p", "greedy")]))
+    tokens = torch.full((6,), -9, dtype=torch.int32, device="cuda")
+    paged.sample_rows(rows, cuda(u, torch.float32), tokens, None, cuda(t, torch.float32), cuda(k, torch.int32), cuda(p, torch.float32), cuda(m, torch.float32))
+    assert tokens.tolist() == [chain(x[r], t[r], int(k[r]), p[r], m[r], u[r])[0] for r in range(6)]
+
+
+# ---------------------------------------------------------------- large pools, many rows, calls at once
+
+@gpu
+def test_positions_of_a_pool_beyond_32_bits():
+    """Pools of more than 2^32 bytes and 2^31 values, in the largest pages: rows written and read at their end are those that were meant."""
+    H, K, D, page, n = 8, 8, 128, 65536, 65600
+    pages = (1 << 31) // (K * D * page) + 3                  # 2^31 values and three pages
+    keys, values = (torch.empty(pages, page, K, D, dtype=torch.float16, device="cuda") for _ in range(2))
+    cache = paged.PagedCache(keys, values, torch.tensor([[pages - 1, pages - 2], [0, 1]], dtype=torch.int32, device="cuda"))
+    small = Cache([n], K, D, 4096, seed=3)                   # the same sequence in small pages
+    line = torch.from_numpy(small.line(0, n)).cuda()
+    for mine, other in ((keys, small.keys), (values, small.values)):
+        mine[pages - 1] = other.view(-1, K, D)[line[:page]]
+        mine[pages - 2, :n - page] = other.view(-1, K, D)[line[page:]]
+        mine[0].zero_()
+    scratch = small.scratch(H)
+    new, ids = 3, torch.zeros(3, dtype=torch.int32, device="cuda")
+    qkv = torch.randn(new, (H + 2 * K) * D, device="cuda")
+    at = torch.tensor([n - 1, n - 2, n - 3], dtype=torch.int32, device="cuda")
+    outs = []
+    for c in (cache, small.cache):
+        q = torch.empty(new, H, D, device="cuda")
+        c.rope_store(qkv, ids, at, at[None], q, base=1e6, neox=True)
+        one, some = torch.zeros_like(q), torch.zeros(new, H, D, dtype=torch.float16, device="cuda")
+        c.attention(q, ids, at + 1, n, one, scratch)
+        c.attention_prompt(q.half(), ids[:1], torch.tensor([0, new], dtype=torch.int32, device="cuda"), at[:1] + 1, some, scratch)
+        outs.append((q, one, some))
+    assert status() == (L.OK, 0)
+    for a, b in zip(*outs):
+        assert torch.equal(a, b)
+    assert (keys[0] == 0).all() and (keys[pages - 2, n - page - 3:n - page] == small.keys.view(-1, K, D)[line[n - 3:]]).all()
+
+
+@gpu
+def test_more_rows_than_threads():
+    """Batches of thousands of short sequences."""
+    lengths = [1 + i % 3 for i in range(2500)]
+    cache = Cache(lengths, 1, 64, 16, seed=8)
+    check_decode(cache, lengths, 2, torch.float16, idle=range(0, 2500, 7))
+    check_prompt(cache, [i % 2 for i in range(2500)], lengths, 2, idle=range(0, 2500, 7))
+
+
+@gpu
+def test_calls_at_once_on_two_streams():
+    """Every operator on two streams at the same time, each with its own scratch and outputs: what each gives is what it gives alone."""
+    H, K, D, V = 16, 4, 128, 30000
+    g = np.random.default_rng(12)
+
+    def side(seed):
+        lengths = [5000, 17, 900, 64]
+        cache = Cache([n + 1 for n in lengths], K, D, 16, seed=seed)
+        stream, scratch = torch.cuda.Stream(), cache.scratch(H)
+        seq, at = torch.arange(4, dtype=torch.int32, device="cuda"), cuda(np.array(lengths, np.int32))
+        qkv, logits, u = torch.randn(4, (H + 2 * K) * D, device="cuda"), torch.randn(64, V, device="cuda") * 2, torch.rand(64, device="cuda")
+        top_k = cuda(g.choice([0, 40], 64), torch.int32)
+        pq, start = torch.randn(2400, H, D, device="cuda").half(), cuda(np.array([0, 900, 910, 1100, 1164], np.int32))
+
+        def run():
+            q, out, pout = torch.empty(4, H, D, device="cuda"), torch.zeros(4, H, D, device="cuda"), torch.zeros_like(pq)
+            tokens, prob = torch.zeros(64, dtype=torch.int32, device="cuda"), torch.zeros(64, device="cuda")
+            s = stream.cuda_stream
+            cache.cache.rope_store(qkv, seq, at, at[None], q, base=1e4, neox=True, stream=s)
+            cache.cache.attention(q, seq, at + 1, 5001, out, scratch, stream=s)
+            cache.cache.attention_prompt(pq, seq, start, at + 1, pout, scratch, stream=s)
+            paged.sample_rows(logits, u, tokens, prob, top_k=top_k, stream=s)
+            return q, out, pout, tokens, prob
+        return stream, run
+    sides = [side(1), side(2)]
+    torch.cuda.synchronize()
+    alone = []
+    for stream, run in sides:
+        with torch.cuda.stream(stream):
+            alone.append(run())
+        torch.cuda.synchronize()
+    results = [[], []]
+    for _ in range(10):
+        for i, (stream, run) in enumerate(sides):
+            with torch.cuda.stream(stream):
+                results[i].append(run())
+    torch.cuda.synchronize()
+    assert status() == (L.OK, 0)
+    for i in range(2):
+        for result in results[i]:
+            assert all(torch.equal(a, b) for a, b in zip(result, alone[i]))
 
 
 # ---------------------------------------------------------------- together
