@@ -38,6 +38,7 @@ constexpr int kFar = 240;              // the bin of everything from 10 nats bel
 constexpr int kPowers = 256;
 constexpr int kNearMost = 8192, kPerWarp = kNearMost / (kThreads / 32);      // logits a block lists, and each of its warps
 constexpr int kSamples = 8;            // logits per thread that say how far down a list goes
+constexpr int kTurns = 4;              // passes over what is below the list before it is a histogram's
 constexpr double kNoLimit = 1e300;     // (gaps are below 2^129, or infinite)
 static_assert(kList == kThreads && kBins <= kThreads, "one list element and at most one bin per thread");
 
@@ -166,6 +167,38 @@ __device__ __forceinline__ void each(const Row & r, F f) {
     }
     for (; i < quads; i += kThreads) four(i + lane < quads ? __ldg(x4 + i + lane) : make_float4(none, none, none, none), i + lane);
     if (warp == 0 && 4 * quads < r.here) f(4 * quads + lane < r.here ? r.x[4 * quads + lane] : none, 4 * quads + lane);
+}
+
+// The same four at a time: f(values, place of the first).
+template <int kAhead, class F>
+__device__ __forceinline__ void each_four(const Row & r, F f) {
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const float none = __int_as_float(0x7fffffff);
+    if (!r.wide) {
+        for (int i = warp * 32; i < r.here; i += kThreads) {
+            const float v[4] = {i + lane < r.here ? r.x[i + lane] : none, none, none, none};
+            f(v, i + lane);
+        }
+        return;
+    }
+    const int quads = (r.here + 3) / 4;
+    const float4 * x4 = reinterpret_cast<const float4 *>(r.x);
+    for (int i = warp * 32; i < quads; i += kAhead * kThreads) {
+        float v[kAhead][4];
+        #pragma unroll
+        for (int j = 0; j < kAhead; j++) {
+            const int q = i + lane + j * kThreads;
+            if (4 * q + 3 < r.here) {
+                const float4 w = __ldg(x4 + q);
+                v[j][0] = w.x; v[j][1] = w.y; v[j][2] = w.z; v[j][3] = w.w;
+            } else {
+                #pragma unroll
+                for (int k = 0; k < 4; k++) v[j][k] = 4 * q + k < r.here ? r.x[4 * q + k] : none;
+            }
+        }
+        #pragma unroll
+        for (int j = 0; j < kAhead; j++) f(v[j], 4 * (i + lane + j * kThreads));
+    }
 }
 
 // Inclusive sums over the block of a value per thread; *total: of all.
@@ -393,9 +426,9 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const SampleArgs a)
     const float t = a.temperature ? a.temperature[row] : 1.f, top_p = a.top_p ? a.top_p[row] : 1.f, min_p = a.min_p ? a.min_p[row] : 0.f, uniform = a.uniform[row];
     const int k = a.top_k ? a.top_k[row] : 0;
     const bool greedy = !(t > 0.f), by_k = k > 0 && k < a.n, by_p = top_p < 1.f, by_m = min_p > 0.f;
-    // open: a total of everything is needed. What is listed there is what lies above the least of the warps' m-th largest of the threads' largest of kSamples logits each: a
-    // share of the row that does not depend on what its logits are like.
-    const bool open = !greedy && !by_k && (by_p || !by_m), bounded = open || (by_k && k <= kThreads && !greedy);
+    // open: a total of everything is needed. sampled: what is listed there, and for a top-k of more than there are threads, is what lies above the least of the warps' m-th
+    // largest of the threads' largest of kSamples logits each: a share of the row that does not depend on what its logits are like.
+    const bool open = !greedy && !by_k && (by_p || !by_m), sampled = open || (!greedy && by_k && k > kThreads), bounded = !greedy && (open || by_k);
     // (rows of the other launch: their clusters leave at once)
     if (a.rows_of != kAllRows && open != (a.rows_of == kOpenRows)) { if (a.rows_of == kOpenRows) pdl_wait(); return; }
     if (threadIdx.x < kPowers) s.power[threadIdx.x] = exp2(double(threadIdx.x) * (-1.0 / kPowers));
@@ -406,7 +439,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const SampleArgs a)
     float mine = -CUDART_INF_F, sample = -CUDART_INF_F;
     uint32_t mine_at = 0xffffffffu;
     if (greedy) each<8>(r, [&](float v, int i) { if (v > mine) { mine = v; mine_at = uint32_t(first + i); } });      // (a NaN loses, and the first of equal ones wins)
-    else if (!open) each<8>(r, [&](float v, int) { mine = fmaxf(mine, v); });
+    else if (!sampled) each<8>(r, [&](float v, int) { mine = fmaxf(mine, v); });
     else each<8>(r, [&](float v, int i) {
         mine = fmaxf(mine, v);
         if (i % 4 == 0 && (i / (4 * kThreads) & (a.sample_every - 1)) == 0) sample = fmaxf(sample, v);
@@ -417,7 +450,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const SampleArgs a)
     // A bound for a top-k: if every warp has m = k / 16 (rounded up) threads with a logit of at least b, the row has k of them. b: the least of the warps' m-th largest.
     float bound = -CUDART_INF_F;
     if (bounded) {
-        float v = open ? sample : mine;      // sorted over the lanes, largest first
+        float v = sampled ? sample : mine;      // sorted over the lanes, largest first
         #pragma unroll
         for (int size = 2; size <= 32; size *= 2) {
             #pragma unroll
@@ -427,7 +460,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const SampleArgs a)
                 v = larger_first ? fmaxf(v, o) : fminf(v, o);
             }
         }
-        bound = __shfl_sync(0xffffffffu, v, open ? a.sample_rank - 1 : (k + kThreads / 32 - 1) / (kThreads / 32) - 1);
+        bound = __shfl_sync(0xffffffffu, v, sampled ? a.sample_rank - 1 : (k + kThreads / 32 - 1) / (kThreads / 32) - 1);
     }
     float2 * const tops = reinterpret_cast<float2 *>(s.warp_sum);
     if (lane == 0) tops[warp] = make_float2(top, bound);
@@ -516,14 +549,14 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const SampleArgs a)
         // ---- a top-k's bound, or a min-p alone, says at once what to look at ----
         const bool alone = least > -CUDART_INF_F && !by_k && !by_p;
         const float near = alone ? least : fmaxf(bound, -3.402823466e38f);
-        if (alone || (by_k && bounded)) {
+        if (alone || by_k) {
             list_begin();
             each<4>(r, [&](float v, int i) { append(v >= near, v, i); });
             list_end();
             cluster_barrier();
             const uint32_t n_near = of_blocks(&s.n_near, blocks, 0u, [](uint32_t v) { return __reduce_add_sync(0xffffffffu, v); });
-            if (fits()) use_list();
-            if (n_near <= kList) {
+            if (fits() && (!sampled || n_near >= uint32_t(k))) use_list();      // (sampled: a top-k's, and not sure to hold it)
+            if (n_near <= kList && !sampled) {
                 n = gather(r, [](float v, int) { return v == v; });
                 listed = true;
             }
@@ -541,54 +574,87 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const SampleArgs a)
         auto divide = [&](bool by_count, double per, auto goal) {
             where = 0;
             if (!r.at && !by_count) {
-                const float nat = float(kLog2e / per), down1 = near - 0.7f * nat, down2 = near - 1.6f * nat;
-                unsigned long long rest[3] = {0, 0, 0};       // the weights below near, down1, down2
-                list_begin();
-                if (threadIdx.x < 3) s.rest[threadIdx.x] = 0;
-                each<2>(r, [&](float v, int i) {
-                    const bool kept = r.kept(v, i);
-                    const unsigned long long w = r.weight_of(kept ? (r.top64 - double(v)) * per : 64.0);
-                    rest[0] += v < near ? w : 0ull;
-                    rest[1] += v < down1 ? w : 0ull;
-                    rest[2] += v < down2 ? w : 0ull;
-                    append(kept && v >= near, v, i);
-                });
-                __syncthreads();
-                #pragma unroll
-                for (int j = 0; j < 3; j++) {
+                const float nat = float(kLog2e / per);
+                unsigned long long all = 0, g = 0, below = 0;       // below: the weights below `from`
+                float from = near;
+                for (int turn = 0; turn < kTurns; turn++) {
+                    // the weights below three ends; in the first turn what is above the first is listed
+                    const float width = turn ? 0.9f * nat : 0.8f * nat, end[3] = {turn ? from - width : from, turn ? from - 2.f * width : from - width, turn ? from - 3.f * width : from - 2.f * width};
+                    unsigned long long rest[3] = {0, 0, 0};
+                    list_begin();
+                    if (threadIdx.x < 3) s.rest[threadIdx.x] = 0;
+                    each_four<2>(r, [&](const float (&v)[4], int i) {
+                        bool kept[4];
+                        unsigned long long w[4];
+                        #pragma unroll
+                        for (int j = 0; j < 4; j++) {
+                            kept[j] = r.kept(v[j], i + j);
+                            w[j] = r.weight_of(kept[j] ? (r.top64 - double(v[j])) * per : 64.0);
+                        }
+                        #pragma unroll
+                        for (int j = 0; j < 4; j++) {
+                            #pragma unroll
+                            for (int e = 0; e < 3; e++) rest[e] += v[j] < end[e] ? w[j] : 0ull;
+                        }
+                        if (turn == 0) {
+                            #pragma unroll
+                            for (int j = 0; j < 4; j++) append(kept[j] && v[j] >= near, v[j], i + j);
+                        }
+                    });
+                    __syncthreads();
                     #pragma unroll
-                    for (int d = 16; d; d >>= 1) rest[j] += __shfl_xor_sync(0xffffffffu, rest[j], d);
-                    if (lane == 0) atomicAdd(&s.rest[j], rest[j]);
-                }
-                list_end();
-                cluster_barrier();
-                #pragma unroll
-                for (int j = 0; j < 3; j++) {
-                    rest[j] = lane < int(blocks) ? ld_remote(&s.rest[j], lane) : 0ull;
+                    for (int e = 0; e < 3; e++) {
+                        #pragma unroll
+                        for (int d = 16; d; d >>= 1) rest[e] += __shfl_xor_sync(0xffffffffu, rest[e], d);
+                        if (lane == 0) atomicAdd(&s.rest[e], rest[e]);
+                    }
+                    list_end();
+                    cluster_barrier();
                     #pragma unroll
-                    for (int d = kMostBlocks / 2; d; d >>= 1) rest[j] += __shfl_xor_sync(0xffffffffu, rest[j], d);
-                    rest[j] = __shfl_sync(0xffffffffu, rest[j], 0);
-                }
-                if (fits()) {
-                    use_list();
-                    histogram<false>(r, false, per, 0, rest[0], every, from_top, goal);
-                    if (s.bin < kBins) return;
-                    const unsigned long long all = s.total, g = goal(all);
-                    use_share();
-                    if (g <= all - rest[2]) {
-                        const bool second = g > all - rest[1];
+                    for (int e = 0; e < 3; e++) {
+                        rest[e] = lane < int(blocks) ? ld_remote(&s.rest[e], lane) : 0ull;
+                        #pragma unroll
+                        for (int d = kMostBlocks / 2; d; d >>= 1) rest[e] += __shfl_xor_sync(0xffffffffu, rest[e], d);
+                        rest[e] = __shfl_sync(0xffffffffu, rest[e], 0);
+                    }
+                    if (turn == 0) {
+                        if (!fits()) break;
+                        use_list();
+                        histogram<false>(r, false, per, 0, rest[0], every, from_top, goal);
+                        if (s.bin < kBins) return;
+                        all = s.total;
+                        g = goal(all);
+                        use_share();
+                        below = rest[0];
+                    }
+                    // the step, from `from` down to an end, that the goal falls in
+                    unsigned long long below_end = below;
+                    step_end = from;
+                    bool found = false;
+                    #pragma unroll
+                    for (int e = 0; e < 3; e++) {
+                        if (!found) {
+                            below = below_end;
+                            from = step_end;
+                            step_end = end[e];
+                            below_end = rest[e];
+                            found = g <= all - below_end;
+                        }
+                    }
+                    if (found) {
                         where = 2;
-                        step_top = second ? down1 : near;
-                        step_end = second ? down2 : down1;
+                        step_top = from;
                         step_scale = float(kBins) / (step_top - step_end);
                         list_begin();
                         each<4>(r, [&](float v, int i) { append(v < step_top && v >= step_end && r.kept(v, i), v, i); });
                         list_end();
                         cluster_barrier();
                         if (fits()) use_list();
-                        histogram<false>(r, false, per, second ? all - rest[1] : all - rest[0], second ? rest[2] : rest[1], [&](float v) { return v < step_top && v >= step_end; }, step_bin, goal);
+                        histogram<false>(r, false, per, all - below, below_end, [&](float v) { return v < step_top && v >= step_end; }, step_bin, goal);
                         return;
                     }
+                    from = step_end;
+                    below = below_end;
                 }
             }
             if (r.at) {
