@@ -22,14 +22,14 @@ constexpr int kThreads = 256, kAtOnce = 4;      // kAtOnce: units of a thread wh
 
 struct RopeArgs {
     double turns[64];                   // base^(-2 i / d) / (2 pi): turns per position
-    int neox, n_axes, axis_end[4];      // axis x has the pairs [axis_end[x - 1], axis_end[x])
+    int n_axes, axis_end[4];            // axis x has the pairs [axis_end[x - 1], axis_end[x])
 };
 
 __device__ __forceinline__ uint32_t pack(float a, float b) { const __half2 h = __floats2half2_rn(a, b); return *reinterpret_cast<const uint32_t *>(&h); }
 
 // Bound by device memory, and close to being bound by instructions: a row has TPR threads, each of which has the same eight values (four pairs) of every head it takes, so
 // that its sines and cosines stay in registers and its addresses are a step apart. (With rows and heads dealt by division and the pairs chosen at run time a unit
-// was 325 instructions: 68 us for 6000 rows of 40 + 8 heads of 128 instead of what the table in the design notes has.) Every thread asks for its first units,
+// was 325 instructions: 68 us for 6000 rows of 40 + 8 + 8 heads of 128, where this takes 50; their bytes alone take 39.5.) Every thread asks for its first units,
 // then the block makes its rows' (cos, sin) in shared memory, one thread per pair, and looks the rows' places up, while those are on their way.
 template <int D, bool HALF_Q, bool NEOX, int TPR>
 __global__ void __launch_bounds__(kThreads, 4) k_rope_store_paged(const PagedView c, const __grid_constant__ RopeArgs r, const float * __restrict__ qkv, int64_t stride, int n_head,
@@ -148,7 +148,6 @@ cudaError_t launch_rope_store_paged(const PagedCache & cache, const RopeSections
         table.head_dim = cache.head_dim;
     }
     RopeArgs r = table.args;
-    r.neox = rope.neox;
     r.n_axes = rope.n_axes;
     for (int x = 0, end = 0; x < 4; x++) r.axis_end[x] = end += rope.sections[x];
     const int heads = n_head + 2 * cache.n_head_kv;

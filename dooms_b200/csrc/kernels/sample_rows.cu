@@ -10,7 +10,7 @@
 // an element costs a histogram some hundred instructions, a list two votes, and the sum of the weights that are in no list some fifty. Where at most kList
 // elements are left to look at, they are sorted and everything else is decided among them. A bin of more than kList elements is divided again by the bits of the
 // logits, down to a single value, whose elements are counted out in the order of their indices.
-// Bound by instructions where a total is needed (256 rows of 128256, B200: 231 us at no filter, 291 at a nucleus), else by latencies and memory (top-k 40: 60 us, the largest alone: 34 us of
+// Bound by instructions where a total is needed (256 rows of 128256, B200: 194 us at no filter, 304 at a nucleus), else by latencies and memory (top-k 40: 59 us, the largest alone: 34 us of
 // the 20 that reading the 131 MB takes).
 // Weights are 64-bit integers, e^-x 2^45 rounded (x and the exponential in 64-bit floating point): sums do not depend on the order of the atomics, and the blocks of
 // a cluster, which all work out every cut for themselves, agree on it. 2^18 logits of the largest weight still fit. What is rounded off is 2^-46 of
@@ -38,8 +38,7 @@ constexpr int kFar = 240;              // the bin of everything from 10 nats bel
 constexpr int kPowers = 256;
 constexpr int kNearMost = 8192, kPerWarp = kNearMost / (kThreads / 32);      // logits a block lists, and each of its warps
 constexpr int kSamples = 8;            // logits per thread that say how far down a list goes
-constexpr int kTurns = 4;              // passes over what is below the list before it is a histogram's
-constexpr double kNoLimit = 1e300;     // (gaps are below 2^129, or infinite)
+constexpr int kTurns = 4;              // passes that weigh steps before it is a histogram's: ten nats, at temperature 1, below the list
 static_assert(kList == kThreads && kBins <= kThreads, "one list element and at most one bin per thread");
 
 struct SampleArgs {
@@ -564,8 +563,9 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const SampleArgs a)
 
         // A cut over what is kept. Of a list: the histogram. Of the share, by count: the histogram, its far bin divided if the goal falls there; what is in front of the goal
         // becomes the list where it fits. Of the share, by weight: one pass without a branch adds up the weights below three steps down from the bound and lists what
-        // is above it; if the goal is in front of the end of one of the steps, that step is listed; if not (or if a list does not fit), the histogram of the share. Then
-        // the element.
+        // is above it; if the goal is in front of the end of one of the steps, that step is listed; if it is further down, the next three steps are weighed; where that ends
+        // (or the first list does not fit), the histogram of the share. (With that histogram for everything below the first steps a single row that drew from there kept
+        // 256 rows of a mix waiting: 246 us against 203.) Then the element.
         int where = 0;      // what the histogram was of: 0 bins from the largest logit down, 1 the far bin's, 2 a step's
         float step_top = 0.f, step_scale = 0.f, step_end = 0.f;
         auto step_bin = [&](float v) { return int(fminf((step_top - v) * step_scale, float(kBins - 1))); };
@@ -768,8 +768,8 @@ cudaError_t launch_sample_rows(const float * logits, int64_t stride, int rows, i
     const int all = blocks_for(4 * sm_count()), open = std::max(all, std::min(blocks_for(INT64_MAX), 4));
     if (all == open) return go(kAllRows, all);
     // Too many rows for four blocks each: those that a bound leaves little of get fewer, the others four, in two launches that overlap. Rows x logits, mix of filters /
-    // nucleus alone, with eight blocks for the open rows against four, in us: 256 x 32000 143 / 321 against 105 / 143, 256 x 128256 257 / 499 against 244 / 291,
-    // 128 x 151936 (four fit all rows, one launch) 178 / 267 against 178 / 194. One launch of two blocks for all 256 rows: 300 for the mix, of four: 95 for top-k 40 alone (two: 59).
+    // nucleus alone, with eight blocks for the open rows against four, in us: 256 x 32000 139 / 322 against 98 / 147, 256 x 128256 232 / 506 against 206 / 304,
+    // 128 x 151936 (four fit all rows, one launch) 151 / 275 against 128 / 203. Four for all 256 rows: 95 for top-k 40 alone, two: 59.
     e = go(kBoundedRows, all);
     return e == cudaSuccess ? go(kOpenRows, open) : e;
 }
