@@ -37,6 +37,11 @@ constexpr int kThreads = 320;               // two softmax groups of four warps,
 constexpr int kMostBlocks = 160;
 constexpr int kUnitCost = 256;              // what a unit costs besides its keys, in keys
 constexpr int kShortestSpan = kUnitCost + kRows;      // of the line, per block: a block inside a cut unit has at least two whole tiles
+// Where no unit has more than kUncutTiles key tiles none is cut, and a block takes the units that are kUnitCost + kHalf or more inside the line of it: spans that are shorter
+// than any unit leave a block one at most. A join costs 10 us, which is the work of some six tiles. Never cut / cut, in us: 8B shape, 1 x 200 queries 17.7 / 28.5,
+// 1 x 1000 28.9 / 35, 4 x 64 behind 700 keys 24 / 28, 40 x 120 43 / 42, 16 x 16 behind 900 33 / 29; 0.5B, 30 x 36 behind 200 14 / 28. One unit per block at most
+// instead of spans of 384, where no unit has two tiles: 24 questions 13.0 against 15.6.
+constexpr int kSpanUncut = 192, kUncutTiles = 8;
 constexpr float kRescale = 8.f;             // log2 of the growth of a maximum that is let be
 constexpr float kLift = 6.f;                // probabilities are kept times 2^kLift: those of 2^-20 are still normal f16 values, and 2^(kLift + kRescale) is one
 
@@ -301,10 +306,17 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention_prompt(const __grid_c
 
     // ---- the line: every thread adds up a run of prompts, the block scans the runs ----
     const int wide = 2 * a.tile_queries, per = (a.n_prompts + kThreads - 1) / kThreads;
+    bool uncut;
     {
         const int i0 = min(a.n_prompts, int(threadIdx.x) * per), i1 = min(a.n_prompts, i0 + per);
         int64_t mine = 0;
-        for (int i = i0; i < i1; i++) mine += prompt_length(a, prompt_at(a, i));
+        bool many = false;
+        for (int i = i0; i < i1; i++) {
+            const Prompt q = prompt_at(a, i);
+            mine += prompt_length(a, q);
+            const int keys = q.queries ? q.ahead + q.queries : 0;
+            many = many || keys > kUncutTiles * kRows;
+        }
         int64_t run = mine;
         for (int d = 1; d < 32; d <<= 1) { const int64_t o = __shfl_up_sync(0xffffffffu, run, d); if (lane >= d) run += o; }
         if (lane == 31) sums[kThreads + warp] = run;
@@ -313,14 +325,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention_prompt(const __grid_c
         sums[threadIdx.x] = run - mine;
         if (threadIdx.x == kThreads - 1) sums[kThreads + 14] = run;
         tc_fence_before();
-        __syncthreads();
+        uncut = __syncthreads_or(many) == 0;
         tc_fence_after();
     }
     uint32_t tmem;
     asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(tmem_slot));
     tmem = __shfl_sync(0xffffffffu, tmem, 0);
     const int64_t total = sums[kThreads + 14];
-    const int blocks = max(1, int(min(int64_t(gridDim.x), total / kShortestSpan)));
+    const int blocks = max(1, int(min(int64_t(gridDim.x), total / (uncut ? kSpanUncut : kShortestSpan))));
     const int64_t each = quotient(total, blocks);
     auto part_at = [&](int b) { return part_of(total, each, b, blocks); };
     const bool idle = total == 0 || int(blockIdx.x) >= blocks;
@@ -347,7 +359,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention_prompt(const __grid_c
     }
     // The segment of unit u that is this block's: key tiles [t0, t1) of its `tiles`.
     struct Segment { int row, queries, first, keys, tiles, t0, t1; int64_t next; };
-    auto tile_of = [&](int64_t x, int tiles) { return int(max(int64_t(0), min(int64_t(tiles), (x - kUnitCost + kRows / 2) / kRows))); };      // (x - kUnitCost < 0 rounds to 0)
+    auto tile_of = [&](int64_t x, int tiles) { return uncut ? (x < kUnitCost + kRows / 2 ? 0 : tiles) : int(max(int64_t(0), min(int64_t(tiles), (x - kUnitCost + kRows / 2) / kRows))); };      // (x - kUnitCost < 0 rounds to 0)
     auto segment = [&]() -> Segment {
         const int q0 = u.tile * wide, n = min(wide, p.queries - q0), keys = p.ahead + q0 + n, tiles = (keys + kRows - 1) / kRows;
         const int64_t end = unit_at + keys + kUnitCost;
