@@ -13,7 +13,10 @@
 //     back only when a row's maximum has grown by more than 2^8 since they were last (probabilities may stand up to 2^8 higher meanwhile).
 // Blocks are persistent, one per SM. The units of all prompts lie end to end, each as long as its last query's keys and a constant for what a unit costs besides; every
 // block takes the same length of this line, cutting units between key tiles. The parts of a cut unit (f32 outputs, maxima, sums) are joined by the last of its
-// blocks to arrive, in the order of the blocks: one prompt of 8192 queries, four pieces of 500 behind 6000 keys and a single query behind 40000 keep all SMs alike.
+// blocks to arrive, in the order of the blocks: one prompt of 8192 queries, four pieces of 500 behind 6000 keys and a single query behind 40000 keep all SMs alike. Where
+// all units are short none is cut.
+// B200: 8192 queries of 40 / 8 heads of 128 in 651 us (1060 TFLOP/s, 765 us when the GPU's power limit holds), four pieces of 300 to 512 behind 6000 keys (32 / 8 heads) in
+// 127 (144): a tile's step is a chain of scores, softmax and weighted sum of 3500 cycles, in which the tensor core works 2048 for both tiles.
 // Queries and probabilities are f16 (the type queries come in; a probability's rounding is 2^-12 of it on average, the outputs' own rounding the same again),
 // scores, sums and outputs f32.
 #include <cuda.h>
