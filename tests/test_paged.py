@@ -512,6 +512,18 @@ def test_attention_of_few_and_many_prompts(new, cached):
 
 
 @gpu
+@pytest.mark.parametrize("longest", [1024, 1025])
+@pytest.mark.parametrize("heads, head_dim", [((8, 2), 64), ((5, 1), 128)])
+def test_attention_of_prompts_whole_units_and_cut_ones(heads, head_dim, longest):
+    """Batches whose longest unit has eight tiles of keys, and nine; more units than there are blocks, and fewer."""
+    H, K = heads
+    for copies in (1, 12):
+        new = [longest, 130, 1, 64, 0, 200] * copies
+        lengths = [longest, 900, 700, 64, 5, 333] * copies
+        check_prompt(Cache(lengths, K, head_dim, 32, seed=copies), new, lengths, H, gaps=(1, 2), every=97)
+
+
+@gpu
 def test_attention_of_prompts_longer_than_their_lengths():
     """The rows in front of the first position see nothing: zeros."""
     check_prompt(Cache([5, 0, 140], 2, 128, 16), [9, 4, 150], [5, 0, 140], 8)
