@@ -12,11 +12,12 @@
 //   * Four warps per tile do the softmax, a thread per row: the row's scores come from tensor memory once, maximum and sum need no other thread. Outputs are scaled
 //     back only when a row's maximum has grown by more than 2^8 since they were last (probabilities may stand up to 2^8 higher meanwhile).
 // Blocks are persistent, one per SM. The units of all prompts lie end to end, each as long as its last query's keys and a constant for what a unit costs besides; every
-// block takes the same length of this line, cutting units between key tiles. The parts of a cut unit (f32 outputs, maxima, sums) are joined by the last of its
-// blocks to arrive, in the order of the blocks: one prompt of 8192 queries, four pieces of 500 behind 6000 keys and a single query behind 40000 keep all SMs alike. Where
-// all units are short none is cut.
-// B200: 8192 queries of 40 / 8 heads of 128 in 651 us (1060 TFLOP/s, 765 us when the GPU's power limit holds), four pieces of 300 to 512 behind 6000 keys (32 / 8 heads) in
-// 127 (144): a tile's step is a chain of scores, softmax and weighted sum of 3500 cycles, in which the tensor core works 2048 for both tiles.
+// block takes the same length of this line, cutting units between key tiles (where all units are short none is cut): one prompt of 8192 queries, four pieces of 500 behind
+// 6000 keys and a single query behind 40000 keep all SMs alike. Of a unit that two blocks share the second, which has its end first thing, leaves its part (f32
+// outputs, maxima, sums), and the first, which has its beginning last, waits for that and adds it to what it has in tensor memory; of more than two the last to arrive
+// joins the parts in the order of the blocks. (With a part and a join for two as well four pieces of 300 to 512 took 127 us.)
+// B200: 8192 queries of 40 / 8 heads of 128 in 651 us (1060 TFLOP/s, 770 us when the GPU's power limit holds), four pieces of 300 to 512 behind 6000 keys (32 / 8 heads) in
+// 120 (138): a tile's step is a chain of scores, softmax and weighted sum of 3500 cycles, in which the tensor core works 2048 for both tiles.
 // Queries and probabilities are f16 (the type queries come in; a probability's rounding is 2^-12 of it on average, the outputs' own rounding the same again),
 // scores, sums and outputs f32.
 #include <cuda.h>
@@ -41,7 +42,7 @@ constexpr int kMostBlocks = 160;
 constexpr int kUnitCost = 256;              // what a unit costs besides its keys, in keys
 constexpr int kShortestSpan = kUnitCost + kRows;      // of the line, per block: a block inside a cut unit has at least two whole tiles
 // Where no unit has more than kUncutTiles key tiles none is cut, and a block takes the units that are kUnitCost + kHalf or more inside the line of it: spans that are shorter
-// than any unit leave a block one at most. A join costs 10 us, which is the work of some six tiles. Never cut / cut, in us: 8B shape, 1 x 200 queries 17.7 / 28.5,
+// than any unit leave a block one at most. A cut costs 5 to 10 us, which is the work of three to six tiles. Never cut / cut, in us: 8B shape, 1 x 200 queries 17.7 / 28.5,
 // 1 x 1000 28.9 / 35, 4 x 64 behind 700 keys 24 / 28, 40 x 120 43 / 42, 16 x 16 behind 900 33 / 29; 0.5B, 30 x 36 behind 200 14 / 28. One unit per block at most
 // instead of spans of 384, where no unit has two tiles: 24 questions 13.0 against 15.6.
 constexpr int kSpanUncut = 192, kUncutTiles = 8;
@@ -238,11 +239,12 @@ __device__ __forceinline__ void join(const Args & a, int b0, int b1, int rows0, 
 // or NaN is NaN. A warp's rows of one tile, of those in `rows` (a NaN among their outputs, of a finite sum); key0, key1: the segment's keys that the tile had. Such a row whose
 // unseen values are at fault is worked out once more, key by key over the segment, against the reference its sum stands for.
 struct Spoilt { uint32_t rows; int seq, kvh, q_row, row0, first, key0, key1, queries; };      // row0: the warp's first row; first: the position of the tile's first query
-// out: the tile's outputs, f16, times by; else part: the tile's part.
+// out: the tile's outputs, f16, times by; else part: the tile's part. Returns the rows that it wrote.
 template <int D>
-__device__ __noinline__ void mend_rows(const Args & a, const Spoilt w, float ref, float by, __half * out, float * part) {
+__device__ __noinline__ uint32_t mend_rows(const Args & a, const Spoilt w, float ref, float by, __half * out, float * part) {
     constexpr int kMine = D / 32;
     const int lane = threadIdx.x % 32;
+    uint32_t written = 0;
     auto line = [&](int key) { return max(a.c.row(w.seq, key), int64_t(0)) * a.c.n_kv + w.kvh; };
     for (uint32_t rest = w.rows; rest; rest &= rest - 1) {
         const int i = __ffs(rest) - 1, r = w.row0 + i, position = w.first + min(r / a.group, w.queries - 1);
@@ -252,6 +254,7 @@ __device__ __noinline__ void mend_rows(const Args & a, const Spoilt w, float ref
             for (int d = 0; d < kMine; d++) odd = odd || !(fabsf(__half2float(v[d])) <= 65504.f);
         }
         if (!__any_sync(0xffffffffu, odd)) continue;
+        written |= 1u << i;
         const float minus = kLift - __shfl_sync(0xffffffffu, ref, i);
         const __half * q = a.q + ((int64_t(w.q_row) + r / a.group) * a.n_head + w.kvh * a.group + r % a.group) * D;
         float o[kMine] = {};
@@ -278,6 +281,7 @@ __device__ __noinline__ void mend_rows(const Args & a, const Spoilt w, float ref
         }
     }
     __syncwarp();
+    return written;
 }
 
 template <int D>
@@ -711,7 +715,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention_prompt(const __grid_c
                         if (w.rows) mend_rows<D>(a, w, ref, by, out, nullptr);
                     }
                 } else {
+                    // the blocks that share the unit: those whose tiles are not none
+                    int b0 = int(quotient((unit_at + 1) * blocks - 1, total)), b1 = int(quotient(s.next * blocks - 1, total));
+                    if (tile_of(part_at(b0 + 1) - unit_at, s.tiles) == 0) b0++;
+                    if (tile_of(part_at(b1) - unit_at, s.tiles) == s.tiles) b1--;
+                    const bool two = b1 == b0 + 1, keeps = two && s.t0 == 0;      // of two blocks the first adds the other's part to what it has
                     float * const part = a.part + ((int64_t(blockIdx.x) * 2 + (s.t0 == 0 ? 1 : 0)) * 2 + x) * kTilePart<D>;
+                    const float2 mine = make_float2(n > 0 && seen ? ref : -CUDART_INF_F, n > 0 ? sum : 0.f);
+                    uint32_t mended = 0;
                     if (n > 0) {
                         #pragma unroll
                         for (int c = 0; c < D; c += 32) {
@@ -721,31 +732,70 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention_prompt(const __grid_c
                             tie32(o);
                             #pragma unroll
                             for (int i = 0; i < 32; i += 2) odd[i / 2 % 2] = add2(odd[i / 2 % 2], pair(__uint_as_float(o[i]), __uint_as_float(o[i + 1])));
-                            #pragma unroll
-                            for (int i = 0; i < 8; i++) {
-                                reinterpret_cast<uint4 *>(part)[(c / 4 + i) * kRows + r] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                            if (!keeps) {
+                                #pragma unroll
+                                for (int i = 0; i < 8; i++) {
+                                    reinterpret_cast<uint4 *>(part)[(c / 4 + i) * kRows + r] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                                }
                             }
                         }
-                    }
-                    if (n > 0) {
                         const Spoilt w = spoilt(sum);
-                        if (w.rows) mend_rows<D>(a, w, ref, 1.f, nullptr, part);
+                        if (w.rows) mended = mend_rows<D>(a, w, ref, 1.f, nullptr, part);
                     }
-                    // (a tile without a step in this segment leaves no outputs, and a maximum that says so)
-                    reinterpret_cast<float2 *>(part + kRows * D)[r] = make_float2(n > 0 && seen ? ref : -CUDART_INF_F, n > 0 ? sum : 0.f);
-                    tc_fence_before();
-                    __threadfence();
-                    asm volatile("bar.sync 1, 256;" ::: "memory");
-                    // the blocks that share the unit: those whose tiles are not none
-                    int b0 = int(quotient((unit_at + 1) * blocks - 1, total)), b1 = int(quotient(s.next * blocks - 1, total));
-                    if (tile_of(part_at(b0 + 1) - unit_at, s.tiles) == 0) b0++;
-                    if (tile_of(part_at(b1) - unit_at, s.tiles) == s.tiles) b1--;
-                    if (threadIdx.x == 0) *flag = paged_counter_arrive(a.arrived + b0, a.call, b1 - b0 + 1, &ok);
-                    asm volatile("bar.sync 1, 256;" ::: "memory");
-                    if (*flag) {
+                    unsigned long long * const counter = a.arrived + b0;
+                    if (!keeps) {
+                        // (a tile without a step in this segment leaves no outputs, and a maximum that says so)
+                        reinterpret_cast<float2 *>(part + kRows * D)[r] = mine;
+                        tc_fence_before();
                         __threadfence();
-                        join<D>(a, b0, b1, x == 0 ? last : min(a.tile_queries, s.queries) * a.group, x == 1 ? last : max(0, s.queries - a.tile_queries) * a.group,
-                                a.out + (int64_t(s.row) * a.n_head + u.kvh * a.group) * D, warp, lane);
+                        asm volatile("bar.sync 1, 256;" ::: "memory");
+                        if (threadIdx.x == 0) *flag = paged_counter_arrive(counter, a.call, two ? 0 : b1 - b0 + 1, &ok);      // (of two blocks none joins by this)
+                        asm volatile("bar.sync 1, 256;" ::: "memory");
+                        if (*flag) {
+                            __threadfence();
+                            join<D>(a, b0, b1, x == 0 ? last : min(a.tile_queries, s.queries) * a.group, x == 1 ? last : max(0, s.queries - a.tile_queries) * a.group,
+                                    a.out + (int64_t(s.row) * a.n_head + u.kvh * a.group) * D, warp, lane);
+                        }
+                    } else {
+                        asm volatile("bar.sync 1, 256;" ::: "memory");
+                        if (threadIdx.x == 0) *flag = ok = paged_counter_wait(counter, a.call, 1) && ok;
+                        asm volatile("bar.sync 1, 256;" ::: "memory");
+                        if (*flag && n > 0) {
+                            __threadfence();
+                            const float * const other = a.part + (int64_t(b1) * 4 + x) * kTilePart<D>;
+                            const float2 theirs = __ldcg(reinterpret_cast<const float2 *>(other + kRows * D) + r);
+                            const float top = fmaxf(mine.x, theirs.x), minus = top == -CUDART_INF_F ? 0.f : top;
+                            const bool some = mine.x > -CUDART_INF_F, theirs_some = theirs.x > -CUDART_INF_F;
+                            const float share = ex2(mine.x - minus), their_share = ex2(theirs.x - minus);
+                            const float l = (some ? mine.y * share : 0.f) + (theirs_some ? theirs.y * their_share : 0.f), by = l > 0.f || l != l ? 1.f / l : 0.f;
+                            const float by_mine = share * by, by_theirs = their_share * by;
+                            const bool again = mended >> lane & 1u;      // (this row's outputs were worked out again, into the part)
+                            #pragma unroll
+                            for (int c = 0; c < D; c += 32) {
+                                uint32_t o[32];
+                                float4 w[8];
+                                #pragma unroll
+                                for (int i = 0; i < 8; i++) w[i] = theirs_some ? __ldcg(reinterpret_cast<const float4 *>(other) + (c / 4 + i) * kRows + r) : make_float4(0.f, 0.f, 0.f, 0.f);
+                                tc_ld32(o_at + c, o);
+                                tc_wait_ld();
+                                tie32(o);
+                                if (again) {
+                                    #pragma unroll
+                                    for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__ldcg(part + ((c / 4 + i / 4) * kRows + r) * 4 + i % 4));
+                                }
+                                #pragma unroll
+                                for (int i = 0; i < 8; i++) {
+                                    float v[4] = {__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]), __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3])};
+                                    #pragma unroll
+                                    for (int k = 0; k < 4; k++) v[k] = some ? v[k] * by_mine : 0.f;
+                                    const __half2 h0 = __floats2half2_rn(fmaf(w[i].x, by_theirs, v[0]), fmaf(w[i].y, by_theirs, v[1]));
+                                    const __half2 h1 = __floats2half2_rn(fmaf(w[i].z, by_theirs, v[2]), fmaf(w[i].w, by_theirs, v[3]));
+                                    o[2 * i] = *reinterpret_cast<const uint32_t *>(&h0);
+                                    o[2 * i + 1] = *reinterpret_cast<const uint32_t *>(&h1);
+                                }
+                                write_rows(o, c);
+                            }
+                        }
                     }
                 }
                 tc_fence_before();

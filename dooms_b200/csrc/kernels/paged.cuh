@@ -57,6 +57,15 @@ __device__ __forceinline__ bool paged_counter_arrive(unsigned long long * counte
     return true;
 }
 
+// One thread of the block that owns the counter: whether `count` others have arrived (one that has not within the limit never counts). The counter is zero then.
+__device__ __forceinline__ bool paged_counter_wait(unsigned long long * counter, unsigned long long call, int count) {
+    uint32_t polls = 0;
+    const unsigned long long all = call << 16 | (unsigned long long)count;
+    while (*reinterpret_cast<volatile unsigned long long *>(counter) != all && ++polls < (1u << 22)) {}
+    *reinterpret_cast<volatile unsigned long long *>(counter) = 0;
+    return polls < (1u << 22);
+}
+
 inline PagedView paged_view(const PagedCache & c, int * error) {
     int shift = 0;
     while ((1 << shift) < c.page_size) shift++;
