@@ -575,6 +575,36 @@ def test_attention_of_prompts_values_that_are_not_finite(heads, head_dim, page, 
 
 
 @gpu
+@pytest.mark.parametrize("heads, head_dim, batch", [((3, 3), 64, 30), ((2, 2), 128, 44), ((14, 2), 64, 40)])
+def test_attention_of_prompts_cut_in_two_around_a_value_that_is_not_finite(heads, head_dim, batch):
+    """So many units that a cut one is shared by two blocks, at every tile in turn; the position that is not finite is now in the part of the one, now of the other."""
+    H, K = heads
+    n, at, s = 300, 130, 1 / math.sqrt(head_dim)
+    lengths = [900 + 17 * i + n for i in range(batch)]
+    cache = Cache(lengths, K, head_dim, 64, seed=H)
+    for i in range(batch):
+        cache.rows(cache.host[1], i)[cache.line(i, lengths[i])[lengths[i] - n + at], :, i % head_dim] = (math.nan, math.inf)[i % 2]
+    cache.upload()
+    q = np.random.default_rng(4).standard_normal((batch * n, H, head_dim)).astype(np.float16)
+    start = np.arange(batch + 1, dtype=np.int32) * n
+    out = torch.full(q.shape, 77.0, dtype=torch.float16, device="cuda")
+    cache.cache.attention_prompt(cuda(q), cuda(np.arange(batch, dtype=np.int32)), cuda(start), cuda(np.array(lengths, np.int32)), out, cache.scratch(H))
+    assert status() == (L.OK, 0)
+    got = out.cpu().numpy().astype(np.float64).reshape(batch, n, H, head_dim)
+    assert np.isfinite(got[:, :at]).all()
+    for i in range(batch):
+        k, v = cache.sequence(i, lengths[i])
+        v = np.where(np.isfinite(v), v, 0.0)
+        for j in (0, 70, 120, at - 1, at, 299):
+            r = got[i, j].copy()
+            want, mass, reach = attend(q[i * n + j].astype(np.float64), k[:lengths[i] - n + j + 1], v[:lengths[i] - n + j + 1], s)
+            if j >= at:
+                assert not np.isfinite(r[:, i % head_dim]).any()
+                want[:, i % head_dim] = r[:, i % head_dim] = 0.0
+            assert (np.abs(r - want) <= bound(want, mass, reach, head_dim, s, True)).all(), (i, j)
+
+
+@gpu
 def test_a_long_prompt_in_one_call_is_its_pieces():
     """2100 positions at once, and as pieces behind what is cached: the same rows up to the roundings of two results."""
     H, D, n = 10, 128, 2100
