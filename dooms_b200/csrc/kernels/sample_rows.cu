@@ -413,8 +413,10 @@ __device__ void resolve(Row & r, bool by_count, double per, unsigned long long g
 __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const SampleArgs a) {
     extern __shared__ __align__(16) uint8_t smem[];
     Shared & s = *reinterpret_cast<Shared *>(smem);
-    // With two launches the second may start as soon as the first's blocks have, which is when what both read is there; it waits for the first at its end.
-    if (a.rows_of != kOpenRows) { pdl_wait(); pdl_trigger(); }
+    // With two launches the second may start as soon as the first's blocks have, which is when what both read is there; it waits for the first at its end. What follows the
+    // call in the stream is the caller's (and may be a programmatic dependent that does not wait before it reads): it is released by the last launch's finishing alone.
+    if (a.rows_of != kOpenRows) pdl_wait();
+    if (a.rows_of == kBoundedRows) pdl_trigger();
     uint32_t rank, blocks;
     asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
     asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(blocks));
