@@ -45,7 +45,7 @@ struct Args {
     const int32_t * sequence, * lengths;
     float scale_log2;
     unsigned long long call;               // the call's number, not zero
-    unsigned long long * arrived;          // [block]: of the item cut behind that block, the call's number << 16 | blocks that have left their part
+    Arrivals * arrived;                    // [block]: of the item cut behind that block, the blocks that have left their part
     float * part;                          // [block][2]: outputs [kHeads][D], then (max, sum) [kHeads]
 };
 
@@ -270,7 +270,6 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) k_attention_paged(cons
         }
         rows_without(lane, 32);
     } else {
-        paged_counter_begin(a.arrived + blockIdx.x, a.call);      // of the item that this block's span may end in
         const int g = lane >> 2, t = lane & 3;
         // where this lane's ldmatrix rows lie in a stage: keys 16 warp + .., as rows of the A operand (S^T = K Q^T), and as its columns (O^T = V^T P^T)
         const int krow = warp * 16 + (lane & 7) + ((lane >> 3) & 1) * 8, kchunk = lane >> 4;
@@ -484,9 +483,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) k_attention_paged(cons
                 if (warp == 0) {
                     __threadfence();
                     __syncwarp();
-                    if (lane == 0) {
-                        *last = paged_counter_arrive(a.arrived + first, a.call, count, &ok);
-                    }
+                    if (lane == 0) *last = paged_counter_arrive(a.arrived + first, a.call, count, !ok);
                 }
                 asm volatile("bar.sync 1, 128;" ::: "memory");
                 if (*last) {
@@ -524,7 +521,7 @@ cudaError_t launch_attention_paged(const PagedCache & cache, const void * q, voi
     a.sequence = sequence; a.lengths = lengths;
     a.scale_log2 = scale * 1.44269504f;
     a.call = paged_call();
-    a.arrived = static_cast<unsigned long long *>(scratch);
+    a.arrived = static_cast<Arrivals *>(scratch);
     a.part = reinterpret_cast<float *>(a.arrived + kMostBlocks);
     const int blocks = std::min(kMostBlocks, kBlocksPerSm * sm_count());
     const int64_t rows = int64_t(cache.n_pages) * cache.page_size;

@@ -56,7 +56,8 @@ struct Args {
     int n_head, group, tile_queries, n_prompts, n_rows;      // tile_queries: queries per tile
     const int32_t * sequence, * start, * lengths;
     float scale_log2;
-    unsigned long long call, * arrived;
+    unsigned long long call;
+    Arrivals * arrived;                     // [block]: of the unit cut behind that block, the blocks that have left their part
     float * part;                           // [block][2][tile]: outputs [D / 4][kRows] float4, then (max, sum) [kRows]
 };
 
@@ -542,7 +543,6 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention_prompt(const __grid_c
         const int query = x * a.tile_queries + r / a.group;      // of the unit
         const bool row_there = r < a.tile_queries * a.group;
         uint32_t step = 0;      // scores taken
-        paged_counter_begin(a.arrived + blockIdx.x, a.call);      // of the unit that this block's part of the line may end in
         while (unit_at < to) {
             const Segment s = segment();
             if (s.t0 < s.t1) {
@@ -742,14 +742,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention_prompt(const __grid_c
                         const Spoilt w = spoilt(sum);
                         if (w.rows) mended = mend_rows<D>(a, w, ref, 1.f, nullptr, part);
                     }
-                    unsigned long long * const counter = a.arrived + b0;
+                    Arrivals * const counter = a.arrived + b0;
                     if (!keeps) {
                         // (a tile without a step in this segment leaves no outputs, and a maximum that says so)
                         reinterpret_cast<float2 *>(part + kRows * D)[r] = mine;
                         tc_fence_before();
                         __threadfence();
                         asm volatile("bar.sync 1, 256;" ::: "memory");
-                        if (threadIdx.x == 0) *flag = paged_counter_arrive(counter, a.call, two ? 0 : b1 - b0 + 1, &ok);      // (of two blocks none joins by this)
+                        if (threadIdx.x == 0) *flag = paged_counter_arrive(counter, a.call, b1 - b0 + 1, !ok);      // (of two blocks the first arrives last)
                         asm volatile("bar.sync 1, 256;" ::: "memory");
                         if (*flag) {
                             __threadfence();
@@ -758,7 +758,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention_prompt(const __grid_c
                         }
                     } else {
                         asm volatile("bar.sync 1, 256;" ::: "memory");
-                        if (threadIdx.x == 0) *flag = ok = paged_counter_wait(counter, a.call, 1) && ok;
+                        if (threadIdx.x == 0) *flag = ok = paged_counter_wait(counter, a.call, !ok);
                         asm volatile("bar.sync 1, 256;" ::: "memory");
                         if (*flag && n > 0) {
                             __threadfence();
@@ -841,7 +841,7 @@ cudaError_t launch_attention_prompt_paged(const PagedCache & cache, const void *
     a.sequence = sequence; a.start = start; a.lengths = lengths;
     a.scale_log2 = scale * 1.44269504f;
     a.call = paged_call();
-    a.arrived = static_cast<unsigned long long *>(scratch);
+    a.arrived = static_cast<Arrivals *>(scratch);
     a.part = reinterpret_cast<float *>(a.arrived + kMostBlocks);
     TensorMap qmap, kmap, vmap;
     const int box = std::min(kRows, cache.page_size);

@@ -6,6 +6,7 @@
 #include <atomic>
 #include <chrono>
 
+#include "arrivals.h"
 #include "kernels.h"
 
 namespace dooms {
@@ -35,35 +36,33 @@ __device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
 // Where the b-th of n equal parts of `total` begins.
 __device__ __forceinline__ int64_t part_of(int64_t total, int64_t each, int b, int n) { return each * b + int64_t(uint64_t(total - each * n) * uint32_t(b) / uint32_t(n)); }
 
-// Arrival counters in scratch memory whose contents at the start do not matter: a counter is (a call's own number, 48 bits, not zero) << 16 | blocks that have
-// arrived. The block that owns the counter sets it up when it begins; others (behind it in the grid) wait until it carries the call's number. The last
-// one to arrive leaves zero, so that a replayed call, whose number is the same, finds no count of its own; one that nobody arrived at stays set up for the replay.
+// A call's own number for its arrival counters (arrivals.h).
 inline unsigned long long paged_call() {
     static std::atomic<unsigned long long> calls{(unsigned long long)(std::chrono::steady_clock::now().time_since_epoch().count()) * 0x9E3779B97F4A7C15ull >> 20};
     unsigned long long c;
-    do c = calls.fetch_add(1, std::memory_order_relaxed) & 0xffffffffffffull; while (c == 0 || c == 0xffffffffffffull);
+    do c = calls.fetch_add(1, std::memory_order_relaxed) % kArrivalsCalls; while (c == 0 || c == kArrivalsCalls - 1);
     return c;
 }
-__device__ __forceinline__ void paged_counter_begin(unsigned long long * counter, unsigned long long call) {
-    if (threadIdx.x == 0 && (*reinterpret_cast<volatile unsigned long long *>(counter) >> 16) != call) atomicExch(counter, call << 16);
+struct ArrivalsInMemory {
+    Arrivals * at;
+    __device__ __forceinline__ Arrivals load() const { return *reinterpret_cast<volatile Arrivals *>(at); }
+    __device__ __forceinline__ Arrivals swap(Arrivals was, Arrivals to) const { return atomicCAS(at, was, to); }
+    __device__ __forceinline__ Arrivals add(Arrivals n) const { return atomicAdd(at, n); }
+    __device__ __forceinline__ void store(Arrivals to) const { *reinterpret_cast<volatile Arrivals *>(at) = to; }
+};
+// One thread, behind a barrier of those whose stores it stands for and a __threadfence of each: whether it is the last of `count` to arrive, and none of them failed.
+__device__ __forceinline__ bool paged_counter_arrive(Arrivals * counter, unsigned long long call, int count, bool failed) {
+    return arrive(ArrivalsInMemory{counter}, call, count, failed) == Arrival::kLast;
 }
-// One thread, behind a barrier of those whose stores it stands for and a __threadfence of each: whether it is the last of `count` to arrive.
-__device__ __forceinline__ bool paged_counter_arrive(unsigned long long * counter, unsigned long long call, int count, bool * ok) {
+// One thread of the first of two blocks that share a counter: its own arrival, once the other's is there. False: that one failed, or did not come within the limit (it is
+// the last then, and knows that this one has given up).
+__device__ __forceinline__ bool paged_counter_wait(Arrivals * counter, unsigned long long call, bool failed) {
+    const ArrivalsInMemory memory{counter};
+    const auto there = [&] { const Arrivals a = memory.load(); return arrivals_call(a) == call && arrivals_count(a) == 1; };
     uint32_t polls = 0;
-    while ((*reinterpret_cast<volatile unsigned long long *>(counter) >> 16) != call && ++polls < (1u << 22)) {}
-    *ok = *ok && polls < (1u << 22);
-    if (!*ok || int(atomicAdd(counter, 1ull) & 0xffffu) + 1 != count) return false;
-    *reinterpret_cast<volatile unsigned long long *>(counter) = 0;
-    return true;
-}
-
-// One thread of the block that owns the counter: whether `count` others have arrived (one that has not within the limit never counts). The counter is zero then.
-__device__ __forceinline__ bool paged_counter_wait(unsigned long long * counter, unsigned long long call, int count) {
-    uint32_t polls = 0;
-    const unsigned long long all = call << 16 | (unsigned long long)count;
-    while (*reinterpret_cast<volatile unsigned long long *>(counter) != all && ++polls < (1u << 22)) {}
-    *reinterpret_cast<volatile unsigned long long *>(counter) = 0;
-    return polls < (1u << 22);
+    bool came = there();
+    while (!came && ++polls < (1u << 22)) came = there();
+    return paged_counter_arrive(counter, call, 2, failed || !came);
 }
 
 inline PagedView paged_view(const PagedCache & c, int * error) {

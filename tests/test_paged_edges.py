@@ -8,9 +8,10 @@ import numpy as np
 import pytest
 import torch
 
+from dooms_b200 import _lib as L
 from dooms_b200 import build as B
 from dooms_b200 import paged
-from test_paged import cuda
+from test_paged import Cache, cuda, status
 
 gpu = pytest.mark.gpu
 HERE = Path(__file__).resolve().parent
@@ -46,3 +47,54 @@ def test_what_follows_the_sampling_sees_its_tokens(probes, rows, n):
         assert probes.probe_copy_at_once(tokens.data_ptr(), seen.data_ptr(), rows, stream.cuda_stream) == 0
         torch.cuda.synchronize()
         assert (tokens >= 0).all() and torch.equal(tokens, seen)
+
+
+# ---------------------------------------------------------------- the counters in the scratch
+
+@pytest.fixture(scope="module")
+def arrivals():
+    source, header, out = HERE / "paged_arrivals.cpp", B.CSRC / "kernels" / "arrivals.h", HERE / "_build" / "libpaged_arrivals.so"
+    if not out.exists() or out.stat().st_mtime < max(source.stat().st_mtime, header.stat().st_mtime):
+        out.parent.mkdir(exist_ok=True)
+        subprocess.run(["g++", "-std=c++20", "-O2", "-Wall", "-shared", "-fPIC", f"-I{header.parent}", str(source), "-o", str(out)], check=True, capture_output=True)
+    lib = C.CDLL(str(out))
+    lib.arrivals_orders.argtypes = [C.c_int, C.c_ulonglong, C.c_uint, C.c_ulonglong, C.POINTER(C.c_longlong)]
+    lib.arrivals_orders.restype = C.c_longlong
+    return lib
+
+
+@pytest.mark.parametrize("start", [0, 1, (1 << 64) - 1, 76 << 20 | 3, 78 << 20 | 1 << 10 | 2, 77 << 16 | 1])
+def test_of_those_that_arrive_one_is_the_last_and_leaves_zero(arrivals, start):
+    """In every order of their memory operations, whatever the counter held (but the call's own number), and those that failed before: a launch in which a wait ran out leaves
+    nothing behind that its replay, whose number is the same, would count on from."""
+    for n, orders in ((1, 1), (2, 1), (3, 100)):
+        for failed in range(1 << n):
+            wrong = C.c_longlong(-1)
+            assert arrivals.arrivals_orders(n, 77, failed, start, C.byref(wrong)) >= orders
+            assert wrong.value == 0, (n, failed)
+
+
+@gpu
+def test_counters_are_zero_behind_a_call_and_behind_its_replays():
+    """Of what the scratch held before, every counter that was used is zero and every other is left as it was: items and units that two blocks share and that many do."""
+    H, D = 8, 128
+    cache = Cache([9000, 1, 0, 30000, 64], 1, D, 64)
+    g = np.random.default_rng(4)
+    lengths, seq = cuda(np.array(cache.lengths, np.int32)), torch.arange(5, dtype=torch.int32, device="cuda")
+    q, out = cuda(g.standard_normal((5, H, D)), torch.float32), torch.zeros(5, H, D, device="cuda")
+    start = cuda(np.array([0, 700, 701, 701, 731, 750], np.int32))
+    pq, pout = cuda(g.standard_normal((750, H, D)), torch.float16), torch.zeros(750, H, D, dtype=torch.float16, device="cuda")
+    for call in (lambda s, stream: cache.cache.attention(q, seq, lengths, 30000, out, s, stream=stream),
+                 lambda s, stream: cache.cache.attention_prompt(pq, seq, start, lengths, pout, s, stream=stream)):
+        scratch = cache.scratch(H)
+        counters = scratch[:160 * 8].view(torch.int64)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            call(scratch, torch.cuda.current_stream().cuda_stream)
+        results = []
+        for _ in range(3):
+            graph.replay()
+            results.append((out.clone(), pout.clone()))
+            assert ((counters == 0) | (counters == -1)).all() and (counters == 0).any()
+        assert all(torch.equal(a, b) for r in results[1:] for a, b in zip(r, results[0]))
+    assert status() == (L.OK, 0)
