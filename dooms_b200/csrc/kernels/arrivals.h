@@ -4,7 +4,7 @@
 // A counter is (a call's own number, 44 bits, not zero) << 20 | blocks that failed << 10 | blocks that have arrived, failed ones too. Whoever arrives first finds another
 // call's number, or anything else, and replaces it. Every block of a launch arrives exactly once at each counter that is its, whatever happened to it before, and the
 // last one leaves zero: so when a launch is over no counter has its number, and a replay of it in a graph, whose number is the same, finds no count of an earlier one.
-// That holds for a launch in which a bounded wait ran out as well. Nobody waits for the counter itself.
+// That holds for a launch in which a bounded wait ran out as well. No block needs another one to run beside it.
 #include <cstdint>
 
 #ifdef __CUDACC__

@@ -14,8 +14,9 @@
 // Blocks are persistent, one per SM. The units of all prompts lie end to end, each as long as its last query's keys and a constant for what a unit costs besides; every
 // block takes the same length of this line, cutting units between key tiles (where all units are short none is cut): one prompt of 8192 queries, four pieces of 500 behind
 // 6000 keys and a single query behind 40000 keep all SMs alike. Of a unit that two blocks share the second, which has its end first thing, leaves its part (f32
-// outputs, maxima, sums), and the first, which has its beginning last, waits for that and adds it to what it has in tensor memory; of more than two the last to arrive
-// joins the parts in the order of the blocks. (With a part and a join for two as well four pieces of 300 to 512 took 127 us.)
+// outputs, maxima, sums), and the first, which has its beginning last, adds that to what it has in tensor memory. Where the second has not come within a millisecond (it
+// may be waiting for an SM), the first leaves its part too. Of more than two blocks each leaves its part. The last to arrive joins the parts
+// in the order of the blocks. (With a part and a join for two as well four pieces of 300 to 512 took 127 us.)
 // B200: 8192 queries of 40 / 8 heads of 128 in 651 us (1060 TFLOP/s, 770 us when the GPU's power limit holds), four pieces of 300 to 512 behind 6000 keys (32 / 8 heads) in
 // 120 (138): a tile's step is a chain of scores, softmax and weighted sum of 3500 cycles, in which the tensor core works 2048 for both tiles.
 // Queries and probabilities are f16 (the type queries come in; a probability's rounding is 2^-12 of it on average, the outputs' own rounding the same again),
@@ -719,7 +720,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention_prompt(const __grid_c
                     int b0 = int(quotient((unit_at + 1) * blocks - 1, total)), b1 = int(quotient(s.next * blocks - 1, total));
                     if (tile_of(part_at(b0 + 1) - unit_at, s.tiles) == 0) b0++;
                     if (tile_of(part_at(b1) - unit_at, s.tiles) == s.tiles) b1--;
-                    const bool two = b1 == b0 + 1, keeps = two && s.t0 == 0;      // of two blocks the first adds the other's part to what it has
+                    const bool keeps = b1 == b0 + 1 && s.t0 == 0;      // of two blocks the first adds the other's part to what it has
                     float * const part = a.part + ((int64_t(blockIdx.x) * 2 + (s.t0 == 0 ? 1 : 0)) * 2 + x) * kTilePart<D>;
                     const float2 mine = make_float2(n > 0 && seen ? ref : -CUDART_INF_F, n > 0 ? sum : 0.f);
                     uint32_t mended = 0;
@@ -743,33 +744,24 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention_prompt(const __grid_c
                         if (w.rows) mended = mend_rows<D>(a, w, ref, 1.f, nullptr, part);
                     }
                     Arrivals * const counter = a.arrived + b0;
-                    if (!keeps) {
-                        // (a tile without a step in this segment leaves no outputs, and a maximum that says so)
-                        reinterpret_cast<float2 *>(part + kRows * D)[r] = mine;
-                        tc_fence_before();
-                        __threadfence();
+                    bool leaves = !keeps;
+                    if (keeps) {
                         asm volatile("bar.sync 1, 256;" ::: "memory");
-                        if (threadIdx.x == 0) *flag = paged_counter_arrive(counter, a.call, b1 - b0 + 1, !ok);      // (of two blocks the first arrives last)
+                        if (threadIdx.x == 0) { *flag = paged_counter_wait(counter, a.call, !ok); ok = ok && *flag >= 0; }
                         asm volatile("bar.sync 1, 256;" ::: "memory");
-                        if (*flag) {
-                            __threadfence();
-                            join<D>(a, b0, b1, x == 0 ? last : min(a.tile_queries, s.queries) * a.group, x == 1 ? last : max(0, s.queries - a.tile_queries) * a.group,
-                                    a.out + (int64_t(s.row) * a.n_head + u.kvh * a.group) * D, warp, lane);
-                        }
-                    } else {
-                        asm volatile("bar.sync 1, 256;" ::: "memory");
-                        if (threadIdx.x == 0) *flag = ok = paged_counter_wait(counter, a.call, !ok);
-                        asm volatile("bar.sync 1, 256;" ::: "memory");
-                        if (*flag && n > 0) {
+                        const int came = *flag;
+                        leaves = came == 0;
+                        const bool again = mended >> lane & 1u;      // (this row's outputs were worked out again, into the part)
+                        if (came > 0 && n > 0) {      // (the arithmetic of join(), so that it does not matter which of the two it is)
                             __threadfence();
                             const float * const other = a.part + (int64_t(b1) * 4 + x) * kTilePart<D>;
                             const float2 theirs = __ldcg(reinterpret_cast<const float2 *>(other + kRows * D) + r);
                             const float top = fmaxf(mine.x, theirs.x), minus = top == -CUDART_INF_F ? 0.f : top;
                             const bool some = mine.x > -CUDART_INF_F, theirs_some = theirs.x > -CUDART_INF_F;
                             const float share = ex2(mine.x - minus), their_share = ex2(theirs.x - minus);
-                            const float l = (some ? mine.y * share : 0.f) + (theirs_some ? theirs.y * their_share : 0.f), by = l > 0.f || l != l ? 1.f / l : 0.f;
-                            const float by_mine = share * by, by_theirs = their_share * by;
-                            const bool again = mended >> lane & 1u;      // (this row's outputs were worked out again, into the part)
+                            float l = some ? fmaf(mine.y, share, 0.f) : 0.f;
+                            l = theirs_some ? fmaf(theirs.y, their_share, l) : l;
+                            const float by = l > 0.f || l != l ? 1.f / l : 0.f;
                             #pragma unroll
                             for (int c = 0; c < D; c += 32) {
                                 uint32_t o[32];
@@ -786,15 +778,43 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention_prompt(const __grid_c
                                 #pragma unroll
                                 for (int i = 0; i < 8; i++) {
                                     float v[4] = {__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]), __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3])};
+                                    const float add[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
                                     #pragma unroll
-                                    for (int k = 0; k < 4; k++) v[k] = some ? v[k] * by_mine : 0.f;
-                                    const __half2 h0 = __floats2half2_rn(fmaf(w[i].x, by_theirs, v[0]), fmaf(w[i].y, by_theirs, v[1]));
-                                    const __half2 h1 = __floats2half2_rn(fmaf(w[i].z, by_theirs, v[2]), fmaf(w[i].w, by_theirs, v[3]));
+                                    for (int k = 0; k < 4; k++) v[k] = fmaf(add[k], theirs_some ? their_share : 0.f, some ? fmaf(v[k], share, 0.f) : 0.f) * by;
+                                    const __half2 h0 = __floats2half2_rn(v[0], v[1]), h1 = __floats2half2_rn(v[2], v[3]);
                                     o[2 * i] = *reinterpret_cast<const uint32_t *>(&h0);
                                     o[2 * i + 1] = *reinterpret_cast<const uint32_t *>(&h1);
                                 }
                                 write_rows(o, c);
                             }
+                        } else if (leaves && n > 0) {
+                            #pragma unroll
+                            for (int c = 0; c < D; c += 32) {
+                                uint32_t o[32];
+                                tc_ld32(o_at + c, o);
+                                tc_wait_ld();
+                                tie32(o);
+                                if (!again) {
+                                    #pragma unroll
+                                    for (int i = 0; i < 8; i++) {
+                                        reinterpret_cast<uint4 *>(part)[(c / 4 + i) * kRows + r] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                                    }
+                                }
+                            }
+                        }
+                    }
+                    if (leaves) {
+                        // (a tile without a step in this segment leaves no outputs, and a maximum that says so)
+                        reinterpret_cast<float2 *>(part + kRows * D)[r] = mine;
+                        tc_fence_before();
+                        __threadfence();
+                        asm volatile("bar.sync 1, 256;" ::: "memory");
+                        if (threadIdx.x == 0) *flag = paged_counter_arrive(counter, a.call, b1 - b0 + 1, !ok);
+                        asm volatile("bar.sync 1, 256;" ::: "memory");
+                        if (*flag) {
+                            __threadfence();
+                            join<D>(a, b0, b1, x == 0 ? last : min(a.tile_queries, s.queries) * a.group, x == 1 ? last : max(0, s.queries - a.tile_queries) * a.group,
+                                    a.out + (int64_t(s.row) * a.n_head + u.kvh * a.group) * D, warp, lane);
                         }
                     }
                 }

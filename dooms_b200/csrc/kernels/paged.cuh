@@ -54,15 +54,15 @@ struct ArrivalsInMemory {
 __device__ __forceinline__ bool paged_counter_arrive(Arrivals * counter, unsigned long long call, int count, bool failed) {
     return arrive(ArrivalsInMemory{counter}, call, count, failed) == Arrival::kLast;
 }
-// One thread of the first of two blocks that share a counter: its own arrival, once the other's is there. False: that one failed, or did not come within the limit (it is
-// the last then, and knows that this one has given up).
-__device__ __forceinline__ bool paged_counter_wait(Arrivals * counter, unsigned long long call, bool failed) {
+// One thread of the first of two blocks that share a counter: 1: the other has left its part, and this one has arrived behind it; -1: it came, but failed; 0: it is not there
+// yet, and this one has not arrived. The other block may not run before this one's SM is free (beside a long kernel of another stream, say), so the wait is short: about
+// a millisecond; usually the other came long before.
+__device__ __forceinline__ int paged_counter_wait(Arrivals * counter, unsigned long long call, bool failed) {
     const ArrivalsInMemory memory{counter};
     const auto there = [&] { const Arrivals a = memory.load(); return arrivals_call(a) == call && arrivals_count(a) == 1; };
-    uint32_t polls = 0;
     bool came = there();
-    while (!came && ++polls < (1u << 22)) came = there();
-    return paged_counter_arrive(counter, call, 2, failed || !came);
+    for (int polls = 0; !came && polls < 2048; polls++) came = there();
+    return !came ? 0 : paged_counter_arrive(counter, call, 2, failed) ? 1 : -1;
 }
 
 inline PagedView paged_view(const PagedCache & c, int * error) {

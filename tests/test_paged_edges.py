@@ -2,6 +2,7 @@
 just not allowed. The plain forms and helpers are test_paged.py's."""
 import ctypes as C
 import subprocess
+import time
 from pathlib import Path
 
 import numpy as np
@@ -98,3 +99,49 @@ def test_counters_are_zero_behind_a_call_and_behind_its_replays():
             assert ((counters == 0) | (counters == -1)).all() and (counters == 0).any()
         assert all(torch.equal(a, b) for r in results[1:] for a, b in zip(r, results[0]))
     assert status() == (L.OK, 0)
+
+
+# ---------------------------------------------------------------- beside other work
+
+@gpu
+@pytest.mark.parametrize("heads, head_dim", [((8, 1), 128), ((14, 2), 64)])
+def test_calls_that_get_one_sm_beside_a_long_kernel(probes, heads, head_dim):
+    """Blocks that share an item or a unit may run one after another: no call needs two of its blocks at once, and what it gives does not depend on it. Cut in two and in many, with
+    a value that is not finite and that only later queries see."""
+    (H, K), D = heads, head_dim
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    cache = Cache([30000, 1, 2100, 1300], K, D, 64)
+    for i, at in ((0, 29950), (2, 2050)):
+        cache.host[1].reshape(-1, K, D)[cache.line(i, cache.lengths[i])[at], :, 3] = np.inf
+    cache.upload()
+    g = np.random.default_rng(11)
+    lengths, seq = cuda(np.array(cache.lengths, np.int32)), torch.arange(4, dtype=torch.int32, device="cuda")
+    rows = [300, 1, 500, 1300]
+    start = cuda(np.concatenate([[0], np.cumsum(rows)]).astype(np.int32))
+    q, pq = cuda(g.standard_normal((4, H, D)), torch.float32), cuda(g.standard_normal((sum(rows), H, D)), torch.float16)
+    scratch, side, other = cache.scratch(H), torch.cuda.Stream(), torch.cuda.Stream()
+
+    def run():
+        out, pout = torch.zeros(4, H, D, device="cuda"), torch.zeros_like(pq)
+        torch.cuda.synchronize()
+        return out, pout, lambda: (cache.cache.attention(q, seq, lengths, 30000, out, scratch, stream=side.cuda_stream),
+                                   cache.cache.attention_prompt(pq, seq, start, lengths, pout, scratch, stream=side.cuda_stream))
+    alone, palone, call = run()
+    call()
+    torch.cuda.synchronize()
+    assert palone.isfinite().float().mean() > 0.9 and not palone.isfinite().all()
+    out, pout, call = run()
+    begun, held, done = (torch.cuda.Event() for _ in range(3))
+    with torch.cuda.stream(other):
+        begun.record()
+        assert probes.probe_hold(sms - 1, 1_500_000_000, other.cuda_stream) == 0
+        held.record()
+    begun.synchronize()
+    time.sleep(0.02)
+    call()
+    done.record(side)
+    done.synchronize()
+    assert not held.query()      # (they did not have to wait for the other SMs)
+    torch.cuda.synchronize()
+    assert status() == (L.OK, 0)
+    assert torch.equal(out, alone) and torch.equal(pout.nan_to_num(5.0), palone.nan_to_num(5.0))
