@@ -269,6 +269,8 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) k_attention_paged(cons
             if (left > 0) next_item();
         }
         rows_without(lane, 32);
+        // no copy is under way when the block ends, not behind a wait that ran out either: each stage's last one (of this round in front of `stage`, of the round before from there on)
+        for (int s = 0; s < K::kStages; s++) ok = mbar_wait(full + 8 * s, s < stage ? phase : phase ^ 1u) && ok;
     } else {
         const int g = lane >> 2, t = lane & 3;
         // where this lane's ldmatrix rows lie in a stage: keys 16 warp + .., as rows of the A operand (S^T = K Q^T), and as its columns (O^T = V^T P^T)
@@ -415,7 +417,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) k_attention_paged(cons
                     if (valid < 16) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");      // (the zeros, before a copy may land on them)
                 }
                 __syncwarp();
-                if (lane == 0) mbar_arrive(empty + 8 * stage);
+                if (lane == 0 && ok) mbar_arrive(empty + 8 * stage);      // (a stage whose copy did not come is not filled again)
                 advance();
             }
             const bool ends = p.tile == p.tiles;

@@ -296,11 +296,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention_prompt(const __grid_c
     int * const flag = reinterpret_cast<int *>(sums + kThreads + 15);
     const uint32_t bars = smem_u32(sums + kThreads + 16);
     const uint32_t q_full = bars, q_empty = bars + 8, s_full = bars + 16, p_full = bars + 32, o_done = bars + 64, k_full = bars + 80, k_empty = k_full + 8 * S, v_full = k_empty + 8 * S,
-                   v_empty = v_full + 8 * S, v_fixed = v_empty + 8 * S, tmem_slot = v_fixed + 8 * S;
+                   v_empty = v_full + 8 * S, v_fixed = v_empty + 8 * S, tmem_slot = v_fixed + 8 * S, all_done = tmem_slot + 8;
     const uint32_t staged = (bars + 256 + 15u) & ~15u;      // 2 KB per softmax warp
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;      // (a warp's number, as something the whole warp has)
     if (threadIdx.x == 0) {
-        mbar_init(q_full, 1); mbar_init(q_empty, 1);
+        mbar_init(q_full, 1); mbar_init(q_empty, 1); mbar_init(all_done, 1);
         for (int x = 0; x < 2; x++) { mbar_init(s_full + 8 * x, 1); mbar_init(p_full + 16 * x, 4); mbar_init(p_full + 16 * x + 8, 4); mbar_init(o_done + 8 * x, 1); }
         for (int s = 0; s < S; s++) { mbar_init(k_full + 8 * s, 1); mbar_init(k_empty + 8 * s, 1); mbar_init(v_full + 8 * s, 1); mbar_init(v_empty + 8 * s, 1); mbar_init(v_fixed + 8 * s, 1); }
         mbar_init_fence();
@@ -395,7 +395,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention_prompt(const __grid_c
     } else if (warp == 8) {
         // ---- the copies ----
         const int box = min(kRows, 1 << a.c.page_shift), piece = lane / (D / 64), half = lane % (D / 64);
-        int stage = 0, units = 0;
+        int stage = 0, units = 0, begun = 0;      // begun: copies into the stage at hand (keys, then values)
         uint32_t phase = 0;
         while (unit_at < to && ok) {
             const Segment s = segment();
@@ -431,6 +431,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention_prompt(const __grid_c
                         if (lane == 0) mbar_arrive_expect_tx(full, uint32_t(used * box) * D * 2u);
                         __syncwarp();
                         if (piece < used) tma_load_3d((kv ? v_at : k_at) + at, kv ? &vmap : &kmap, half * 64, u.kvh, z, full);
+                        begun++;
                     }
                     if (!ok) break;
                     if (valid < kRows) {      // values behind the last key seen are zeros: a probability of zero times what a page may hold there has to stay zero
@@ -442,12 +443,20 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention_prompt(const __grid_c
                         }
                         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                         __syncwarp();
-                        if (lane == 0) mbar_arrive(v_fixed + 8 * stage);
+                        if (lane == 0 && ok) mbar_arrive(v_fixed + 8 * stage);
                     }
+                    if (!ok) break;
+                    begun = 0;
                     if (++stage == S) { stage = 0; phase ^= 1u; }
                 }
             }
             next_unit(s);
+        }
+        // no copy is under way when the block ends, not behind a wait that ran out either: the last queries, and each stage's last keys and values
+        if (units) ok = mbar_wait(q_full, uint32_t(units - 1) & 1u) && ok;
+        for (int s = 0; s < S; s++) {
+            ok = mbar_wait(k_full + 8 * s, s < stage || (s == stage && begun > 0) ? phase : phase ^ 1u) && ok;
+            ok = mbar_wait(v_full + 8 * s, s < stage || (s == stage && begun > 1) ? phase : phase ^ 1u) && ok;
         }
     } else if (warp == 9) {
         // ---- the MMAs: the whole warp walks the steps, so that what describes them stays uniform; one elected thread issues ----
@@ -537,6 +546,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention_prompt(const __grid_c
             }
             next_unit(s);
         }
+        // nor is a product, when the tensor memory is given back
+        const bool fine = ok;
+        commit(all_done);
+        ok = wait(all_done, 0u) && fine;
     } else {
         // ---- softmax: group x (four warps) has tile x, a thread has row r of it ----
         const int x = warp / 4, r = threadIdx.x % kRows;
