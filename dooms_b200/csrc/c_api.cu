@@ -164,32 +164,57 @@ struct SetUpUnderCapture {
     ~SetUpUnderCapture() { (void)cudaThreadExchangeStreamCaptureMode(&mode); }
 };
 
-// Every pointer has to be memory that kernels of the current device can use: a pointer of another device, or plain host memory, would fault in the kernel, and so would one
-// that is not on a 4-byte boundary.
-int32_t check_device(const char * what, std::initializer_list<const void *> pointers) {
-    for (const void * p : pointers) {
-        if (reinterpret_cast<uintptr_t>(p) & 3u) return fail(DOOMS_INVALID_ARGUMENT, std::string(what) + ": a pointer is not on a boundary of 4 bytes");
+// A piece of memory that a call reads or writes: `rows` rows of `bytes` bytes, `stride` bytes apart (one row: bytes in a piece). NULL: not there.
+struct Span {
+    const void * at;
+    int64_t bytes, rows = 1, stride = 0;
+    // Whether it has a byte in common with `other`, which has one row.
+    bool meets(const Span & other) const {
+        if (!at || !other.at || bytes <= 0 || other.bytes <= 0) return false;
+        const uintptr_t begin = reinterpret_cast<uintptr_t>(at), from = reinterpret_cast<uintptr_t>(other.at), to = from + uintptr_t(other.bytes);
+        if (to <= begin) return false;
+        if (from <= begin) return true;
+        // the row that begins at or in front of `from`, and the next one
+        const int64_t row = rows > 1 ? std::min(int64_t((from - begin) / uintptr_t(stride)), rows - 1) : 0;
+        const uintptr_t there = begin + uintptr_t(row * stride);
+        return from < there + uintptr_t(bytes) || (row + 1 < rows && to > there + uintptr_t(stride));
+    }
+};
+
+// Memory of a call over the paged cache, before its launch. A pointer of another device, or plain host memory, would fault in the kernel, and so would one that is not on a
+// 4-byte boundary: every pointer has to be memory that kernels of the current device can use. Blocks read while others write, so what is written (pieces of one row) may
+// meet neither what is read nor what else is written.
+int32_t check_memory(const char * what, std::initializer_list<Span> written, std::initializer_list<Span> read) {
+    for (const auto & spans : {written, read}) {
+        for (const Span & s : spans) {
+            if (reinterpret_cast<uintptr_t>(s.at) & 3u) return fail(DOOMS_INVALID_ARGUMENT, std::string(what) + ": a pointer is not on a boundary of 4 bytes");
+        }
+    }
+    for (const Span * w = written.begin(); w != written.end(); w++) {
+        bool meets = false;
+        for (const Span * o = w + 1; o != written.end(); o++) meets = meets || o->meets(*w);
+        for (const Span & r : read) meets = meets || r.meets(*w);
+        if (meets) return fail(DOOMS_INVALID_ARGUMENT, std::string(what) + ": memory that is written may not overlap what is read or what else is written");
     }
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) { (void)cudaGetLastError(); return fail(DOOMS_UNSUPPORTED, std::string(what) + ": no CUDA device"); }
-    for (const void * p : pointers) {
-        if (!p) continue;
-        cudaPointerAttributes at{};
-        const cudaError_t e = cudaPointerGetAttributes(&at, p);
-        if (e != cudaSuccess) { (void)cudaGetLastError(); return fail(DOOMS_UNSUPPORTED, std::string(what) + ": " + cudaGetErrorString(e)); }
-        const bool here = at.type == cudaMemoryTypeManaged || (at.type == cudaMemoryTypeDevice && at.device == dev) || (at.type == cudaMemoryTypeHost && at.devicePointer == p);
-        if (!here) return fail(DOOMS_INVALID_ARGUMENT, std::string(what) + ": a pointer is not memory of the current device");
+    for (const auto & spans : {written, read}) {
+        for (const Span & s : spans) {
+            if (!s.at) continue;
+            cudaPointerAttributes at{};
+            const cudaError_t e = cudaPointerGetAttributes(&at, s.at);
+            if (e != cudaSuccess) { (void)cudaGetLastError(); return fail(DOOMS_UNSUPPORTED, std::string(what) + ": " + cudaGetErrorString(e)); }
+            const bool here = at.type == cudaMemoryTypeManaged || (at.type == cudaMemoryTypeDevice && at.device == dev) || (at.type == cudaMemoryTypeHost && at.devicePointer == s.at);
+            if (!here) return fail(DOOMS_INVALID_ARGUMENT, std::string(what) + ": a pointer is not memory of the current device");
+        }
     }
     return DOOMS_OK;
 }
 
-// Whether two pieces of memory have a byte in common.
-bool overlap(const void * a, int64_t a_bytes, const void * b, int64_t b_bytes) {
-    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
-    return x < y + uintptr_t(b_bytes) && y < x + uintptr_t(a_bytes);
-}
-
 bool aligned16(const void * p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+Span pool_of(const void * at, const cuda::PagedCache & c) { return {at, int64_t(c.n_pages) * c.page_size * c.n_head_kv * c.head_dim * 2}; }
+Span table_of(const cuda::PagedCache & c) { return {c.page_table, int64_t(c.n_sequences) * c.max_pages * 4}; }
 
 constexpr int kMostGroup = 64;      // query heads per key / value head
 int32_t check_paged(const char * what, const dooms_cuda_paged_cache * c, int32_t n_head, cuda::PagedCache * out) {
@@ -927,11 +952,10 @@ DOOMS_CUDA_API int32_t dooms_cuda_rope_store_paged(const dooms_cuda_paged_cache 
     if (!d_qkv || !d_sequence || !d_at || !d_positions || !d_q || n_rows < 0 || qkv_stride < row || qkv_stride % 4 != 0 || !aligned16(d_qkv) || !aligned16(d_q)) {
         return fail(DOOMS_INVALID_ARGUMENT, "rope_store_paged: a NULL or unaligned pointer, a negative n_rows, or a qkv_stride that is no multiple of 4 or shorter than a row");
     }
-    if (overlap(d_q, int64_t(n_rows) * n_head * c.head_dim * (q_dtype == DOOMS_F16 ? 2 : 4), d_qkv, ((int64_t(n_rows) - 1) * qkv_stride + row) * 4)) {
-        return fail(DOOMS_INVALID_ARGUMENT, "rope_store_paged: d_q overlaps d_qkv");
-    }
     const SetUpUnderCapture relaxed;
-    code = check_device("rope_store_paged", {c.keys, c.values, c.page_table, d_qkv, d_sequence, d_at, d_positions, d_q});
+    const int64_t each = int64_t(n_rows) * 4;
+    code = check_memory("rope_store_paged", {{d_q, int64_t(n_rows) * n_head * c.head_dim * (q_dtype == DOOMS_F16 ? 2 : 4)}, pool_of(c.keys, c), pool_of(c.values, c)},
+                        {{d_qkv, row * 4, n_rows, qkv_stride * 4}, table_of(c), {d_sequence, each}, {d_at, each}, {d_positions, rope->n_axes * each}});
     if (code != DOOMS_OK) return code;
     return launch_result(cuda::launch_rope_store_paged(c, r, d_qkv, qkv_stride, n_head, n_rows, d_sequence, d_at, d_positions, d_q, q_dtype == DOOMS_F16, kernel_error_word(),
                                                        static_cast<cudaStream_t>(stream)), "rope_store_paged");
@@ -956,11 +980,10 @@ DOOMS_CUDA_API int32_t dooms_cuda_attention_paged(const dooms_cuda_paged_cache *
     }
     const int64_t needed = dooms_cuda_attention_paged_scratch_bytes(n_head, c.n_head_kv, c.head_dim), io = int64_t(n_rows) * n_head * c.head_dim * (dtype == DOOMS_F16 ? 2 : 4);
     if (scratch_bytes < needed) return fail(DOOMS_RESOURCE_EXHAUSTED, "attention_paged: the scratch is too small");
-    if (overlap(d_q, io, d_out, io) || overlap(d_scratch, needed, d_q, io) || overlap(d_scratch, needed, d_out, io)) {
-        return fail(DOOMS_INVALID_ARGUMENT, "attention_paged: d_q, d_out and d_scratch may not overlap");
-    }
     const SetUpUnderCapture relaxed;
-    code = check_device("attention_paged", {c.keys, c.values, c.page_table, d_q, d_sequence, d_lengths, d_out, d_scratch});
+    const int64_t each = int64_t(n_rows) * 4;
+    code = check_memory("attention_paged", {{d_out, io}, {d_scratch, needed}},
+                        {{d_q, io}, pool_of(c.keys, c), pool_of(c.values, c), table_of(c), {d_sequence, each}, {d_lengths, each}});
     if (code != DOOMS_OK) return code;
     return launch_result(cuda::launch_attention_paged(c, d_q, d_out, dtype == DOOMS_F16, n_head, n_rows, d_sequence, d_lengths, max_length,
                                                       scale > 0.f ? scale : 1.f / std::sqrt(float(c.head_dim)), d_scratch, kernel_error_word(), static_cast<cudaStream_t>(stream)),
@@ -980,11 +1003,10 @@ DOOMS_CUDA_API int32_t dooms_cuda_attention_prompt_paged(const dooms_cuda_paged_
     }
     const int64_t needed = dooms_cuda_attention_paged_scratch_bytes(n_head, c.n_head_kv, c.head_dim), io = int64_t(n_rows) * n_head * c.head_dim * 2;
     if (scratch_bytes < needed) return fail(DOOMS_RESOURCE_EXHAUSTED, "attention_prompt_paged: the scratch is too small");
-    if (overlap(d_q, io, d_out, io) || overlap(d_scratch, needed, d_q, io) || overlap(d_scratch, needed, d_out, io)) {
-        return fail(DOOMS_INVALID_ARGUMENT, "attention_prompt_paged: d_q, d_out and d_scratch may not overlap");
-    }
     const SetUpUnderCapture relaxed;
-    code = check_device("attention_prompt_paged", {c.keys, c.values, c.page_table, d_q, d_sequence, d_start, d_lengths, d_out, d_scratch});
+    const int64_t each = int64_t(n_prompts) * 4;
+    code = check_memory("attention_prompt_paged", {{d_out, io}, {d_scratch, needed}},
+                        {{d_q, io}, pool_of(c.keys, c), pool_of(c.values, c), table_of(c), {d_sequence, each}, {d_lengths, each}, {d_start, each + 4}});
     if (code != DOOMS_OK) return code;
     return launch_result(cuda::launch_attention_prompt_paged(c, d_q, d_out, n_head, n_rows, n_prompts, d_sequence, d_start, d_lengths,
                                                              scale > 0.f ? scale : 1.f / std::sqrt(float(c.head_dim)), d_scratch, kernel_error_word(),
@@ -1000,7 +1022,9 @@ DOOMS_CUDA_API int32_t dooms_cuda_sample_rows(const float * d_logits, int64_t st
     if (n > cuda::sample_rows_most()) return fail(DOOMS_UNSUPPORTED, "sample_rows: rows of at most " + std::to_string(cuda::sample_rows_most()) + " logits");
     if (rows > (1 << 24)) return fail(DOOMS_INVALID_ARGUMENT, "sample_rows: at most 2^24 rows");
     const SetUpUnderCapture relaxed;
-    const int32_t code = check_device("sample_rows", {d_logits, d_temperature, d_top_k, d_top_p, d_min_p, d_uniform, d_tokens, d_probability});
+    const int64_t each = int64_t(rows) * 4;
+    const int32_t code = check_memory("sample_rows", {{d_tokens, each}, {d_probability, each}},
+                                      {{d_logits, int64_t(n) * 4, rows, stride * 4}, {d_temperature, each}, {d_top_k, each}, {d_top_p, each}, {d_min_p, each}, {d_uniform, each}});
     if (code != DOOMS_OK) return code;
     return launch_result(cuda::launch_sample_rows(d_logits, stride, rows, n, d_temperature, d_top_k, d_top_p, d_min_p, d_uniform, d_tokens, d_probability,
                                                   static_cast<cudaStream_t>(stream)), "sample_rows");

@@ -12,7 +12,7 @@ import torch
 from dooms_b200 import _lib as L
 from dooms_b200 import build as B
 from dooms_b200 import paged
-from test_paged import Cache, cuda, status
+from test_paged import Cache, attention_code, chain, cuda, fake_cache, fake_rope, prompt_code, sample_code, status, store_code
 
 gpu = pytest.mark.gpu
 HERE = Path(__file__).resolve().parent
@@ -145,3 +145,98 @@ def test_calls_that_get_one_sm_beside_a_long_kernel(probes, heads, head_dim):
     torch.cuda.synchronize()
     assert status() == (L.OK, 0)
     assert torch.equal(out, alone) and torch.equal(pout.nan_to_num(5.0), palone.nan_to_num(5.0))
+
+
+# ---------------------------------------------------------------- memory that overlaps
+
+POOL = 10 * 16 * 2 * 64 * 2      # bytes of fake_cache's pools; its page table has 48
+BIG = 1 << 32
+
+
+def apart():
+    return fake_cache(keys=BIG, values=2 * BIG, page_table=3 * BIG)
+
+
+WRITTEN_AND_READ = [
+    # the entry, what is written (argument, bytes), and what it may not meet (argument or field of the cache, bytes)
+    (lambda **kw: store(**kw), {"q": 2 * 4 * 64 * 4, "keys": POOL, "values": POOL}, {"q": 2 * 4 * 64 * 4, "keys": POOL, "values": POOL, "qkv": 2 * 512 * 4, "page_table": 48, "seq": 8, "at": 8, "pos": 8}),
+    (lambda **kw: attend_one(**kw), {"out": 2 * 4 * 64 * 4, "scratch": None}, {"out": 2 * 4 * 64 * 4, "scratch": None, "q": 2 * 4 * 64 * 4, "keys": POOL, "values": POOL, "page_table": 48, "seq": 8, "lengths": 8}),
+    (lambda **kw: attend_prompt(**kw), {"out": 5 * 4 * 64 * 2, "scratch": None},
+     {"out": 5 * 4 * 64 * 2, "scratch": None, "q": 5 * 4 * 64 * 2, "keys": POOL, "values": POOL, "page_table": 48, "seq": 8, "start": 12, "lengths": 8}),
+    (lambda **kw: sample(**kw), {"tokens": 8, "prob": 8}, {"tokens": 8, "prob": 8, "logits": 800, "t": 8, "k": 8, "p": 8, "m": 8, "u": 8}),
+]
+
+
+def split(kw):
+    return apart_with({k: v for k, v in kw.items() if k in ("keys", "values", "page_table")}), {k: v for k, v in kw.items() if k not in ("keys", "values", "page_table")}
+
+
+def apart_with(fields):
+    c = apart()
+    for k, v in fields.items():
+        setattr(c, k, v)
+    return c
+
+
+def store(**kw):
+    c, kw = split(kw)
+    return store_code(c, fake_rope(), **({"qkv": 4 * BIG, "seq": 5 * BIG, "at": 6 * BIG, "pos": 7 * BIG, "q": 8 * BIG} | kw))
+
+
+def attend_one(**kw):
+    c, kw = split(kw)
+    return attention_code(c, **({"q": 4 * BIG, "seq": 5 * BIG, "lengths": 6 * BIG, "out": 7 * BIG, "scratch": 8 * BIG} | kw))
+
+
+def attend_prompt(**kw):
+    c, kw = split(kw)
+    return prompt_code(c, **({"q": 4 * BIG, "seq": 5 * BIG, "start": 9 * BIG, "lengths": 6 * BIG, "out": 7 * BIG, "scratch": 8 * BIG} | kw))
+
+
+def sample(**kw):
+    return sample_code(**({"logits": BIG, "t": 2 * BIG, "k": 3 * BIG, "p": 4 * BIG, "m": 5 * BIG, "u": 6 * BIG, "tokens": 7 * BIG, "prob": 8 * BIG} | kw))
+
+
+def overlaps(code):
+    return code == L.INVALID_ARGUMENT and b"overlap" in L.lib().dooms_cuda_last_error()
+
+
+@pytest.mark.parametrize("entry", range(4))
+def test_what_is_written_may_meet_nothing_else(entry):
+    """Every pair of a piece that a call writes and any other, by their first and by their last bytes; side by side they are fine (the refusal is another one then)."""
+    call, written, others = WRITTEN_AND_READ[entry]
+    scratch = L.lib().dooms_cuda_attention_paged_scratch_bytes(4, 2, 64)
+    assert not overlaps(call())
+    for w, w_bytes in written.items():
+        for o, o_bytes in others.items():
+            if w == o:
+                continue
+            w_size, o_size, at = w_bytes or scratch, o_bytes or scratch, 64 * BIG
+            # (on boundaries of 16 bytes, which some of them need)
+            for there in (at, at + (w_size - 1) // 16 * 16, at - (o_size - 1) // 16 * 16):
+                assert overlaps(call(**{w: at, o: there})), (w, o, there - at)
+            for there in (at + (w_size + 15) // 16 * 16, at - (o_size + 15) // 16 * 16):
+                assert not overlaps(call(**{w: at, o: there})), (w, o, there - at)
+
+
+def test_what_is_written_between_rows_meets_nothing():
+    """Rows that are further apart than they are long leave room between them, which belongs to no row."""
+    for tokens, meets in ((BIG + 400, False), (BIG + 396, True), (BIG + 632, False), (BIG + 636, True), (BIG + 640 + 400, False), (BIG - 8, False), (BIG - 4, True)):
+        assert overlaps(sample(logits=BIG, stride=160, tokens=tokens)) == meets, tokens - BIG
+    for q, meets in ((4 * BIG + 2048, False), (4 * BIG + 2032, True), (4 * BIG + 6144, True), (4 * BIG + 8192, False)):
+        assert overlaps(store(qkv=4 * BIG, stride=1024 + 512, q=q)) == meets, q - 4 * BIG
+
+
+@gpu
+def test_tokens_behind_each_row_of_logits():
+    """Logits with room behind every row, and outputs in the first rows' room: allowed, and what is there is what separate outputs get."""
+    g = np.random.default_rng(3)
+    rows, n = 6, 1000
+    buffer = torch.zeros(rows, 1024, device="cuda")
+    x, u = g.standard_normal((rows, n)).astype(np.float32) * 2, g.random(rows).astype(np.float32)
+    buffer[:, :n] = cuda(x)
+    tokens, prob = buffer[0, n + 4:n + 4 + rows].view(torch.int32), buffer[2, n + 4:n + 4 + rows]
+    paged.sample_rows(buffer[:, :n], cuda(u), tokens, prob)
+    assert tokens.tolist() == [chain(x[r], 1.0, 0, 1.0, 0.0, u[r])[0] for r in range(rows)] and (prob > 0).all()
+    with pytest.raises(L.DoomsError, match="overlap"):
+        paged.sample_rows(buffer[:, :n], cuda(u), buffer[3, n - rows:n].view(torch.int32))
