@@ -4,6 +4,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <cstddef>
 #include <cstring>
@@ -115,14 +116,18 @@ Status scratch_for(size_t bytes, void ** out) {
 
 // The error word of the single-kernel entry points: kernels with bounded waits (tensor copies, mbarriers) set it instead of waiting for ever. One word of
 // mapped pinned host memory per process, never freed, read and cleared by dooms_cuda_kernel_status.
+// NULL: it could not be allocated now (the first call may have come under a capture, which forbids it, or without memory left); the next call tries again.
+std::mutex g_error_word_mutex;
 int32_t * kernel_error_word() {
-    static int32_t * word = [] {
-        int32_t * w = nullptr;
-        if (cudaHostAlloc(reinterpret_cast<void **>(&w), 64, cudaHostAllocMapped | cudaHostAllocPortable) != cudaSuccess) { (void)cudaGetLastError(); return static_cast<int32_t *>(nullptr); }
-        *w = 0;
-        return w;
-    }();
-    return word;
+    static std::atomic<int32_t *> word{nullptr};
+    int32_t * w = word.load(std::memory_order_acquire);
+    if (w) return w;
+    std::lock_guard<std::mutex> lock(g_error_word_mutex);
+    if ((w = word.load(std::memory_order_relaxed))) return w;
+    if (cudaHostAlloc(reinterpret_cast<void **>(&w), 64, cudaHostAllocMapped | cudaHostAllocPortable) != cudaSuccess) { (void)cudaGetLastError(); return nullptr; }
+    std::memset(w, 0, 64);
+    word.store(w, std::memory_order_release);
+    return w;
 }
 
 int32_t launch_result(cudaError_t e, const char * what) {
@@ -215,6 +220,9 @@ bool aligned16(const void * p) { return (reinterpret_cast<uintptr_t>(p) & 15u) =
 
 Span pool_of(const void * at, const cuda::PagedCache & c) { return {at, int64_t(c.n_pages) * c.page_size * c.n_head_kv * c.head_dim * 2}; }
 Span table_of(const cuda::PagedCache & c) { return {c.page_table, int64_t(c.n_sequences) * c.max_pages * 4}; }
+
+// Out-of-range entries and waits that run out are only known by the error word, so nothing is launched without one.
+int32_t no_error_word(const char * what) { return fail(DOOMS_RESOURCE_EXHAUSTED, std::string(what) + ": could not allocate the kernel error word"); }
 
 constexpr int kMostGroup = 64;      // query heads per key / value head
 int32_t check_paged(const char * what, const dooms_cuda_paged_cache * c, int32_t n_head, cuda::PagedCache * out) {
@@ -957,7 +965,9 @@ DOOMS_CUDA_API int32_t dooms_cuda_rope_store_paged(const dooms_cuda_paged_cache 
     code = check_memory("rope_store_paged", {{d_q, int64_t(n_rows) * n_head * c.head_dim * (q_dtype == DOOMS_F16 ? 2 : 4)}, pool_of(c.keys, c), pool_of(c.values, c)},
                         {{d_qkv, row * 4, n_rows, qkv_stride * 4}, table_of(c), {d_sequence, each}, {d_at, each}, {d_positions, rope->n_axes * each}});
     if (code != DOOMS_OK) return code;
-    return launch_result(cuda::launch_rope_store_paged(c, r, d_qkv, qkv_stride, n_head, n_rows, d_sequence, d_at, d_positions, d_q, q_dtype == DOOMS_F16, kernel_error_word(),
+    int32_t * const err = kernel_error_word();
+    if (!err) return no_error_word("rope_store_paged");
+    return launch_result(cuda::launch_rope_store_paged(c, r, d_qkv, qkv_stride, n_head, n_rows, d_sequence, d_at, d_positions, d_q, q_dtype == DOOMS_F16, err,
                                                        static_cast<cudaStream_t>(stream)), "rope_store_paged");
 }
 
@@ -985,8 +995,10 @@ DOOMS_CUDA_API int32_t dooms_cuda_attention_paged(const dooms_cuda_paged_cache *
     code = check_memory("attention_paged", {{d_out, io}, {d_scratch, needed}},
                         {{d_q, io}, pool_of(c.keys, c), pool_of(c.values, c), table_of(c), {d_sequence, each}, {d_lengths, each}});
     if (code != DOOMS_OK) return code;
+    int32_t * const err = kernel_error_word();
+    if (!err) return no_error_word("attention_paged");
     return launch_result(cuda::launch_attention_paged(c, d_q, d_out, dtype == DOOMS_F16, n_head, n_rows, d_sequence, d_lengths, max_length,
-                                                      scale > 0.f ? scale : 1.f / std::sqrt(float(c.head_dim)), d_scratch, kernel_error_word(), static_cast<cudaStream_t>(stream)),
+                                                      scale > 0.f ? scale : 1.f / std::sqrt(float(c.head_dim)), d_scratch, err, static_cast<cudaStream_t>(stream)),
                          "attention_paged");
 }
 
@@ -1008,8 +1020,10 @@ DOOMS_CUDA_API int32_t dooms_cuda_attention_prompt_paged(const dooms_cuda_paged_
     code = check_memory("attention_prompt_paged", {{d_out, io}, {d_scratch, needed}},
                         {{d_q, io}, pool_of(c.keys, c), pool_of(c.values, c), table_of(c), {d_sequence, each}, {d_lengths, each}, {d_start, each + 4}});
     if (code != DOOMS_OK) return code;
+    int32_t * const err = kernel_error_word();
+    if (!err) return no_error_word("attention_prompt_paged");
     return launch_result(cuda::launch_attention_prompt_paged(c, d_q, d_out, n_head, n_rows, n_prompts, d_sequence, d_start, d_lengths,
-                                                             scale > 0.f ? scale : 1.f / std::sqrt(float(c.head_dim)), d_scratch, kernel_error_word(),
+                                                             scale > 0.f ? scale : 1.f / std::sqrt(float(c.head_dim)), d_scratch, err,
                                                              static_cast<cudaStream_t>(stream)), "attention_prompt_paged");
 }
 

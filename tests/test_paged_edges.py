@@ -2,6 +2,7 @@
 just not allowed. The plain forms and helpers are test_paged.py's."""
 import ctypes as C
 import subprocess
+import sys
 import time
 from pathlib import Path
 
@@ -240,3 +241,39 @@ def test_tokens_behind_each_row_of_logits():
     assert tokens.tolist() == [chain(x[r], 1.0, 0, 1.0, 0.0, u[r])[0] for r in range(rows)] and (prob > 0).all()
     with pytest.raises(L.DoomsError, match="overlap"):
         paged.sample_rows(buffer[:, :n], cuda(u), buffer[3, n - rows:n].view(torch.int32))
+
+
+# ---------------------------------------------------------------- the error word
+
+@gpu
+def test_a_bad_page_is_reported_after_a_call_that_could_not_allocate_the_error_word():
+    """A process whose first call needs the word under a capture, which forbids its allocation: that call fails, and the word is there for the next one."""
+    code = """
+import ctypes as C
+import torch
+from dooms_b200 import _lib as L
+from dooms_b200 import paged
+w, x, y = torch.zeros(6145 * 4096 // 32 * 18, dtype=torch.uint8, device="cuda"), torch.zeros(4096, device="cuda"), torch.zeros(6145, device="cuda")
+keys, values = (torch.randn(8, 16, 2, 64, device="cuda").half() for _ in range(2))
+cache = paged.PagedCache(keys, values, torch.full((2, 4), 99, dtype=torch.int32, device="cuda"))
+scratch = torch.empty(cache.scratch_bytes(4), dtype=torch.uint8, device="cuda")
+seq, lengths = torch.arange(2, dtype=torch.int32, device="cuda"), torch.full((2,), 20, dtype=torch.int32, device="cuda")
+q, out = (torch.zeros(2, 4, 64, device="cuda") for _ in range(2))
+torch.cuda.synchronize()
+stream, graph, first = torch.cuda.Stream(), torch.cuda.CUDAGraph(), None
+with torch.cuda.stream(stream):
+    graph.capture_begin()
+    first = L.lib().dooms_cuda_matvec(L.Q4_0, w.data_ptr(), x.data_ptr(), y.data_ptr(), None, 6145, 4096, 0, stream.cuda_stream)
+    try:
+        graph.capture_end()
+    except RuntimeError as e:
+        print("capture:", e)
+torch.cuda.synchronize()
+print("first:", first)
+assert first != L.OK
+cache.attention(q, seq, lengths, 64, out, scratch)
+flag = C.c_int32()
+print("status:", L.lib().dooms_cuda_kernel_status(None, C.byref(flag)), flag.value)
+"""
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300, cwd=HERE.parent)
+    assert r.returncode == 0 and f"status: {L.INTERNAL} 8" in r.stdout, r.stdout[-2000:] + r.stderr[-2000:]
