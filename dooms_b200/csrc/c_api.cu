@@ -114,8 +114,8 @@ Status scratch_for(size_t bytes, void ** out) {
     return Status();
 }
 
-// The error word of the single-kernel entry points: kernels with bounded waits (tensor copies, mbarriers) set it instead of waiting for ever. One word of
-// mapped pinned host memory per process, never freed, read and cleared by dooms_cuda_kernel_status.
+// The error words of the single-kernel entry points: kernels with bounded waits (tensor copies, mbarriers) set the first instead of waiting for ever, the paged operators'
+// kernels two of their own behind it. Mapped pinned host memory of the process, never freed, read and cleared by dooms_cuda_kernel_status.
 // NULL: it could not be allocated now (the first call may have come under a capture, which forbids it, or without memory left); the next call tries again.
 std::mutex g_error_word_mutex;
 int32_t * kernel_error_word() {
@@ -223,6 +223,21 @@ Span table_of(const cuda::PagedCache & c) { return {c.page_table, int64_t(c.n_se
 
 // Out-of-range entries and waits that run out are only known by the error word, so nothing is launched without one.
 int32_t no_error_word(const char * what) { return fail(DOOMS_RESOURCE_EXHAUSTED, std::string(what) + ": could not allocate the kernel error word"); }
+
+// What dooms_cuda_kernel_status says of the flags it found, every one of them.
+int32_t kernel_errors(int32_t seen) {
+    if (seen == 0) return DOOMS_OK;
+    std::string message;
+    const int32_t waits = seen & ~cuda::kErrorPaged, other = waits & ~cuda::kErrorPagedWait;
+    if (waits) {
+        message = "a kernel gave up a bounded wait (flag " + std::to_string(waits) + (other == 2 ? ": matmul" : other == 4 ? ": matvec / gate_up tensor copy" : "") +
+                  (waits != other ? ": attention over pages" : "") + "); its output is not valid";
+    }
+    if (seen & cuda::kErrorPaged) {
+        message += std::string(message.empty() ? "" : "; ") + "a page id, sequence, position or length of a paged cache call was out of range (flag 8); the output of its row is not valid";
+    }
+    return fail(DOOMS_INTERNAL, message);
+}
 
 constexpr int kMostGroup = 64;      // query heads per key / value head
 int32_t check_paged(const char * what, const dooms_cuda_paged_cache * c, int32_t n_head, cuda::PagedCache * out) {
@@ -863,13 +878,10 @@ DOOMS_CUDA_API int32_t dooms_cuda_kernel_status(void * stream, int32_t * flag) {
     const cudaError_t e = cudaStreamSynchronize(static_cast<cudaStream_t>(stream));
     if (e != cudaSuccess) return launch_result(e, "kernel_status");
     int32_t * err = kernel_error_word();
-    const int32_t seen = err ? *err : 0;
-    if (err) *err = 0;
+    int32_t seen = 0;
+    for (int i = 0; err && i < cuda::kErrorWords; i++) seen |= __atomic_exchange_n(err + i, 0, __ATOMIC_RELAXED);
     if (flag) *flag = seen;
-    if (seen == 0) return DOOMS_OK;
-    if (seen == cuda::kErrorPaged) return fail(DOOMS_INTERNAL, "a page id, sequence, position or length of a paged cache call was out of range (flag 8); the output of its row is not valid");
-    return fail(DOOMS_INTERNAL, "a kernel gave up a bounded wait (flag " + std::to_string(seen) + (seen == 2 ? ": matmul" : seen == 4 ? ": matvec / gate_up tensor copy" : "") +
-                                    "); its output is not valid");
+    return kernel_errors(seen);
 }
 
 DOOMS_CUDA_API int32_t dooms_cuda_rms_norm(const float * d_x, const float * d_gamma, float * d_out, int64_t rows, int64_t cols, float eps, void * stream) {

@@ -496,7 +496,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) k_attention_paged(cons
             if (left > 0) next_item();
         }
     }
-    if (!ok && lane == 0 && a.c.error) *reinterpret_cast<volatile int *>(a.c.error) = kErrorPagedWait;
+    if (!ok && lane == 0) a.c.gave_up();
 }
 
 template <int D, bool HALF, bool WIDE>

@@ -836,7 +836,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention_prompt(const __grid_c
             next_unit(s);
         }
     }
-    if (!ok && lane == 0 && a.c.error) *reinterpret_cast<volatile int *>(a.c.error) = kErrorPagedWait;
+    if (!ok && lane == 0) a.c.gave_up();
     // ---- what is out of range is reported, queries that see nothing are zero ----
     for (int i = blockIdx.x; i < a.n_prompts; i += gridDim.x) {
         bool bad = false;

@@ -277,8 +277,10 @@ cudaError_t launch_add_shares(float * x, const float * shares, int k_splits, int
 
 // ---- a serving step over a key / value cache in pages ----
 // Pools of f16 [n_pages][page_size][n_head_kv][head_dim] (page_size a power of two from 16, head_dim 64 or 128) and the page ids of every sequence. Ids, sequences,
-// positions and lengths are read on the device; one that is out of range is not followed: its row is skipped and *error becomes 8.
-constexpr int kErrorPaged = 8, kErrorPagedWait = 16;      // (16: a bounded wait of the attention kernels ran out)
+// positions and lengths are read on the device; one that is out of range is not followed: its row is skipped and error[1] becomes 8.
+// (error: words of their own behind the one that the other kernels set, so that no flag takes another's place: [1] kErrorPaged, [2] kErrorPagedWait, a bounded wait of the
+// attention kernels that ran out)
+constexpr int kErrorPaged = 8, kErrorPagedWait = 16, kErrorWords = 3;
 struct PagedCache {
     void * keys, * values;
     const int32_t * page_table;       // [n_sequences][max_pages]

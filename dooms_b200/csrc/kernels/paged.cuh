@@ -1,6 +1,6 @@
 #pragma once
 // A key / value cache in pages, as the kernels see it: pools of f16 [n_pages][page_size][n_kv][D] and a table of page ids per sequence. Every id, sequence and
-// position that a kernel takes from device memory is checked before an address is made of it; what fails is skipped and reported through the error word.
+// position that a kernel takes from device memory is checked before an address is made of it; what fails is skipped and reported through the error words.
 #include <cuda_fp16.h>
 
 #include <atomic>
@@ -16,9 +16,10 @@ struct PagedView {
     __half * k, * v;
     const int32_t * table;        // [n_sequences][max_pages]
     int n_pages, page_shift, n_sequences, max_pages, n_kv;
-    int * error;
+    int * error;                  // kErrorWords of them
 
-    __device__ __forceinline__ void fail() const { if (error) *reinterpret_cast<volatile int *>(error) = kErrorPaged; }
+    __device__ __forceinline__ void fail() const { reinterpret_cast<volatile int *>(error)[1] = kErrorPaged; }
+    __device__ __forceinline__ void gave_up() const { reinterpret_cast<volatile int *>(error)[2] = kErrorPagedWait; }
     // Positions a sequence can have: its pages, kept inside 32 bits.
     __device__ __forceinline__ int capacity() const { return int(min(int64_t(max_pages) << page_shift, int64_t(0x7fffff00))); }
     // The pool's row (of n_kv * D values) of position `at` of sequence `seq`, both in range; -1: the page is not one.

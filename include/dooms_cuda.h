@@ -222,8 +222,8 @@ DOOMS_CUDA_API int32_t dooms_cuda_matmul(int32_t dtype, const void * d_w, const 
                                          int32_t tokens, int64_t rows, int64_t cols, uint32_t flags, void * stream);
 /* No counterpart in the reference (Metal command buffers report their own errors). The matvec / gate_up / matmul kernels above wait for their tensor copies
  * and tensor-core stages with a limit; a wait that runs out sets a process-wide error word instead of hanging the GPU, and the kernel's output is then
- * not valid. This call waits for `stream`, reads the word into *flag (may be NULL; 0: none, 2: matmul, 4: matvec / gate_up, 8: an entry of a paged cache call out of range,
- * 16: a wait of attention_paged / attention_prompt_paged) and clears it; it returns
+ * not valid. This call waits for `stream`, reads the word into *flag (may be NULL; 0: none, 2: matmul, 4: matvec / gate_up, and beside them, added up, 8: an entry of a paged
+ * cache call out of range, 16: a wait of attention_paged / attention_prompt_paged) and clears it; it returns
  * DOOMS_OK when the word was 0 and DOOMS_INTERNAL otherwise. */
 DOOMS_CUDA_API int32_t dooms_cuda_kernel_status(void * stream, int32_t * flag);
 /* norm_vec (llama_kernels.h:1272-1286): xn = x * rsqrt(mean(x^2) + eps) * gamma for `rows` rows of `cols`. */

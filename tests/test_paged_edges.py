@@ -277,3 +277,28 @@ print("status:", L.lib().dooms_cuda_kernel_status(None, C.byref(flag)), flag.val
 """
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300, cwd=HERE.parent)
     assert r.returncode == 0 and f"status: {L.INTERNAL} 8" in r.stdout, r.stdout[-2000:] + r.stderr[-2000:]
+
+
+@gpu
+def test_a_flag_takes_no_other_flags_place():
+    """A page out of range is noted behind what other kernels have noted, and read and cleared with it."""
+    objects = [B.OBJ / (str(src.relative_to(B.CSRC)).replace("/", "_") + ".o") for src in B.sources() if src.parent.name == "kernels"]
+    if not all(o.exists() for o in objects):
+        B.build()
+    source, out = HERE / "paged_entries.cpp", HERE / "_build" / "libpaged_entries.so"
+    if not out.exists() or out.stat().st_mtime < max(p.stat().st_mtime for p in [source, *objects]):
+        out.parent.mkdir(exist_ok=True)
+        subprocess.run([B.nvcc(), *B.NVCC_FLAGS, "-shared", "-x", "cu", str(source), *[f"-Xlinker={o}" for o in objects], "-o", str(out), "-ldl"], check=True, capture_output=True)
+    entry = C.CDLL(str(out)).paged_entry_rope_store
+    P, I = C.c_void_p, C.c_int
+    entry.argtypes = [P, P, P, I, I, I, I, I, I, P, I, I, P, P, P, P, P]
+    cache = Cache([40, 40], 2, 64, fill=0.0)
+    cache.table[1, 2] = -1
+    cache.upload()
+    seq, at = cuda(np.array([0, 1], np.int32)), cuda(np.array([3, 39], np.int32))
+    qkv, q = torch.randn(2, 8 * 64, device="cuda"), torch.zeros(2, 4, 64, device="cuda")
+    error = torch.tensor([2, 0, 16, 0], dtype=torch.int32).pin_memory()
+    assert entry(cache.keys.data_ptr(), cache.values.data_ptr(), cache.d_table.data_ptr(), cache.keys.shape[0], 16, 2, cache.table.shape[1], 2, 64, qkv.data_ptr(), 4, 2, seq.data_ptr(),
+                 at.data_ptr(), at.data_ptr(), q.data_ptr(), error.data_ptr()) == 0
+    torch.cuda.synchronize()
+    assert error.tolist() == [2, 8, 16, 0]
