@@ -426,7 +426,8 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const SampleArgs a)
     const bool wide = (reinterpret_cast<uintptr_t>(from) & 15u) == 0;
     const float t = a.temperature ? a.temperature[row] : 1.f, top_p = a.top_p ? a.top_p[row] : 1.f, min_p = a.min_p ? a.min_p[row] : 0.f, uniform = a.uniform[row];
     const int k = a.top_k ? a.top_k[row] : 0;
-    const bool greedy = !(t > 0.f), by_k = k > 0 && k < a.n, by_p = top_p < 1.f, by_m = min_p > 0.f;
+    // (a min-p above 1 is reached by no token: the first alone is kept, as of a temperature of 0)
+    const bool greedy = !(t > 0.f) || min_p > 1.f, by_k = k > 0 && k < a.n, by_p = top_p < 1.f, by_m = min_p > 0.f;
     // open: a total of everything is needed. sampled: what is listed there, and for a top-k of more than there are threads, is what lies above the least of the warps' m-th
     // largest of the threads' largest of kSamples logits each: a share of the row that does not depend on what its logits are like.
     const bool open = !greedy && !by_k && (by_p || !by_m), sampled = open || (!greedy && by_k && k > kThreads), bounded = !greedy && (open || by_k);
@@ -504,7 +505,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const SampleArgs a)
         if (top == CUDART_INF_F) {
             least = top;      // an infinity takes all
         } else if (by_m) {
-            const double limit = min_p >= 1.f ? 0.0 : -log(double(min_p));
+            const double limit = min_p == 1.f ? 0.0 : -log(double(min_p));
             least = __double2float_ru(double(top) - limit);
             while (r.gap(least) > limit) least = nextafterf(least, CUDART_INF_F);
         }

@@ -298,7 +298,8 @@ DOOMS_CUDA_API int32_t dooms_cuda_attention_prompt_paged(const dooms_cuda_paged_
 /* One token per row of n logits (rows `stride` floats apart), as dooms_cuda_sample's chain picks it, from given random numbers d_uniform[r] in [0, 1): in the order (logit
  * descending, index ascending) the first d_top_k[r] (0 or less: all), then the shortest run whose probability reaches d_top_p[r] (1 or more: all), then those of at
  * least d_min_p[r] times the largest probability (0 or less: all), probabilities being those at temperature 1; then the first whose cumulative probability at temperature
- * d_temperature[r] exceeds d_uniform[r]. At least one token is kept. temperature <= 0: the largest logit. A NaN is never picked, nor a logit of -inf; a row that has
+ * d_temperature[r] exceeds d_uniform[r]. At least one token, the first, is kept (a min-p above 1 keeps it
+ * alone). temperature <= 0: the largest logit. A NaN is never picked, nor a logit of -inf; a row that has
  * nothing else gives its first number (0: none) with probability 0. NULL: temperature 1, top-k, top-p and min-p off. d_probability (may be NULL): the token's
  * probability among those kept. n at most 262144. */
 DOOMS_CUDA_API int32_t dooms_cuda_sample_rows(const float * d_logits, int64_t stride, int32_t rows, int32_t n, const float * d_temperature, const int32_t * d_top_k,

@@ -13,7 +13,7 @@ import torch
 from dooms_b200 import _lib as L
 from dooms_b200 import build as B
 from dooms_b200 import paged
-from test_paged import Cache, attention_code, chain, cuda, fake_cache, fake_rope, prompt_code, sample_code, status, store_code
+from test_paged import Cache, attention_code, chain, check_sample, cuda, fake_cache, fake_rope, prompt_code, sample_code, status, store_code
 
 gpu = pytest.mark.gpu
 HERE = Path(__file__).resolve().parent
@@ -49,6 +49,21 @@ def test_what_follows_the_sampling_sees_its_tokens(probes, rows, n):
         assert probes.probe_copy_at_once(tokens.data_ptr(), seen.data_ptr(), rows, stream.cuda_stream) == 0
         torch.cuda.synchronize()
         assert (tokens >= 0).all() and torch.equal(tokens, seen)
+
+
+# ---------------------------------------------------------------- sampling
+
+@gpu
+@pytest.mark.parametrize("n", [5, 3000, 151936])
+def test_a_min_p_above_one_keeps_the_first_alone(n):
+    """None of the tokens reaches more than the largest probability, so the first of them, and it alone, is kept: of equal largest logits the one in front, whatever the other
+    filters and the random number. A min-p of 1 keeps all of the largest."""
+    g = np.random.default_rng(n)
+    x = g.standard_normal((16, n)).astype(np.float32)
+    x[:, g.integers(0, n, 4)] = 9.0
+    x[3], x[5, n // 2] = 0.25, np.inf
+    m = np.array([1.0, np.nextafter(np.float32(1), np.float32(2)), 1.5, 7.0, np.inf, 1.25, 1.0, 2.0] * 2, np.float32)
+    check_sample(x, np.array([1.0, 0.7] * 8), np.array([0, 0, 40, 2] * 4), np.array([1.0] * 8 + [0.9] * 8), m, g.random(16))
 
 
 # ---------------------------------------------------------------- the counters in the scratch
