@@ -1,6 +1,6 @@
 """Python face of the operators of a serving step over a key / value cache in pages (include/dooms_cuda.h: dooms_cuda_paged_cache): rotary positions with the cache
 write, attention of single tokens and of packed prompts over the pages, and sampling. Tensors are device tensors (torch's); outputs are written in place and nothing is
-allocated. `stream` is a cudaStream_t as an integer (0: the default stream)."""
+allocated. `stream` is a cudaStream_t as an integer (0: the default stream); without one a call goes to torch's current stream, as the tensors' own work does."""
 from __future__ import annotations
 
 import ctypes as C
@@ -35,6 +35,12 @@ def _scratch(t) -> tuple[int, int]:
     return t.data_ptr(), t.numel() * t.element_size()
 
 
+def _stream(stream: int | None) -> int:
+    if stream is None:      # (where torch has not begun to use a GPU there is no other stream than the default one)
+        return torch.cuda.current_stream().cuda_stream if torch.cuda.is_initialized() else 0
+    return stream
+
+
 class PagedCache:
     """Pools of keys and values, f16 [n_pages][page_size][n_head_kv][head_dim], and the pages of every sequence, int32 [n_sequences][max_pages]. The object refers to the
     tensors' memory (and keeps them alive); their contents may change between calls, the page table's too."""
@@ -58,7 +64,7 @@ class PagedCache:
             raise L.DoomsError(L.INVALID_ARGUMENT, f"{n_head} query heads on {self._c.n_head_kv} key / value heads of {self._c.head_dim}")
         return n
 
-    def rope_store(self, qkv, sequence, at, positions, q, base: float, neox: bool, sections: Sequence[int] | None = None, stream: int = 0) -> None:
+    def rope_store(self, qkv, sequence, at, positions, q, base: float, neox: bool, sections: Sequence[int] | None = None, stream: int | None = None) -> None:
         """Rows [n][(n_head + 2 n_head_kv) head_dim] of f32 (rows may be further apart): turned queries into q [n][n_head][head_dim] (f32 or f16), turned keys and the values
         into position at[r] of sequence[r] (negative: an idle row). positions: int32 [n_axes][n]; sections: rotary pairs per axis (one axis: all of them)."""
         c, (n, n_head, head_dim) = self._c, q.shape
@@ -73,26 +79,26 @@ class PagedCache:
         stride = qkv.stride(0) if n > 1 else qkv.shape[1]
         L.check(L.lib().dooms_cuda_rope_store_paged(self._ref, C.byref(rope), qkv.data_ptr(), stride, n_head, n, _pointer("sequence", sequence, _I32, (n,)),
                                                     _pointer("at", at, _I32, (n,)), _pointer("positions", positions, _I32, (len(sections), n)),
-                                                    _dtype("q", q), _pointer("q", q, q.dtype, (n, n_head, c.head_dim)), stream))
+                                                    _dtype("q", q), _pointer("q", q, q.dtype, (n, n_head, c.head_dim)), _stream(stream)))
 
-    def attention(self, q, sequence, lengths, max_length: int, out, scratch, scale: float = 0.0, stream: int = 0) -> None:
+    def attention(self, q, sequence, lengths, max_length: int, out, scratch, scale: float = 0.0, stream: int | None = None) -> None:
         """One new token per row: q, out [n][n_head][head_dim], both f32 or both f16; row r sees the first lengths[r] <= max_length positions of sequence[r]."""
         n, n_head = q.shape[0], q.shape[1]
         shape = (n, n_head, self._c.head_dim)
         L.check(L.lib().dooms_cuda_attention_paged(self._ref, _dtype("q", q), _pointer("q", q, q.dtype, shape), _pointer("sequence", sequence, _I32, (n,)),
                                                    _pointer("lengths", lengths, _I32, (n,)), max_length, _pointer("out", out, q.dtype, shape), n_head, n, scale,
-                                                   *_scratch(scratch), stream))
+                                                   *_scratch(scratch), _stream(stream)))
 
-    def attention_prompt(self, q, sequence, start, lengths, out, scratch, scale: float = 0.0, stream: int = 0) -> None:
+    def attention_prompt(self, q, sequence, start, lengths, out, scratch, scale: float = 0.0, stream: int | None = None) -> None:
         """Packed prompts, causal: q, out f16 [rows][n_head][head_dim]; prompt i has rows start[i] .. start[i + 1] - 1, the last of lengths[i] positions of sequence[i]."""
         rows, n_head = q.shape[0], q.shape[1]
         shape, n = (rows, n_head, self._c.head_dim), sequence.shape[0]
         L.check(L.lib().dooms_cuda_attention_prompt_paged(self._ref, _pointer("q", q, _F16, shape), _pointer("sequence", sequence, _I32, (n,)),
                                                           _pointer("start", start, _I32, (n + 1,)), _pointer("lengths", lengths, _I32, (n,)),
-                                                          _pointer("out", out, _F16, shape), n_head, n, rows, scale, *_scratch(scratch), stream))
+                                                          _pointer("out", out, _F16, shape), n_head, n, rows, scale, *_scratch(scratch), _stream(stream)))
 
 
-def sample_rows(logits, uniform, tokens, probability=None, temperature=None, top_k=None, top_p=None, min_p=None, stream: int = 0) -> None:
+def sample_rows(logits, uniform, tokens, probability=None, temperature=None, top_k=None, top_p=None, min_p=None, stream: int | None = None) -> None:
     """tokens[r] (int32) from logits [rows][n] (f32; rows may be further apart) and uniform[r] in [0, 1); the filters are f32 (top_k: int32) tensors of one value per row, or
     None for off (temperature: 1). See dooms_cuda_sample_rows."""
     rows, n = logits.shape
@@ -103,4 +109,4 @@ def sample_rows(logits, uniform, tokens, probability=None, temperature=None, top
         return None if t is None else _pointer(name, t, dtype, (rows,))
     L.check(L.lib().dooms_cuda_sample_rows(logits.data_ptr(), logits.stride(0) if rows > 1 else n, rows, n, row("temperature", temperature), row("top_k", top_k, _I32),
                                            row("top_p", top_p), row("min_p", min_p), row("uniform", uniform), row("tokens", tokens, _I32), row("probability", probability),
-                                           stream))
+                                           _stream(stream)))

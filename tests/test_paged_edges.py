@@ -117,6 +117,54 @@ def test_counters_are_zero_behind_a_call_and_behind_its_replays():
     assert status() == (L.OK, 0)
 
 
+# ---------------------------------------------------------------- streams
+
+def test_where_torch_has_no_gpu_the_default_stream_is_meant():
+    if not torch.cuda.is_available():
+        assert paged._stream(None) == 0
+    assert paged._stream(0) == 0 and paged._stream(77) == 77
+
+
+@gpu
+def test_calls_without_a_stream_go_to_torchs_current_one(probes):
+    """Under torch.cuda.stream, with tensors that the stream's own work makes (behind half a second of something else) and reads; and captured, as part of the graph."""
+    H, K, D, V = 8, 2, 64, 5000
+    cache = Cache([100, 40], K, D, 16, fill=0.0)
+    scratch, seq = cache.scratch(H), torch.arange(2, dtype=torch.int32, device="cuda")
+    lengths, start = cuda(np.array([100, 40], np.int32)), cuda(np.array([0, 5, 12], np.int32))
+    made = [torch.randn(2, (H + 2 * K) * D, device="cuda"), torch.randn(12, H, D, device="cuda").half(), torch.randn(2, V, device="cuda")]
+    u = torch.rand(2, device="cuda")
+
+    def run(inputs):
+        qkv, pq, logits = inputs
+        q, out, pout, tokens = torch.zeros(2, H, D, device="cuda"), torch.zeros(2, H, D, device="cuda"), torch.zeros_like(pq), torch.zeros(2, dtype=torch.int32, device="cuda")
+        cache.cache.rope_store(qkv, seq, lengths - 1, (lengths - 1)[None], q, base=1e4, neox=True)
+        cache.cache.attention(q, seq, lengths, 100, out, scratch)
+        cache.cache.attention_prompt(pq, seq, start, lengths, pout, scratch)
+        paged.sample_rows(logits, u, tokens)
+        return [t.clone() for t in (q, out, pout, tokens)]
+    want = run(made)
+    torch.cuda.synchronize()
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        inputs = [torch.zeros_like(t) for t in made]
+        torch.cuda.synchronize()
+        assert probes.probe_hold(1, 500_000_000, stream.cuda_stream) == 0
+        for t, m in zip(inputs, made):
+            t.copy_(m)
+        got = run(inputs)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = run(inputs)
+    for t in captured:
+        t.zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(want, captured)) and status() == (L.OK, 0)
+
+
 # ---------------------------------------------------------------- beside other work
 
 @gpu
