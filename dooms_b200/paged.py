@@ -21,6 +21,15 @@ def _pointer(name: str, t, dtype, shape: tuple) -> int:
     return t.data_ptr()
 
 
+_MOST = (1 << 31) - 1
+
+
+def _int32(name: str, *values: int) -> None:
+    """That the values fit the C arguments, which would take the low 32 bits of one that does not."""
+    if not all(-_MOST <= v <= _MOST for v in values):
+        raise L.DoomsError(L.INVALID_ARGUMENT, f"{name}: {values} does not fit 32 bits")
+
+
 def _dtype(name: str, t) -> int:
     dt = _DTYPES.get(t.dtype)
     if dt is None:
@@ -49,6 +58,7 @@ class PagedCache:
         if len(keys.shape) != 4 or len(page_table.shape) != 2:
             raise L.DoomsError(L.INVALID_ARGUMENT, "pools of four dimensions and a page table of two expected")
         n_pages, page_size, n_head_kv, head_dim = keys.shape
+        _int32("pools and page table", *keys.shape, *page_table.shape)
         c = L.PagedCache()
         c.struct_size = C.sizeof(L.PagedCache)
         c.keys, c.values = _pointer("keys", keys, _F16, tuple(keys.shape)), _pointer("values", values, _F16, tuple(keys.shape))
@@ -59,6 +69,7 @@ class PagedCache:
 
     def scratch_bytes(self, n_head: int) -> int:
         """Bytes of scratch memory that attention and attention_prompt take, for any number of rows."""
+        _int32("n_head", n_head)
         n = L.lib().dooms_cuda_attention_paged_scratch_bytes(n_head, self._c.n_head_kv, self._c.head_dim)
         if n == 0:
             raise L.DoomsError(L.INVALID_ARGUMENT, f"{n_head} query heads on {self._c.n_head_kv} key / value heads of {self._c.head_dim}")
@@ -68,9 +79,11 @@ class PagedCache:
         """Rows [n][(n_head + 2 n_head_kv) head_dim] of f32 (rows may be further apart): turned queries into q [n][n_head][head_dim] (f32 or f16), turned keys and the values
         into position at[r] of sequence[r] (negative: an idle row). positions: int32 [n_axes][n]; sections: rotary pairs per axis (one axis: all of them)."""
         c, (n, n_head, head_dim) = self._c, q.shape
+        _int32("q", n, n_head)
         sections = (head_dim // 2,) if sections is None else tuple(sections)
         if not 1 <= len(sections) <= 4:
             raise L.DoomsError(L.INVALID_ARGUMENT, "sections: 1 to 4 axes")
+        _int32("sections", *sections)
         rope = self._ropes.get((base, neox, sections))      # (the argument struct: a program has one or two)
         if rope is None:
             rope = self._ropes[base, neox, sections] = L.Rope(C.sizeof(L.Rope), base, int(neox), len(sections), (C.c_int32 * 4)(*sections))
@@ -85,6 +98,8 @@ class PagedCache:
         """One new token per row: q, out [n][n_head][head_dim], both f32 or both f16; row r sees the first lengths[r] <= max_length positions of sequence[r]."""
         n, n_head = q.shape[0], q.shape[1]
         shape = (n, n_head, self._c.head_dim)
+        _int32("q", n, n_head)
+        max_length = max(-1, min(max_length, _MOST))      # (no sequence is longer; a larger bound means the same)
         L.check(L.lib().dooms_cuda_attention_paged(self._ref, _dtype("q", q), _pointer("q", q, q.dtype, shape), _pointer("sequence", sequence, _I32, (n,)),
                                                    _pointer("lengths", lengths, _I32, (n,)), max_length, _pointer("out", out, q.dtype, shape), n_head, n, scale,
                                                    *_scratch(scratch), _stream(stream)))
@@ -93,6 +108,7 @@ class PagedCache:
         """Packed prompts, causal: q, out f16 [rows][n_head][head_dim]; prompt i has rows start[i] .. start[i + 1] - 1, the last of lengths[i] positions of sequence[i]."""
         rows, n_head = q.shape[0], q.shape[1]
         shape, n = (rows, n_head, self._c.head_dim), sequence.shape[0]
+        _int32("q and sequence", rows, n_head, n)
         L.check(L.lib().dooms_cuda_attention_prompt_paged(self._ref, _pointer("q", q, _F16, shape), _pointer("sequence", sequence, _I32, (n,)),
                                                           _pointer("start", start, _I32, (n + 1,)), _pointer("lengths", lengths, _I32, (n,)),
                                                           _pointer("out", out, _F16, shape), n_head, n, rows, scale, *_scratch(scratch), _stream(stream)))
@@ -102,6 +118,7 @@ def sample_rows(logits, uniform, tokens, probability=None, temperature=None, top
     """tokens[r] (int32) from logits [rows][n] (f32; rows may be further apart) and uniform[r] in [0, 1); the filters are f32 (top_k: int32) tensors of one value per row, or
     None for off (temperature: 1). See dooms_cuda_sample_rows."""
     rows, n = logits.shape
+    _int32("logits", rows, n)
     if logits.dtype is not _F32 or (n > 1 and logits.stride(1) != 1):
         raise L.DoomsError(L.INVALID_ARGUMENT, "logits: rows of float32 expected")
 

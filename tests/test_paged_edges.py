@@ -117,6 +117,39 @@ def test_counters_are_zero_behind_a_call_and_behind_its_replays():
     assert status() == (L.OK, 0)
 
 
+# ---------------------------------------------------------------- numbers beyond 32 bits
+
+def test_the_python_face_refuses_sizes_beyond_32_bits():
+    """The C arguments would be their low 32 bits: a row of the first 100 logits, say."""
+    keys, ids, q = torch.zeros(4, 16, 2, 64, dtype=torch.float16), torch.zeros(3, dtype=torch.int32), torch.zeros(3, 4, 64)
+    cache = paged.PagedCache(keys, keys.clone(), torch.zeros(2, 2, dtype=torch.int32))
+    with pytest.raises(L.DoomsError, match="32 bits"):
+        paged.sample_rows(torch.empty(1, (1 << 32) + 100, device="meta"), torch.zeros(1), ids[:1])
+    with pytest.raises(L.DoomsError, match="32 bits"):
+        paged.PagedCache(keys, keys.clone(), torch.empty(1, (1 << 32) + 1, dtype=torch.int32, device="meta"))
+    with pytest.raises(L.DoomsError, match="32 bits"):
+        cache.rope_store(torch.zeros(3, 512), ids, ids, ids[None], q, 1e4, True, sections=[(1 << 32) + 32])
+    with pytest.raises(L.DoomsError, match="32 bits"):
+        cache.attention_prompt(q.half(), torch.empty(1 << 32, dtype=torch.int32, device="meta"), ids, ids, q.half(), torch.zeros(1))
+    with pytest.raises(L.DoomsError, match="32 bits"):
+        cache.scratch_bytes((1 << 32) + 4)
+
+
+def test_a_longest_length_beyond_32_bits_is_the_longest_there_is(monkeypatch):
+    seen = []
+
+    class Library:
+        def dooms_cuda_attention_paged(self, *args):
+            seen.append(args[5])
+            return L.OK
+    keys, ids, q = torch.zeros(4, 16, 2, 64, dtype=torch.float16), torch.zeros(3, dtype=torch.int32), torch.zeros(3, 4, 64)
+    cache = paged.PagedCache(keys, keys.clone(), torch.zeros(2, 2, dtype=torch.int32))
+    monkeypatch.setattr(L, "lib", Library)
+    for most in (0, 5, (1 << 31) - 1, 1 << 31, 1 << 32, 1 << 60, -1, -(1 << 33)):
+        cache.attention(q, ids, ids, most, q.clone(), torch.zeros(1))
+    assert seen == [0, 5] + [(1 << 31) - 1] * 4 + [-1, -1]
+
+
 # ---------------------------------------------------------------- streams
 
 def test_where_torch_has_no_gpu_the_default_stream_is_meant():
