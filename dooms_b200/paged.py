@@ -25,7 +25,7 @@ _MOST = (1 << 31) - 1
 
 
 def _int32(name: str, *values: int) -> None:
-    """That the values fit the C arguments, which would take the low 32 bits of one that does not."""
+    """That the values fit the C arguments, which would take the low 32 bits of one that does not. (Rows of queries need no such check: 2^31 of them fit no GPU.)"""
     if not all(-_MOST <= v <= _MOST for v in values):
         raise L.DoomsError(L.INVALID_ARGUMENT, f"{name}: {values} does not fit 32 bits")
 
@@ -79,13 +79,12 @@ class PagedCache:
         """Rows [n][(n_head + 2 n_head_kv) head_dim] of f32 (rows may be further apart): turned queries into q [n][n_head][head_dim] (f32 or f16), turned keys and the values
         into position at[r] of sequence[r] (negative: an idle row). positions: int32 [n_axes][n]; sections: rotary pairs per axis (one axis: all of them)."""
         c, (n, n_head, head_dim) = self._c, q.shape
-        _int32("q", n, n_head)
         sections = (head_dim // 2,) if sections is None else tuple(sections)
         if not 1 <= len(sections) <= 4:
             raise L.DoomsError(L.INVALID_ARGUMENT, "sections: 1 to 4 axes")
-        _int32("sections", *sections)
         rope = self._ropes.get((base, neox, sections))      # (the argument struct: a program has one or two)
         if rope is None:
+            _int32("sections", *sections)
             rope = self._ropes[base, neox, sections] = L.Rope(C.sizeof(L.Rope), base, int(neox), len(sections), (C.c_int32 * 4)(*sections))
         if qkv.dtype is not _F32 or tuple(qkv.shape) != (n, (n_head + 2 * c.n_head_kv) * head_dim) or qkv.stride(1) != 1:
             raise L.DoomsError(L.INVALID_ARGUMENT, f"qkv: float32 rows of {(n_head + 2 * c.n_head_kv) * head_dim} values expected, one for each of the {n} rows of q")
@@ -98,8 +97,8 @@ class PagedCache:
         """One new token per row: q, out [n][n_head][head_dim], both f32 or both f16; row r sees the first lengths[r] <= max_length positions of sequence[r]."""
         n, n_head = q.shape[0], q.shape[1]
         shape = (n, n_head, self._c.head_dim)
-        _int32("q", n, n_head)
-        max_length = max(-1, min(max_length, _MOST))      # (no sequence is longer; a larger bound means the same)
+        if not 0 <= max_length <= _MOST:      # (no sequence is longer; a larger bound means the same)
+            max_length = max(-1, min(max_length, _MOST))
         L.check(L.lib().dooms_cuda_attention_paged(self._ref, _dtype("q", q), _pointer("q", q, q.dtype, shape), _pointer("sequence", sequence, _I32, (n,)),
                                                    _pointer("lengths", lengths, _I32, (n,)), max_length, _pointer("out", out, q.dtype, shape), n_head, n, scale,
                                                    *_scratch(scratch), _stream(stream)))
@@ -108,7 +107,8 @@ class PagedCache:
         """Packed prompts, causal: q, out f16 [rows][n_head][head_dim]; prompt i has rows start[i] .. start[i + 1] - 1, the last of lengths[i] positions of sequence[i]."""
         rows, n_head = q.shape[0], q.shape[1]
         shape, n = (rows, n_head, self._c.head_dim), sequence.shape[0]
-        _int32("q and sequence", rows, n_head, n)
+        if n > _MOST:
+            _int32("sequence", n)
         L.check(L.lib().dooms_cuda_attention_prompt_paged(self._ref, _pointer("q", q, _F16, shape), _pointer("sequence", sequence, _I32, (n,)),
                                                           _pointer("start", start, _I32, (n + 1,)), _pointer("lengths", lengths, _I32, (n,)),
                                                           _pointer("out", out, _F16, shape), n_head, n, rows, scale, *_scratch(scratch), _stream(stream)))
@@ -118,7 +118,8 @@ def sample_rows(logits, uniform, tokens, probability=None, temperature=None, top
     """tokens[r] (int32) from logits [rows][n] (f32; rows may be further apart) and uniform[r] in [0, 1); the filters are f32 (top_k: int32) tensors of one value per row, or
     None for off (temperature: 1). See dooms_cuda_sample_rows."""
     rows, n = logits.shape
-    _int32("logits", rows, n)
+    if rows > _MOST or n > _MOST:
+        _int32("logits", rows, n)
     if logits.dtype is not _F32 or (n > 1 and logits.stride(1) != 1):
         raise L.DoomsError(L.INVALID_ARGUMENT, "logits: rows of float32 expected")
 
