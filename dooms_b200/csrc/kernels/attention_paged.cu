@@ -11,10 +11,11 @@
 //
 // The G query heads are the eight columns (G > 8: twice eight; more than 16 are several items) of m16n8k16 MMAs, S^T = K Q^T and O^T = V^T P^T, f16 operands, f32
 // accumulators: keys and values are their 16-row operands, so that no row is spent on heads that are not there (with the heads as rows a step was twice the
-// MMAs, and heads of 128 spilled: 118 against 100 us for one row of 131071 keys). With f32 queries, query and probabilities enter as f16
-// value + f16 rounding error (2^-22 together), the query after its row was scaled by a power of two, and each tile's products are added to the outputs in f32
-// (round to nearest; the tensor core's own accumulation truncates): as exact as f32 arithmetic. Probabilities are kept times 2^10, so that their second part
-// stays in f16's normal range.
+// MMAs, and heads of 128 spilled: 118 against 100 us for one row of 131071 keys). Probabilities enter as f16 value + f16 rest (2^-22 together), with
+// f32 queries the query too, after its row was scaled by a power of two, and each tile's products are added to the outputs in f32 (round to nearest; the tensor
+// core's own accumulation truncates): as exact as f32 arithmetic. Probabilities are kept times 2^10, so that their second part stays in f16's normal range. (With one
+// f16 probability for f16 rows their error against 64 bits was 2.5e-4 where the rounding of the result alone is 2.1e-4. The second product costs nothing at 4 or 5
+// heads per key / value head, 1 us at 16 of 64, and 199 against 180 us at 256 rows of 32 to 4096 keys of 64 heads on one.)
 #include <cuda.h>
 #include <math_constants.h>
 
@@ -71,14 +72,12 @@ __device__ __forceinline__ uint32_t transposed(uint32_t v) {
     return r;
 }
 __device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
-// (a, b) as f16 pairs; `rest`: what the rounding left, rounded to f16 too
+// (a, b) as f16 pairs; *rest: what the rounding left, rounded to f16 too
 __device__ __forceinline__ uint32_t split2(float a, float b, uint32_t * rest) {
     const __half2 h = __floats2half2_rn(a, b);
-    if (rest) {
-        const float2 f = __half22float2(h);
-        const __half2 r = __floats2half2_rn(a - f.x, b - f.y);
-        *rest = *reinterpret_cast<const uint32_t *>(&r);
-    }
+    const float2 f = __half22float2(h);
+    const __half2 r = __floats2half2_rn(a - f.x, b - f.y);
+    *rest = *reinterpret_cast<const uint32_t *>(&r);
     return *reinterpret_cast<const uint32_t *>(&h);
 }
 
@@ -396,9 +395,9 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) k_attention_paged(cons
                         #pragma unroll
                         for (int i = 0; i < 2; i++) {
                             uint32_t low = 0;
-                            const uint32_t high = HALF ? split2(x[2 * i], x[2 * i + 1], nullptr) : split_p(x[2 * i], x[2 * i + 1], &low);
+                            const uint32_t high = split_p(x[2 * i], x[2 * i + 1], &low);
                             ph[e][i] = transposed(high);
-                            if (!HALF) pl[e][i] = transposed(low);
+                            pl[e][i] = transposed(low);
                         }
                     }
                     #pragma unroll
@@ -409,7 +408,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) k_attention_paged(cons
                         for (int e = 0; e < K::NT; e++) {
                             float c[4] = {0.f, 0.f, 0.f, 0.f};
                             mma_f16(c, v, ph[e][0], ph[e][1]);
-                            if (!HALF) mma_f16(c, v, pl[e][0], pl[e][1]);
+                            mma_f16(c, v, pl[e][0], pl[e][1]);
                             #pragma unroll
                             for (int i = 0; i < 4; i++) o[e][j][i] = fmaf(o[e][j][i], keep[e][i % 2], c[i]);
                         }

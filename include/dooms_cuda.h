@@ -281,7 +281,7 @@ DOOMS_CUDA_API int32_t dooms_cuda_rope_store_paged(const dooms_cuda_paged_cache 
 DOOMS_CUDA_API int64_t dooms_cuda_attention_paged_scratch_bytes(int32_t n_head, int32_t n_head_kv, int32_t head_dim);
 /* attention_split + attention_combine (llama_kernels.h:860-929) for one new token of each of many sequences: row r of d_q [n_rows][n_head][head_dim] (turned) attends to
  * the first d_lengths[r] positions of sequence d_sequence[r] (negative: an idle row, whose output is left as it is; length 0: zeros). d_q and d_out: dtype DOOMS_F32 or
- * DOOMS_F16, 16-byte aligned, apart from one another and from the scratch; with f32 the products are as exact as f32 arithmetic (an infinite
+ * DOOMS_F16, 16-byte aligned, apart from one another and from the scratch; the arithmetic is as exact as f32's with either (an infinite
  * key among those seen gives NaN, though). max_length: at least every length (a longer one is out of range); it may be generous.
  * scale: of the scores; 0: 1 / sqrt(head_dim). */
 DOOMS_CUDA_API int32_t dooms_cuda_attention_paged(const dooms_cuda_paged_cache * cache, int32_t dtype, const void * d_q, const int32_t * d_sequence, const int32_t * d_lengths,

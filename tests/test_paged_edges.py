@@ -13,7 +13,7 @@ import torch
 from dooms_b200 import _lib as L
 from dooms_b200 import build as B
 from dooms_b200 import paged
-from test_paged import Cache, attention_code, chain, check_sample, cuda, fake_cache, fake_rope, prompt_code, sample_code, status, store_code
+from test_paged import HALF, Cache, attend, attention_code, bound, chain, check_sample, cuda, fake_cache, fake_rope, prompt_code, sample_code, status, store_code
 
 gpu = pytest.mark.gpu
 HERE = Path(__file__).resolve().parent
@@ -49,6 +49,27 @@ def test_what_follows_the_sampling_sees_its_tokens(probes, rows, n):
         assert probes.probe_copy_at_once(tokens.data_ptr(), seen.data_ptr(), rows, stream.cuda_stream) == 0
         torch.cuda.synchronize()
         assert (tokens >= 0).all() and torch.equal(tokens, seen)
+
+
+# ---------------------------------------------------------------- one token in f16
+
+@gpu
+@pytest.mark.parametrize("heads, head_dim", [((14, 2), 64), ((32, 8), 128), ((16, 1), 64), ((40, 2), 128)])
+def test_f16_rows_of_one_token_are_rounded_once(heads, head_dim):
+    """Queries, keys and values are f16 numbers, and what happens between them and the result is f32 arithmetic: the bound of f32 rows and half a step of the result (2^-11 of it,
+    2^-25 where it is subnormal). A probability of f16 would be half a step of every product, 2^-11 of their sum."""
+    (H, K), D = heads, head_dim
+    lengths = [1, 2, 17, 63, 64, 65, 300, 2000, 9000]
+    cache = Cache(lengths, K, D, 16, seed=5)
+    q = np.random.default_rng(6).standard_normal((len(lengths), H, D)).astype(np.float16)
+    out = torch.zeros(len(lengths), H, D, dtype=torch.float16, device="cuda")
+    cache.cache.attention(cuda(q), torch.arange(len(lengths), dtype=torch.int32, device="cuda"), cuda(np.array(lengths, np.int32)), max(lengths), out, cache.scratch(H))
+    assert status() == (L.OK, 0)
+    s = 1 / np.sqrt(D)
+    for r, n in enumerate(lengths):
+        want, mass, reach = attend(q[r].astype(np.float64), *cache.sequence(r, n), s)
+        tol = bound(want, mass, reach, D, s, False) + np.abs(want) * HALF + 2.0 ** -25
+        assert (np.abs(out[r].cpu().numpy().astype(np.float64) - want) <= tol).all(), n
 
 
 # ---------------------------------------------------------------- sampling
