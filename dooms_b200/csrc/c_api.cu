@@ -173,6 +173,7 @@ struct SetUpUnderCapture {
 struct Span {
     const void * at;
     int64_t bytes, rows = 1, stride = 0;
+    bool device_only = false;      // tensor copies read it, or blocks count in it: neither is tried on memory of the host or on pages that migrate
     // Whether it has a byte in common with `other`, which has one row.
     bool meets(const Span & other) const {
         if (!at || !other.at || bytes <= 0 || other.bytes <= 0) return false;
@@ -209,8 +210,10 @@ int32_t check_memory(const char * what, std::initializer_list<Span> written, std
             cudaPointerAttributes at{};
             const cudaError_t e = cudaPointerGetAttributes(&at, s.at);
             if (e != cudaSuccess) { (void)cudaGetLastError(); return fail(DOOMS_UNSUPPORTED, std::string(what) + ": " + cudaGetErrorString(e)); }
-            const bool here = at.type == cudaMemoryTypeManaged || (at.type == cudaMemoryTypeDevice && at.device == dev) || (at.type == cudaMemoryTypeHost && at.devicePointer == s.at);
+            const bool device = at.type == cudaMemoryTypeDevice && at.device == dev;
+            const bool here = device || at.type == cudaMemoryTypeManaged || (at.type == cudaMemoryTypeHost && at.devicePointer == s.at);
             if (!here) return fail(DOOMS_INVALID_ARGUMENT, std::string(what) + ": a pointer is not memory of the current device");
+            if (s.device_only && !device) return fail(DOOMS_INVALID_ARGUMENT, std::string(what) + ": pools, scratch and queries of prompts have to be device memory, not managed or mapped");
         }
     }
     return DOOMS_OK;
@@ -218,7 +221,8 @@ int32_t check_memory(const char * what, std::initializer_list<Span> written, std
 
 bool aligned16(const void * p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
-Span pool_of(const void * at, const cuda::PagedCache & c) { return {at, int64_t(c.n_pages) * c.page_size * c.n_head_kv * c.head_dim * 2}; }
+Span device_span(const void * at, int64_t bytes) { return {at, bytes, 1, 0, true}; }
+Span pool_of(const void * at, const cuda::PagedCache & c) { return device_span(at, int64_t(c.n_pages) * c.page_size * c.n_head_kv * c.head_dim * 2); }
 Span table_of(const cuda::PagedCache & c) { return {c.page_table, int64_t(c.n_sequences) * c.max_pages * 4}; }
 
 // Out-of-range entries and waits that run out are only known by the error word, so nothing is launched without one.
@@ -1004,7 +1008,7 @@ DOOMS_CUDA_API int32_t dooms_cuda_attention_paged(const dooms_cuda_paged_cache *
     if (scratch_bytes < needed) return fail(DOOMS_RESOURCE_EXHAUSTED, "attention_paged: the scratch is too small");
     const SetUpUnderCapture relaxed;
     const int64_t each = int64_t(n_rows) * 4;
-    code = check_memory("attention_paged", {{d_out, io}, {d_scratch, needed}},
+    code = check_memory("attention_paged", {{d_out, io}, device_span(d_scratch, needed)},
                         {{d_q, io}, pool_of(c.keys, c), pool_of(c.values, c), table_of(c), {d_sequence, each}, {d_lengths, each}});
     if (code != DOOMS_OK) return code;
     int32_t * const err = kernel_error_word();
@@ -1029,8 +1033,8 @@ DOOMS_CUDA_API int32_t dooms_cuda_attention_prompt_paged(const dooms_cuda_paged_
     if (scratch_bytes < needed) return fail(DOOMS_RESOURCE_EXHAUSTED, "attention_prompt_paged: the scratch is too small");
     const SetUpUnderCapture relaxed;
     const int64_t each = int64_t(n_prompts) * 4;
-    code = check_memory("attention_prompt_paged", {{d_out, io}, {d_scratch, needed}},
-                        {{d_q, io}, pool_of(c.keys, c), pool_of(c.values, c), table_of(c), {d_sequence, each}, {d_lengths, each}, {d_start, each + 4}});
+    code = check_memory("attention_prompt_paged", {{d_out, io}, device_span(d_scratch, needed)},
+                        {device_span(d_q, io), pool_of(c.keys, c), pool_of(c.values, c), table_of(c), {d_sequence, each}, {d_lengths, each}, {d_start, each + 4}});
     if (code != DOOMS_OK) return code;
     int32_t * const err = kernel_error_word();
     if (!err) return no_error_word("attention_prompt_paged");

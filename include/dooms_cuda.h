@@ -246,7 +246,7 @@ DOOMS_CUDA_API int32_t dooms_cuda_attention_decode(const float * d_q, const void
 
 /* ---- The parts of a serving step over a key / value cache in pages, on DEVICE pointers like the single kernels above. No counterpart in the reference, which
  * keeps one contiguous cache (metal_llama_decoder.mm:560-590) and samples on the host (src/models/vlm/text_decoder.cpp:231-246).
- * Every pointer is memory of the current device (or managed, or mapped host memory); anything else is refused with DOOMS_INVALID_ARGUMENT before a launch, as
+ * Every pointer is memory of the current device (or managed, or mapped host memory, but for pools, scratch and the queries of prompts); anything else is refused with DOOMS_INVALID_ARGUMENT before a launch, as
  * are NULL pointers, bad sizes, and memory that a call writes where it overlaps memory that it reads, or that it writes besides (outputs, scratch, the pools in rope_store). What only the device can read (page ids, sequences, positions, lengths) is checked there: an entry that is out of range is
  * not followed, its row's output is not valid, and dooms_cuda_kernel_status then reports flag 8. Calls allocate nothing and may be captured. Calls that
  * overlap on the GPU need scratch memory of their own; a scratch needs no initialization. ---- */

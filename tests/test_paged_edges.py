@@ -360,6 +360,29 @@ def test_tokens_behind_each_row_of_logits():
         paged.sample_rows(buffer[:, :n], cuda(u), buffer[3, n - rows:n].view(torch.int32))
 
 
+@gpu
+def test_pools_scratch_and_queries_of_prompts_are_device_memory():
+    """Mapped host memory serves for what the kernels read with plain loads; what tensor copies read, and what blocks count in, is refused there."""
+    H, K, D = 4, 2, 64
+    cache = Cache([40, 20], K, D, 16)
+    scratch, seq, lengths = cache.scratch(H), torch.arange(2, dtype=torch.int32, device="cuda"), cuda(np.array([40, 20], np.int32))
+    q, start = torch.randn(2, H, D, device="cuda"), torch.arange(3, dtype=torch.int32, device="cuda")
+    out, want = torch.zeros_like(q), torch.zeros_like(q)
+    pinned = lambda t: t.cpu().pin_memory()  # noqa: E731
+    cache.cache.attention(q, seq, lengths, 40, want, scratch)
+    cache.cache.attention(pinned(q), pinned(seq), pinned(lengths), 40, out, scratch)
+    torch.cuda.synchronize()
+    assert torch.equal(out, want) and status() == (L.OK, 0)
+    pools = paged.PagedCache(pinned(cache.keys), pinned(cache.values), cache.d_table)
+    pout = torch.zeros_like(q).half()
+    for call in (lambda: pools.attention(q, seq, lengths, 40, out, scratch), lambda: cache.cache.attention(q, seq, lengths, 40, out, pinned(scratch)),
+                 lambda: pools.attention_prompt(q.half(), seq, start, lengths, pout, scratch), lambda: cache.cache.attention_prompt(pinned(q.half()), seq, start, lengths, pout, scratch),
+                 lambda: pools.rope_store(torch.zeros(2, 8 * D, device="cuda"), seq, lengths - 1, lengths[None], torch.zeros_like(q), 1e4, True)):
+        with pytest.raises(L.DoomsError, match="device memory"):
+            call()
+    assert status() == (L.OK, 0)
+
+
 # ---------------------------------------------------------------- the error word
 
 @gpu
