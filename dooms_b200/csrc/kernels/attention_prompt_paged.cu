@@ -17,8 +17,9 @@
 // outputs, maxima, sums), and the first, which has its beginning last, adds that to what it has in tensor memory. Where the second has not come within a millisecond (it
 // may be waiting for an SM), the first leaves its part too. Of more than two blocks each leaves its part. The last to arrive joins the parts
 // in the order of the blocks. (With a part and a join for two as well four pieces of 300 to 512 took 127 us.)
-// B200: 8192 queries of 40 / 8 heads of 128 in 651 us (1060 TFLOP/s, 770 us when the GPU's power limit holds), four pieces of 300 to 512 behind 6000 keys (32 / 8 heads) in
-// 120 (138): a tile's step is a chain of scores, softmax and weighted sum of 3500 cycles, in which the tensor core works 2048 for both tiles.
+// B200: 8192 queries of 40 / 8 heads of 128 in 760 us (905 TFLOP/s at the 1657 MHz that the power limit leaves; 690 in short runs), four pieces of 300 to 512 behind 1900
+// to 4400 keys (32 / 8 heads) in 138 (760 TFLOP/s, 1740 MHz). A pair of steps, one of each tile, takes 4340 cycles of the first (whole time x clock / steps, units' begins
+// and ends included) and 5180 of the second; each step more of a unit 4100 to 4500. It is a chain of scores, softmax and weighted sum, and the tensor core works 2048 cycles of it.
 // Queries and probabilities are f16 (the type queries come in; a probability's rounding is 2^-12 of it on average, the outputs' own rounding the same again),
 // scores, sums and outputs f32.
 #include <cuda.h>
@@ -44,8 +45,9 @@ constexpr int kUnitCost = 256;              // what a unit costs besides its key
 constexpr int kShortestSpan = kUnitCost + kRows;      // of the line, per block: a block inside a cut unit has at least two whole tiles
 // Where no unit has more than kUncutTiles key tiles none is cut, and a block takes the units that are kUnitCost + kHalf or more inside the line of it: spans that are shorter
 // than any unit leave a block one at most. A cut costs 5 to 10 us, which is the work of three to six tiles. Never cut / cut, in us: 8B shape, 1 x 200 queries 17.7 / 28.5,
-// 1 x 1000 28.9 / 35, 4 x 64 behind 700 keys 24 / 28, 40 x 120 43 / 42, 16 x 16 behind 900 33 / 29; 0.5B, 30 x 36 behind 200 14 / 28. One unit per block at most
-// instead of spans of 384, where no unit has two tiles: 24 questions 13.0 against 15.6.
+// 1 x 1000 28.9 / 35, 4 x 64 behind 700 keys 24 / 28, 40 x 120 43 / 42, 16 x 16 behind 900 33 / 29; 0.5B, 30 x 36 behind 200
+// 14 / 28. (Two of the six are faster cut. The rule looks at the batch's longest unit alone: one prompt of 1025 keys has every unit cut where it falls.) One unit per block
+// at most instead of spans of 384, where no unit has two tiles: 24 questions 13.0 against 15.6.
 constexpr int kSpanUncut = 192, kUncutTiles = 8;
 constexpr float kRescale = 8.f;             // log2 of the growth of a maximum that is let be
 constexpr float kLift = 6.f;                // probabilities are kept times 2^kLift: those of 2^-20 are still normal f16 values, and 2^(kLift + kRescale) is one

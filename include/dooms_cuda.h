@@ -301,7 +301,7 @@ DOOMS_CUDA_API int32_t dooms_cuda_attention_prompt_paged(const dooms_cuda_paged_
  * d_temperature[r] exceeds d_uniform[r]. At least one token, the first, is kept (a min-p above 1 keeps it
  * alone). temperature <= 0: the largest logit. A NaN is never picked, nor a logit of -inf; a row that has
  * nothing else gives its first number (0: none) with probability 0. NULL: temperature 1, top-k, top-p and min-p off. d_probability (may be NULL): the token's
- * probability among those kept. n at most 262144. */
+ * probability among those kept. n at most 262144. Rows that do not begin on 16 bytes (a stride that is no multiple of 4) take up to twice as long. */
 DOOMS_CUDA_API int32_t dooms_cuda_sample_rows(const float * d_logits, int64_t stride, int32_t rows, int32_t n, const float * d_temperature, const int32_t * d_top_k,
                                               const float * d_top_p, const float * d_min_p, const float * d_uniform, int32_t * d_tokens, float * d_probability, void * stream);
 
