@@ -268,7 +268,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) k_attention_paged(cons
             if (left > 0) next_item();
         }
         rows_without(lane, 32);
-        // no copy is under way when the block ends, not behind a wait that ran out either: each stage's last one (of this round in front of `stage`, of the round before from there on)
+        // no copy is under way when the block ends, not behind a wait that ran out either: each stage's last one (of this turn of the ring in front of `stage`, of the turn before from there on)
         for (int s = 0; s < K::kStages; s++) ok = mbar_wait(full + 8 * s, s < stage ? phase : phase ^ 1u) && ok;
     } else {
         const int g = lane >> 2, t = lane & 3;
